@@ -1,0 +1,584 @@
+// MI355X (gfx950) operations on the pages of an INT8 cache pool: accepted
+// paths of drafted tokens, forked and freed rows of a block table, compaction.
+// The argument blocks and their rules are in sharedkv_hip.h.
+//
+// None of these computes; each is bound by the bytes it moves (whole pages and
+// rows, 16 bytes a lane) and, where these are few, by its chain of dependent
+// reads.  Which page goes where follows from counts: the k-th free or moving
+// page in index order, found with prefix sums over chunks of the reference
+// counts, so the result does not depend on the order in which work-groups run.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "sharedkv_hip.h"
+
+namespace {
+
+constexpr int THREADS = 256;
+constexpr int WAVES = THREADS / 64;
+constexpr int PER_THREAD = 8;
+constexpr int CHUNK = THREADS * PER_THREAD;     // pages whose counts one work-group takes
+constexpr int MAX_CHUNKS = 2048;
+constexpr int64_t MAX_PAGES = (int64_t)CHUNK * MAX_CHUNKS;
+constexpr int PATH = 64;                        // path entries that are resident at once
+constexpr int64_t SLICE = 32768;                // bytes of a page that one work-group copies
+constexpr int WANTED = -2;                      // a staged entry that gets a free page
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+template <typename T>
+__device__ __forceinline__ const __attribute__((address_space(1))) T *gptr(uint64_t a)
+{
+    return reinterpret_cast<const __attribute__((address_space(1))) T *>(a);
+}
+template <typename T>
+__device__ __forceinline__ __attribute__((address_space(1))) T *gout(uint64_t a)
+{
+    return reinterpret_cast<__attribute__((address_space(1))) T *>(a);
+}
+
+// Sum over the work-group, in every thread.
+__device__ __forceinline__ int block_sum(int v)
+{
+    __shared__ int part[WAVES];
+#pragma unroll
+    for (int step = 32; step; step /= 2) v += __shfl_xor(v, step);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+    __syncthreads();
+    int total = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) total += part[w];
+    return total;
+}
+
+// Sum over the threads before this one; `total` gets the whole.
+__device__ __forceinline__ int block_before(int v, int &total)
+{
+    __shared__ int part[WAVES];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int upto = v;
+#pragma unroll
+    for (int step = 1; step < 64; step *= 2) {
+        const int other = __shfl_up(upto, step);
+        if (lane >= step) upto += other;
+    }
+    __syncthreads();
+    if (lane == 63) part[wave] = upto;
+    __syncthreads();
+    total = 0;
+    int before = upto - v;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+        if (w < wave) before += part[w];
+        total += part[w];
+    }
+    return before;
+}
+
+// Bytes [first, last) of page `from` to page `to`, over the caches one after
+// another (all multiples of 16).
+__device__ __forceinline__ void copy_page(uint64_t caches, uint32_t count, int64_t from, int64_t to, int64_t first,
+                                          int64_t last)
+{
+    const auto *span = gptr<CacheSpan>(caches);
+    int64_t at = 0;
+    for (uint32_t c = 0; c < count && at < last; ++c) {
+        const int64_t bytes = (int64_t)span[c].bytes;
+        const int64_t lo = first > at ? first - at : 0, hi = last - at < bytes ? last - at : bytes;
+        if (lo < hi) {
+            const auto *src = gptr<u32x4>(span[c].base + (uint64_t)from * span[c].pageStride);
+            auto *dst = gout<u32x4>(span[c].base + (uint64_t)to * span[c].pageStride);
+            const int64_t end = hi / 16;
+            int64_t i = lo / 16 + threadIdx.x;
+            for (; i + 3 * THREADS < end; i += 4 * THREADS) {
+                u32x4 v[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] = src[i + k * THREADS];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) dst[i + k * THREADS] = v[k];
+            }
+            for (; i < end; i += THREADS) dst[i] = src[i];
+        }
+        at += bytes;
+    }
+}
+
+// ------------------------------------------------------------ accepted paths
+
+// One work-group moves a 16-byte column per thread through a request's path:
+// a thread reads a few entries ahead of its writes, which never reach a row
+// that it still has to read (paths[k] >= k and rises).
+constexpr int AHEAD = 8;
+__global__ void __launch_bounds__(THREADS) path_commit(const PathCommitArgs p)
+{
+    __shared__ int32_t place[PATH][4];           // page (-1: no move) and row of source and target
+    __shared__ int kept;
+    const int tid = threadIdx.x, b = (int)blockIdx.x;
+    const int tokens = (int)p.tokens;
+    const int first = min(max(gptr<int32_t>(p.cuQ)[b], 0), tokens);
+    const int nodes = min(max(gptr<int32_t>(p.cuQ)[b + 1], first), tokens) - first;
+    const int length = gptr<int32_t>(p.seqLens)[b];
+    const int most = length > 0 ? min(max(gptr<int32_t>(p.pathLens)[b], 0), (int)p.depth) : 0;
+    const int committed = max(0, length - nodes);
+    const uint32_t columns = p.rowBytes / 16, item = blockIdx.y * THREADS + tid;
+    const uint32_t cache = item / columns, column = item % columns;
+    CacheSpan span = {};
+    if (cache < p.cacheCount) {
+        const auto *from = gptr<CacheSpan>(p.caches) + cache;
+        span.base = from->base, span.pageStride = from->pageStride, span.rowStride = from->rowStride, span.bytes = from->bytes;
+    }
+    const bool mine = cache < p.cacheCount && column * 16 < span.bytes;
+    const auto *path = gptr<int32_t>(p.paths) + (int64_t)b * p.depth;
+    int done = 0;
+    for (int at = 0; at < most; at += PATH) {
+        __syncthreads();
+        if (tid < 64) {
+            const int k = at + tid;
+            const int node = k < most ? path[k] : -1, before = k > 0 && k < most ? path[k - 1] : -1;
+            const bool good = k < most && node > before && node < nodes;
+            const uint64_t bad = __ballot(!good);
+            const int n = bad ? __builtin_ctzll(bad) : 64;
+            if (tid == 0) kept = n;
+            int32_t page[2] = {-1, -1}, row[2] = {0, 0};
+            if (tid < n && node != k) {
+#pragma unroll
+                for (int side = 0; side < 2; ++side) {
+                    const int64_t at_row = (int64_t)committed + (side ? k : node);
+                    const int64_t e = at_row / p.pageRows;
+                    page[side] = e < p.tableWidth ? gptr<int32_t>(p.table)[(int64_t)b * p.tableWidth + e] : -1;
+                    row[side] = (int32_t)(at_row % p.pageRows);
+                }
+            }
+            const bool moves = (uint32_t)page[0] < p.pages && (uint32_t)page[1] < p.pages;
+            place[tid][0] = moves ? page[0] : -1;
+            place[tid][1] = row[0];
+            place[tid][2] = page[1];
+            place[tid][3] = row[1];
+        }
+        __syncthreads();
+        const int n = kept;
+        done += n;
+        if (mine) {
+            for (int k = 0; k < n; k += AHEAD) {
+                u32x4 v[AHEAD];
+#pragma unroll
+                for (int i = 0; i < AHEAD; ++i)
+                    if (k + i < n && place[k + i][0] >= 0)
+                        v[i] = gptr<u32x4>(span.base + (uint64_t)place[k + i][0] * span.pageStride +
+                                           (uint64_t)place[k + i][1] * span.rowStride)[column];
+#pragma unroll
+                for (int i = 0; i < AHEAD; ++i)
+                    if (k + i < n && place[k + i][0] >= 0)
+                        gout<u32x4>(span.base + (uint64_t)place[k + i][2] * span.pageStride +
+                                    (uint64_t)place[k + i][3] * span.rowStride)[column] = v[i];
+            }
+        }
+        if (n < PATH) break;
+    }
+    if (blockIdx.y == 0 && tid == 0)
+        reinterpret_cast<int32_t *>(p.lengths)[b] = length > 0 ? committed + done : 0;
+}
+
+// ------------------------------------------------------------ fork
+
+struct ForkSpace {
+    int32_t *staged;       // [children][width] new entries, WANTED where a free page comes
+    int32_t *source;       // [children] page of the parent's partly filled entry
+    int32_t *need;         // [children] free pages wanted
+    int32_t *length;       // [children] the parent's length
+    int32_t *freed;        // [chunks][CHUNK] the chunk's free pages, in order
+    int32_t *count;        // [chunks] how many there are
+    int32_t *delta;        // [pages] change of the reference counts; zero between launches
+};
+__host__ __device__ inline uint32_t chunks_of(uint32_t pages) { return (pages + CHUNK - 1) / CHUNK; }
+__host__ __device__ inline uint64_t fork_words(uint32_t children, uint32_t width, uint32_t pages)
+{
+    const uint64_t chunks = chunks_of(pages);
+    return (uint64_t)pages + (uint64_t)children * (width + 3) + chunks * (CHUNK + 1);
+}
+__device__ __forceinline__ ForkSpace fork_space(const PageForkArgs &p)
+{
+    ForkSpace w;
+    w.delta = reinterpret_cast<int32_t *>(p.workspace);
+    w.staged = w.delta + p.pages;
+    w.source = w.staged + (int64_t)p.children * p.width;
+    w.need = w.source + p.children;
+    w.length = w.need + p.children;
+    w.count = w.length + p.children;
+    w.freed = w.count + chunks_of(p.pages);
+    return w;
+}
+
+// A row's length and what follows from it: whole pages, pages with room.
+struct Extent {
+    int32_t length, whole, needed;
+};
+__device__ __forceinline__ Extent extent_of(const PageForkArgs &p, int row)
+{
+    const int64_t most = (int64_t)p.width * p.pageRows;
+    const int64_t length = min(max((int64_t)gptr<int32_t>(p.seqLens)[row], (int64_t)0), min(most, (int64_t)0x7fffffff));
+    Extent x;
+    x.length = (int32_t)length;
+    x.whole = (int32_t)(length / p.pageRows);
+    x.needed = (int32_t)min((int64_t)p.width, (length + p.room + p.pageRows - 1) / p.pageRows);
+    return x;
+}
+
+// Children matching `row`, among the first `upto`.
+__device__ __forceinline__ int children_of(const PageForkArgs &p, int row, int upto)
+{
+    int n = 0;
+    for (int i = threadIdx.x; i < upto; i += THREADS) n += gptr<int32_t>(p.parents)[i] == row;
+    return block_sum(n);
+}
+
+// Work-groups: the new rows (staged entries, free pages wanted), the old rows
+// (reference counts), the chunks of pages (free pages).
+__global__ void __launch_bounds__(THREADS) fork_plan(const PageForkArgs p)
+{
+    const ForkSpace w = fork_space(p);
+    const int tid = threadIdx.x;
+    const auto *refs = gptr<int32_t>(p.refs), *table = gptr<int32_t>(p.table);
+    uint32_t at = blockIdx.x;
+    if (at < p.children) {
+        const int parent = gptr<int32_t>(p.parents)[at];
+        const bool alive = (uint32_t)parent < p.rows;
+        Extent x = {};
+        if (alive) x = extent_of(p, parent);
+        const bool first = alive && children_of(p, parent, (int)at) == 0;
+        int wanted = 0;
+        for (int e = tid; e < (int)p.width; e += THREADS) {
+            const int old = alive && e < x.needed ? table[(int64_t)parent * p.width + e] : -1;
+            const bool good = (uint32_t)old < p.pages;
+            int entry = -1;
+            if (e < x.whole) entry = good ? old : -1;
+            else if (e < x.needed) {
+                entry = first && good && refs[old] == 1 ? old : WANTED;
+                wanted += entry == WANTED;
+            }
+            w.staged[(int64_t)at * p.width + e] = entry;
+            if (e == x.whole) w.source[at] = good ? old : -1;
+        }
+        wanted = block_sum(wanted);
+        if (tid == 0) w.need[at] = wanted, w.length[at] = x.length;
+        return;
+    }
+    at -= p.children;
+    if (at < p.rows) {
+        const int children = children_of(p, (int)at, (int)p.children);
+        const Extent x = extent_of(p, (int)at);
+        for (int e = tid; e < (int)p.width; e += THREADS) {
+            const int old = table[(int64_t)at * p.width + e];
+            if ((uint32_t)old >= p.pages) continue;
+            const int held = e < x.whole ? children : children && e < x.needed && refs[old] == 1 ? 1 : 0;
+            if (held != 1) atomicAdd(&w.delta[old], held - 1);
+        }
+        return;
+    }
+    at -= p.rows;
+    const int64_t page = (int64_t)at * CHUNK + tid * PER_THREAD;
+    bool spare[PER_THREAD];
+    int mine = 0;
+#pragma unroll
+    for (int i = 0; i < PER_THREAD; ++i) {
+        spare[i] = page + i < p.pages && refs[page + i] == 0;
+        mine += spare[i];
+    }
+    int total, rank = block_before(mine, total);
+#pragma unroll
+    for (int i = 0; i < PER_THREAD; ++i)
+        if (spare[i]) w.freed[(int64_t)at * CHUNK + rank++] = (int32_t)(page + i);
+    if (tid == 0) w.count[at] = total;
+}
+
+// Work-groups: slices of the new rows (the first writes the row, all copy its
+// partly filled page), then the chunks of pages (reference counts).  The old
+// table, lengths and counts may be the new ones: rows come from the workspace
+// and a page's count is read by the thread that writes it.
+__global__ void __launch_bounds__(THREADS) fork_apply(const PageForkArgs p, uint32_t slices)
+{
+    __shared__ int32_t upto[MAX_CHUNKS];         // free pages up to and with each chunk
+    const ForkSpace w = fork_space(p);
+    const int tid = threadIdx.x;
+    const int chunks = (int)chunks_of(p.pages);
+    uint32_t at = blockIdx.x;
+    if (at < p.children * slices) {
+        const int row = (int)(at / slices), slice = (int)(at % slices);
+        const int wanted = w.need[row];
+        int before = 0;
+        for (int i = tid; i < row; i += THREADS) before += w.need[i];
+        before = block_sum(before);
+        int free_pages = 0;
+        for (int c = 0; c < chunks; c += THREADS) {
+            const int n = c + tid < chunks ? w.count[c + tid] : 0;
+            int total;
+            const int ahead = block_before(n, total);
+            if (c + tid < chunks) upto[c + tid] = free_pages + ahead + n;
+            free_pages += total;
+        }
+        __syncthreads();
+        auto fresh = [&](int rank) {
+            if (rank >= free_pages) return -1;
+            int lo = 0, hi = chunks - 1;         // the first chunk with more than `rank` up to its end
+            while (lo < hi) {
+                const int mid = (lo + hi) / 2;
+                if (upto[mid] > rank) hi = mid;
+                else lo = mid + 1;
+            }
+            return w.freed[(int64_t)lo * CHUNK + rank - (lo ? upto[lo - 1] : 0)];
+        };
+        const int length = w.length[row], whole = length / (int)p.pageRows;
+        const bool partly = length % (int)p.pageRows != 0;
+        const int tail = partly ? w.staged[(int64_t)row * p.width + whole] : -1;
+        const int target = tail == WANTED ? fresh(before) : tail;
+        if (slice == 0) {
+            int rank = before;
+            for (int e0 = 0; e0 < (int)p.width; e0 += THREADS) {
+                const int e = e0 + tid;
+                int entry = e < (int)p.width ? w.staged[(int64_t)row * p.width + e] : -1;
+                int total = 0, ahead = 0;
+                if (wanted) ahead = block_before(entry == WANTED, total);
+                if (entry == WANTED) entry = fresh(rank + ahead);
+                rank += total;
+                if (e < (int)p.width) gout<int32_t>(p.newTable)[(int64_t)row * p.width + e] = entry;
+            }
+            if (tid == 0) gout<int32_t>(p.newLens)[row] = partly && target < 0 ? whole * (int)p.pageRows : length;
+        }
+        const int source = partly && tail == WANTED ? w.source[row] : -1;
+        if (source >= 0 && target >= 0)
+            copy_page(p.caches, p.cacheCount, source, target, slice * SLICE, (slice + 1) * SLICE);
+        return;
+    }
+    at -= p.children * slices;
+    int needed = 0;
+    for (int i = tid; i < (int)p.children; i += THREADS) needed += w.need[i];
+    needed = block_sum(needed);
+    int before = 0, free_pages = 0;
+    for (int c = tid; c < chunks; c += THREADS) {
+        free_pages += w.count[c];
+        if (c < (int)at) before += w.count[c];
+    }
+    before = block_sum(before);
+    if (at == 0) {
+        free_pages = block_sum(free_pages);
+        if (tid == 0) gout<int32_t>(p.missing)[0] = max(0, needed - free_pages);
+    }
+    const int64_t page = (int64_t)at * CHUNK + tid * PER_THREAD;
+    int held[PER_THREAD], mine = 0;
+#pragma unroll
+    for (int i = 0; i < PER_THREAD; ++i) {
+        held[i] = page + i < p.pages ? gptr<int32_t>(p.refs)[page + i] : 1;
+        mine += held[i] == 0;
+    }
+    int total, rank = before + block_before(mine, total);
+#pragma unroll
+    for (int i = 0; i < PER_THREAD; ++i)
+        if (page + i < p.pages) {
+            const int change = w.delta[page + i];
+            if (change) w.delta[page + i] = 0;
+            const int given = held[i] == 0 && rank++ < needed;
+            gout<int32_t>(p.newRefs)[page + i] = held[i] + change + given;
+        }
+}
+
+// ------------------------------------------------------------ compaction
+
+struct CompactSpace {
+    int32_t *count;        // [chunks] pages in use
+    int32_t *moves;        // [1]
+    int32_t *place;        // [pages] a page's own number, -1, or -2 - k: the k-th that moves
+    int32_t *target;       // [pages] free pages below L
+    int32_t *source;       // [pages] pages that move
+    int32_t *refs;         // [pages] their reference counts
+};
+__host__ __device__ inline uint64_t compact_words(uint32_t pages) { return (uint64_t)chunks_of(pages) + 1 + 4ull * pages; }
+__device__ __forceinline__ CompactSpace compact_space(const PageCompactArgs &p)
+{
+    CompactSpace w;
+    w.count = reinterpret_cast<int32_t *>(p.workspace);
+    w.moves = w.count + chunks_of(p.pages);
+    w.place = w.moves + 1;
+    w.target = w.place + p.pages;
+    w.source = w.target + p.pages;
+    w.refs = w.source + p.pages;
+    return w;
+}
+
+__global__ void __launch_bounds__(THREADS) compact_count(const PageCompactArgs p)
+{
+    const CompactSpace w = compact_space(p);
+    const int64_t page = (int64_t)blockIdx.x * CHUNK + threadIdx.x * PER_THREAD;
+    int mine = 0;
+#pragma unroll
+    for (int i = 0; i < PER_THREAD; ++i) mine += page + i < p.pages && gptr<int32_t>(p.refs)[page + i] > 0;
+    const int total = block_sum(mine);
+    if (threadIdx.x == 0) w.count[blockIdx.x] = total;
+}
+
+__global__ void __launch_bounds__(THREADS) compact_plan(const PageCompactArgs p)
+{
+    const CompactSpace w = compact_space(p);
+    const int tid = threadIdx.x, chunks = (int)chunks_of(p.pages), chunk = (int)blockIdx.x;
+    int before = 0, live = 0;
+    for (int c = tid; c < chunks; c += THREADS) {
+        live += w.count[c];
+        if (c < chunk) before += w.count[c];
+    }
+    before = block_sum(before);
+    live = block_sum(live);
+    // Pages in use below L: whole chunks, then a part of L's chunk.
+    const int last = live / CHUNK;
+    int below = 0;
+    for (int c = tid; c < min(last, chunks); c += THREADS) below += w.count[c];
+    for (int64_t i = (int64_t)last * CHUNK + tid; i < live; i += THREADS) below += gptr<int32_t>(p.refs)[i] > 0;
+    below = block_sum(below);
+    if (chunk == 0 && tid == 0) {
+        w.moves[0] = live - below;
+        gout<int32_t>(p.live)[0] = live;
+    }
+    const int64_t page = (int64_t)chunk * CHUNK + tid * PER_THREAD;
+    int held[PER_THREAD], mine = 0;
+#pragma unroll
+    for (int i = 0; i < PER_THREAD; ++i) {
+        held[i] = page + i < p.pages ? gptr<int32_t>(p.refs)[page + i] : 0;
+        mine += held[i] > 0;
+    }
+    int total, rank = before + block_before(mine, total);
+#pragma unroll
+    for (int i = 0; i < PER_THREAD; ++i) {
+        const int64_t at = page + i;
+        if (at >= p.pages) break;
+        int place = -1;
+        if (held[i] > 0) {
+            place = (int)at;
+            if (at >= live) {
+                const int k = rank - below;
+                place = -2 - k;
+                w.source[k] = (int)at;
+                w.refs[k] = held[i];
+            }
+            ++rank;
+        } else if (at < live)
+            w.target[at - rank] = (int)at;
+        w.place[at] = place;
+    }
+}
+
+// Work-groups: chunks of pages, chunks of table entries, then copies.
+__global__ void __launch_bounds__(THREADS) compact_apply(const PageCompactArgs p, uint32_t table_groups, uint32_t copies,
+                                                         uint32_t slices)
+{
+    const CompactSpace w = compact_space(p);
+    const int tid = threadIdx.x;
+    uint32_t at = blockIdx.x;
+    auto settle = [&](int place) { return place <= -2 ? w.target[-2 - place] : place; };
+    if (at < copies) {
+        const int64_t items = (int64_t)w.moves[0] * slices;
+        for (int64_t i = at; i < items; i += copies) {
+            const int k = (int)(i / slices);
+            const int64_t slice = i % slices;
+            copy_page(p.caches, p.cacheCount, w.source[k], w.target[k], slice * SLICE, (slice + 1) * SLICE);
+        }
+        return;
+    }
+    at -= copies;
+    if (at < table_groups) {
+        const int64_t first = (int64_t)at * CHUNK, end = min(first + CHUNK, (int64_t)p.rows * p.width);
+        for (int64_t i = first + tid; i < end; i += THREADS) {
+            const int page = gptr<int32_t>(p.table)[i];
+            gout<int32_t>(p.newTable)[i] = (uint32_t)page < p.pages ? settle(w.place[page]) : -1;
+        }
+        return;
+    }
+    at -= table_groups;
+    const int live = gptr<int32_t>(p.live)[0];
+    const int64_t page = (int64_t)at * CHUNK + tid * PER_THREAD;
+    int held[PER_THREAD];
+#pragma unroll
+    for (int i = 0; i < PER_THREAD; ++i) held[i] = page + i < p.pages ? gptr<int32_t>(p.refs)[page + i] : 0;
+    // Free pages of the chunk below L take the pages that move, in order: their rank is what is left of their index.
+    int spare = 0;
+#pragma unroll
+    for (int i = 0; i < PER_THREAD; ++i) spare += page + i < live && held[i] <= 0;
+    int total, rank = block_before(spare, total);
+    int before = 0;
+    for (int c = tid; c < (int)at; c += THREADS) before += CHUNK - w.count[c];
+    rank += block_sum(before);
+#pragma unroll
+    for (int i = 0; i < PER_THREAD; ++i) {
+        if (page + i >= p.pages) break;
+        const bool inside = page + i < live;
+        int count = 0;
+        if (inside) count = held[i] > 0 ? held[i] : w.refs[rank++];
+        gout<int32_t>(p.newRefs)[page + i] = count;
+        gout<int32_t>(p.moved)[page + i] = settle(w.place[page + i]);
+    }
+}
+
+}  // namespace
+
+extern "C" {
+
+int launch_sharedkv_path_commit(void *stream, const PathCommitArgs *a)
+{
+    if (!a || !a->caches || !a->table || !a->cuQ || !a->seqLens || !a->paths || !a->pathLens || !a->lengths)
+        return (int)hipErrorInvalidValue;
+    if (!a->cacheCount || !a->tableWidth || !a->pages || !a->pageRows || !a->rowBytes || (a->rowBytes & 15) || !a->depth)
+        return (int)hipErrorInvalidValue;
+    if (a->pages > 0x7fffffffu || a->tokens > 0x7fffffffu || a->depth > 0x3fffffffu) return (int)hipErrorInvalidValue;
+    if (!a->batch) return (int)hipSuccess;
+    const uint64_t groups = ((uint64_t)a->cacheCount * (a->rowBytes / 16) + THREADS - 1) / THREADS;
+    if (groups > 65535) return (int)hipErrorInvalidValue;
+    hipLaunchKernelGGL(path_commit, dim3(a->batch, (uint32_t)groups), dim3(THREADS), 0, static_cast<hipStream_t>(stream), *a);
+    return (int)hipGetLastError();
+}
+
+int launch_sharedkv_page_fork(void *stream, const PageForkArgs *a)
+{
+    if (!a || !a->caches || !a->table || !a->seqLens || !a->refs || !a->parents || !a->newTable || !a->newLens ||
+        !a->newRefs || !a->missing || !a->workspace)
+        return (int)hipErrorInvalidValue;
+    if (!a->cacheCount || !a->rows || !a->children || !a->width || !a->pages || !a->pageRows || !a->pageBytes)
+        return (int)hipErrorInvalidValue;
+    const uint64_t slices = (a->pageBytes + SLICE - 1) / SLICE;
+    if (a->pages > MAX_PAGES || a->rows > 0xfffffu || a->children > 0xfffffu || a->width > 0xffffffu ||
+        a->pageRows > 0xffffffu || a->room > 0x3fffffffu || slices * a->children > 0x3fffffffu)
+        return (int)hipErrorInvalidValue;
+    const uint32_t chunks = chunks_of(a->pages);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    hipLaunchKernelGGL(fork_plan, dim3(a->children + a->rows + chunks), dim3(THREADS), 0, s, *a);
+    hipLaunchKernelGGL(fork_apply, dim3((uint32_t)slices * a->children + chunks), dim3(THREADS), 0, s, *a, (uint32_t)slices);
+    return (int)hipGetLastError();
+}
+
+int launch_sharedkv_page_compact(void *stream, const PageCompactArgs *a)
+{
+    if (!a || !a->caches || !a->table || !a->refs || !a->newTable || !a->newRefs || !a->moved || !a->live || !a->workspace)
+        return (int)hipErrorInvalidValue;
+    if (!a->cacheCount || !a->pages || !a->pageBytes || a->pages > MAX_PAGES) return (int)hipErrorInvalidValue;
+    const uint64_t slices = (a->pageBytes + SLICE - 1) / SLICE, entries = (uint64_t)a->rows * a->width;
+    if (slices > 0xfffffu || entries > 0xffffffffull) return (int)hipErrorInvalidValue;
+    const uint32_t chunks = chunks_of(a->pages), table_groups = (uint32_t)((entries + CHUNK - 1) / CHUNK);
+    // At most half of the pages move; eight work-groups per CU fill the chip.
+    const uint64_t most = slices * (a->pages / 2);
+    const uint32_t copies = (uint32_t)(most < 2048 ? most : 2048);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    hipLaunchKernelGGL(compact_count, dim3(chunks), dim3(THREADS), 0, s, *a);
+    hipLaunchKernelGGL(compact_plan, dim3(chunks), dim3(THREADS), 0, s, *a);
+    hipLaunchKernelGGL(compact_apply, dim3(copies + table_groups + chunks), dim3(THREADS), 0, s, *a, table_groups, copies,
+                       (uint32_t)slices);
+    return (int)hipGetLastError();
+}
+
+uint64_t sharedkv_page_fork_workspace(uint32_t children, uint32_t width, uint32_t pages)
+{
+    return 4 * fork_words(children, width, pages);
+}
+uint64_t sharedkv_page_compact_workspace(uint32_t pages) { return 4 * compact_words(pages); }
+
+uint32_t sharedkv_path_commit_args_size(void) { return (uint32_t)sizeof(PathCommitArgs); }
+uint32_t sharedkv_page_fork_args_size(void) { return (uint32_t)sizeof(PageForkArgs); }
+uint32_t sharedkv_page_compact_args_size(void) { return (uint32_t)sizeof(PageCompactArgs); }
+
+}  // extern "C"

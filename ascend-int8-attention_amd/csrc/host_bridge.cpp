@@ -90,11 +90,58 @@ PyObject *cache_write(PyObject *, PyObject *const *args, Py_ssize_t nargs)
     Py_RETURN_NONE;
 }
 
+// A launch that takes (address, stream): the tree and page entries.
+template <typename Args>
+PyObject *launch_block(PyObject *const *args, Py_ssize_t nargs, int (*launch)(void *, const Args *), const char *what)
+{
+    if (nargs != 2) {
+        PyErr_Format(PyExc_TypeError, "%s takes (address, stream)", what);
+        return nullptr;
+    }
+    uint64_t address, stream;
+    if (!read_u64(args[0], &address) || !read_u64(args[1], &stream)) return nullptr;
+    if (!address) {
+        PyErr_Format(PyExc_ValueError, "Invalid %s argument block", what);
+        return nullptr;
+    }
+    int code;
+    Py_BEGIN_ALLOW_THREADS
+    code = launch((void *)(uintptr_t)stream, (const Args *)(uintptr_t)address);
+    Py_END_ALLOW_THREADS
+    if (code) return raise_code(code, what);
+    Py_RETURN_NONE;
+}
+
+PyObject *tree_attention(PyObject *, PyObject *const *args, Py_ssize_t nargs)
+{
+    return launch_block(args, nargs, launch_sharedkv_tree, "sharedkv tree attention");
+}
+PyObject *path_commit(PyObject *, PyObject *const *args, Py_ssize_t nargs)
+{
+    return launch_block(args, nargs, launch_sharedkv_path_commit, "sharedkv path commit");
+}
+PyObject *page_fork(PyObject *, PyObject *const *args, Py_ssize_t nargs)
+{
+    return launch_block(args, nargs, launch_sharedkv_page_fork, "sharedkv page fork");
+}
+PyObject *page_compact(PyObject *, PyObject *const *args, Py_ssize_t nargs)
+{
+    return launch_block(args, nargs, launch_sharedkv_page_compact, "sharedkv page compaction");
+}
+
 PyMethodDef methods[] = {
     {"attention", (PyCFunction)(void (*)(void))attention, METH_FASTCALL,
      "attention(address, blocks, variant, stream): launch a C8 attention argument block on a HIP stream"},
     {"cache_write", (PyCFunction)(void (*)(void))cache_write, METH_FASTCALL,
      "cache_write(address, blocks, stream): launch an INT8 cache-write argument block on a HIP stream"},
+    {"tree_attention", (PyCFunction)(void (*)(void))tree_attention, METH_FASTCALL,
+     "tree_attention(address, stream): launch a tree attention argument block on a HIP stream"},
+    {"path_commit", (PyCFunction)(void (*)(void))path_commit, METH_FASTCALL,
+     "path_commit(address, stream): launch a path commit argument block on a HIP stream"},
+    {"page_fork", (PyCFunction)(void (*)(void))page_fork, METH_FASTCALL,
+     "page_fork(address, stream): launch a page fork argument block on a HIP stream"},
+    {"page_compact", (PyCFunction)(void (*)(void))page_compact, METH_FASTCALL,
+     "page_compact(address, stream): launch a page compaction argument block on a HIP stream"},
     {nullptr, nullptr, 0, nullptr},
 };
 

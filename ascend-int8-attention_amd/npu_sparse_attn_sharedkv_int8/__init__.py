@@ -10,13 +10,18 @@ from importlib import import_module
 __version__ = "0.1.0+mi355x"
 __stage__ = "c8-gfx950"
 
-__all__ = ["CacheQuantization", "SharedKVCase", "PreparedAttention", "PreparedCacheWrite"]
+__all__ = ["CacheQuantization", "SharedKVCase", "PreparedAttention", "PreparedCacheWrite", "PreparedTreeAttention",
+           "PreparedPathCommit", "PreparedPageFork", "PreparedPageCompact"]
 
 _EXPORTS = {
     "CacheQuantization": ("contract", "CacheQuantization"),
     "SharedKVCase": ("contract", "SharedKVCase"),
     "PreparedAttention": ("attention", "PreparedAttention"),
     "PreparedCacheWrite": ("cache", "PreparedCacheWrite"),
+    "PreparedTreeAttention": ("tree", "PreparedTreeAttention"),
+    "PreparedPathCommit": ("pages", "PreparedPathCommit"),
+    "PreparedPageFork": ("pages", "PreparedPageFork"),
+    "PreparedPageCompact": ("pages", "PreparedPageCompact"),
 }
 
 

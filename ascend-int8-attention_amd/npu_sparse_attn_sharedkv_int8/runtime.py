@@ -51,6 +51,45 @@ class SharedKVDebug(ctypes.Structure):
         ("cmpCapacity", ctypes.c_uint32), ("tileCapacity", ctypes.c_uint32)]
 
 
+def _block(wide, narrow, tail=()):
+    return [(name, ctypes.c_uint64) for name in wide.split()] + [(name, ctypes.c_uint32) for name in narrow.split()] \
+        + list(tail)
+
+
+class TreeAttentionArgs(ctypes.Structure):
+    """include/sharedkv_hip.h."""
+    _fields_ = _block("q ori cmp oriScale cmpScale oriTable cmpTable cuQ seqLens sinks parents out lse workspace "
+                      "partial oriStride cmpStride",
+                      "tokens heads batch oriPages cmpPages oriTableWidth cmpTableWidth ratio window",
+                      [("softmaxScale", ctypes.c_float)])
+
+
+class PathCommitArgs(ctypes.Structure):
+    """include/sharedkv_hip.h."""
+    _fields_ = _block("caches table cuQ seqLens paths pathLens lengths",
+                      "cacheCount batch depth tokens tableWidth pages pageRows rowBytes")
+
+
+class PageForkArgs(ctypes.Structure):
+    """include/sharedkv_hip.h."""
+    _fields_ = _block("caches table seqLens refs parents newTable newLens newRefs missing workspace",
+                      "cacheCount rows children width pages pageRows room unused", [("pageBytes", ctypes.c_uint64)])
+
+
+class PageCompactArgs(ctypes.Structure):
+    """include/sharedkv_hip.h."""
+    _fields_ = _block("caches table refs newTable newRefs moved live workspace", "cacheCount rows width pages",
+                      [("pageBytes", ctypes.c_uint64)])
+
+
+# Entries that take (stream, argument block): library function, block, its size query.
+BLOCK_LAUNCHES = {
+    "tree_attention": ("launch_sharedkv_tree", TreeAttentionArgs, "sharedkv_tree_args_size"),
+    "path_commit": ("launch_sharedkv_path_commit", PathCommitArgs, "sharedkv_path_commit_args_size"),
+    "page_fork": ("launch_sharedkv_page_fork", PageForkArgs, "sharedkv_page_fork_args_size"),
+    "page_compact": ("launch_sharedkv_page_compact", PageCompactArgs, "sharedkv_page_compact_args_size"),
+}
+
 EXPORTS = ("launch_sharedkv_c8_sparse", "launch_sharedkv_c8_dense", "launch_sharedkv_c8_sparse_small",
            "launch_sharedkv_c8_dense_paired", "launch_sharedkv_c8_dense_packed",
            "launch_sharedkv_c8_dense_paired_narrow", "launch_sharedkv_c8_dense_packed_narrow",
@@ -58,7 +97,8 @@ EXPORTS = ("launch_sharedkv_c8_sparse", "launch_sharedkv_c8_dense", "launch_shar
            "sharedkv_c8_workspace_bytes", "sharedkv_c8_partial_bytes", "sharedkv_c8_noalloc_scratch_bytes",
            "sharedkv_c8_noalloc_layout", "sharedkv_c8_set_merge_mode", "sharedkv_c8_set_xcd_local",
            "sharedkv_c8_xcd_local", "sharedkv_attention_args_size", "sharedkv_cache_args_size",
-           "sharedkv_abi_version")
+           "sharedkv_abi_version", "sharedkv_page_fork_workspace", "sharedkv_page_compact_workspace",
+           *(name for launch, _, size in BLOCK_LAUNCHES.values() for name in (launch, size)))
 
 
 @lru_cache(maxsize=1)
@@ -101,6 +141,16 @@ def library():
     for name in ("sharedkv_attention_args_size", "sharedkv_cache_args_size", "sharedkv_abi_version"):
         getattr(lib, name).argtypes = []
         getattr(lib, name).restype = ctypes.c_uint32
+    for launch, block, size in BLOCK_LAUNCHES.values():
+        getattr(lib, launch).argtypes = [ctypes.c_void_p, ctypes.c_void_p]
+        getattr(lib, launch).restype = ctypes.c_int
+        getattr(lib, size).argtypes = []
+        getattr(lib, size).restype = ctypes.c_uint32
+        if getattr(lib, size)() != ctypes.sizeof(block):
+            raise RuntimeError(f"Native {block.__name__} ABI changed; rebuild the library")
+    for name, count in (("sharedkv_page_fork_workspace", 3), ("sharedkv_page_compact_workspace", 1)):
+        getattr(lib, name).argtypes = [ctypes.c_uint32] * count
+        getattr(lib, name).restype = ctypes.c_uint64
     if lib.sharedkv_attention_args_size() != ctypes.sizeof(SharedKVArgs):
         raise RuntimeError("Native SharedKVArgs ABI changed; rebuild the library")
     if lib.sharedkv_cache_args_size() != ctypes.sizeof(CacheWriteArgs):
@@ -186,6 +236,18 @@ class _Host:
     def cache_write_queued(self, address, blocks, device):
         self.cache_write(address, blocks, device)
 
+    def launch(self, name, address, device):
+        """Launch the argument block of a BLOCK_LAUNCHES entry on the current stream of `device`, which is made the
+        current device where it is not."""
+        import torch
+        if device != torch.cuda.current_device():
+            with torch.cuda.device(device):
+                return self.launch(name, address, device)
+        if self.bridge is not None:
+            getattr(self.bridge, name)(address, _stream(device))
+            return
+        _check(getattr(self.lib, BLOCK_LAUNCHES[name][0])(_stream(device), address), f"sharedkv {name}")
+
     def stream_id(self, device):
         """Identity of the current stream (launch.cpp:98-103)."""
         return _stream(device if device is not None and device >= 0 else None)
@@ -203,7 +265,7 @@ def native_launcher():
     host = _Host(library(), use_ctypes=os.environ.get("SHAREDKV_USE_CTYPES") == "1")
     if os.environ.get("SHAREDKV_HOST_QUEUE") == "1":
         return SimpleNamespace(attention=host.attention_queued, cache_write=host.cache_write_queued,
-                               attention_args_size=host.attention_args_size,
+                               launch=host.launch, attention_args_size=host.attention_args_size,
                                cache_args_size=host.cache_args_size,
                                attention_variant_count=host.attention_variant_count,
                                stream_id=host.stream_id, _owner=host)

@@ -1,0 +1,126 @@
+"""PreparedTreeAttention: attention of drafted-token trees over the INT8 caches.
+
+No counterpart in the reference, whose draft path lists each token's physical
+slots (SharedKVCase.ori_indices) and reads every token's rows for itself.
+Here the drafted tokens of a request form a tree and share what they read.
+
+Request b has the query tokens cu_q[b] .. cu_q[b + 1] - 1, its drafted tokens,
+and seq_lens[b] rows, the drafted ones included: C = seq_lens[b] - T committed
+rows, and the row of drafted token i is logical row C + i of the original
+cache (written before the launch, by PreparedCacheWrite).  parents[i] is the
+index in the request of token i's parent; an index that is not below the
+token's own (-1, by convention) makes it a root, a child of the last committed
+token.  A token of depth d (0 for a root) stands at position C + d and sees
+  * the original rows j < C with j > C + d - window,
+  * its ancestors and itself, those fewer than `window` steps above it,
+  * with ratio 128, the compressed rows r < C // 128 (what the committed
+    tokens completed; a branch's own rows are not compressed yet).
+For a chain this is PreparedAttention over the same rows.  Top-k layers
+(ratio 4) have a list of their own for every token, so nothing is shared:
+PreparedAttention takes them, with the ancestors' slots in ori_indices.
+
+  out = sum_j e^{s_j} v_j / (e^{sink} + sum_j e^{s_j}),  lse = log of the denominator
+"""
+import ctypes
+
+import torch
+
+from .attention import _check_cache
+from .c8_attention import BLOCK, MAX_HEADS
+from .runtime import TreeAttentionArgs, native_launcher
+
+RATIOS = (1, 128)
+MAX_WINDOW = 2 ** 31 - 1
+
+
+class PreparedTreeAttention:
+    """run() launches on the current stream of the inputs' device, allocates
+    nothing and reads nothing back.  Launches of one operator that may overlap
+    need an operator each.
+
+    Protocol: BF16 q[T, H, 512], 1..128 heads; INT8 caches [P, 32, 1, 512] with
+    any page stride that is a multiple of 16 bytes; frozen FP32[512] scales;
+    ratio 1 (window only) or 128 (and every compressed row); any window >= 1
+    (2**30 attends the whole context).  Rows on pages outside the pool or past
+    the block table are masked.  Tokens past cu_q[batch], and those of requests
+    with seq_lens 0, are graph padding: their outputs are zero.
+    """
+
+    def __init__(self, case, parents, ori_scale, cmp_scale=None, *, output=None, return_lse=False, lse_output=None):
+        q = case.q
+        if q.device.type != "cuda" or q.dtype != torch.bfloat16 or q.ndim != 3 or q.shape[-1] != 512:
+            raise ValueError("Expected BF16 Q[T,H,512] on a GPU")
+        tokens, heads, _ = q.shape
+        if not 1 <= heads <= MAX_HEADS or not q.is_contiguous() or q.data_ptr() % 16:
+            raise ValueError(f"Expected 1..{MAX_HEADS} heads and contiguous, 16-byte aligned Q")
+        if case.ratio not in RATIOS or case.cmp_indices is not None or case.ori_indices is not None:
+            raise ValueError("Trees attend a window (ratio 1) or a window and every compressed row (ratio 128); "
+                             "layers with lists per token (ratio 4, explicit slots) go through PreparedAttention")
+        if not 1 <= case.window <= MAX_WINDOW:
+            raise ValueError("Expected a positive window")
+        device, batch = q.device, case.seq_lens.numel()
+        caches = [(case.ori, case.ori_block_table, ori_scale)]
+        if case.ratio != 1:
+            caches.append((case.cmp, case.cmp_block_table, cmp_scale))
+        for cache, table, scale in caches:
+            _check_cache(cache, table, scale, batch, device)
+            if (cache.shape[1] != BLOCK or cache.stride(0) % 16 or cache.data_ptr() % 16 or scale.data_ptr() % 16
+                    or not table.shape[1]):
+                raise ValueError(f"Expected pages of {BLOCK} rows, 16-byte aligned, and a block table of one page or more")
+        if not batch or tuple(case.cu_q.shape) != (batch + 1,) or case.seq_lens.ndim != 1 \
+                or tuple(case.sink.shape) != (heads,):
+            raise ValueError("Invalid sequence metadata or sink shape")
+        if tuple(parents.shape) != (tokens,):
+            raise ValueError("Expected INT32 parents[T]")
+        for x, dtype in ((case.cu_q, torch.int32), (case.seq_lens, torch.int32), (case.sink, torch.float32),
+                         (parents, torch.int32)):
+            if x.dtype != dtype or x.device != device or not x.is_contiguous():
+                raise ValueError("Invalid metadata dtype, device or contiguity")
+        self.case, self.parents, self.scales = case, parents, (ori_scale, cmp_scale)
+        self.out = output if output is not None else torch.empty_like(q)
+        self.lse = lse_output
+        if lse_output is None and return_lse:
+            self.lse = torch.empty((tokens, heads), dtype=torch.float32, device=device)
+        self._check_outputs(q)
+        self.args = TreeAttentionArgs(
+            tokens=tokens, heads=heads, batch=batch, oriPages=case.ori.shape[0], oriStride=case.ori.stride(0),
+            oriTableWidth=case.ori_block_table.shape[1], ratio=case.ratio, window=case.window,
+            softmaxScale=case.softmax_scale, oriScale=ori_scale.data_ptr())
+        if case.ratio != 1:
+            self.args.cmpPages, self.args.cmpStride = case.cmp.shape[0], case.cmp.stride(0)
+            self.args.cmpTableWidth, self.args.cmpScale = case.cmp_block_table.shape[1], cmp_scale.data_ptr()
+        self._bind()
+        self.native = native_launcher()
+        self.argument_address = ctypes.addressof(self.args)
+        self.device_index = device.index if device.index is not None else torch.cuda.current_device()
+
+    def _check_outputs(self, q):
+        out, lse = self.out, self.lse
+        if (tuple(out.shape) != tuple(q.shape) or out.device != q.device or out.dtype != torch.bfloat16
+                or not out.is_contiguous() or out.data_ptr() % 16):
+            raise ValueError("Invalid output buffer")
+        if lse is not None and (tuple(lse.shape) != tuple(q.shape[:2]) or lse.dtype != torch.float32
+                                or lse.device != q.device or not lse.is_contiguous()):
+            raise ValueError("Invalid FP32 LSE[T,H] output buffer")
+
+    def _bind(self):
+        case, args = self.case, self.args
+        cmp = case.ratio != 1
+        for name, tensor in (("q", case.q), ("ori", case.ori), ("oriTable", case.ori_block_table),
+                             ("cmp", case.cmp if cmp else None), ("cmpTable", case.cmp_block_table if cmp else None),
+                             ("cuQ", case.cu_q), ("seqLens", case.seq_lens), ("sinks", case.sink),
+                             ("parents", self.parents), ("out", self.out), ("lse", self.lse)):
+            setattr(args, name, tensor.data_ptr() if tensor is not None else 0)
+
+    def _rebind_same_geometry(self, case, parents, *, output=None, lse_output=None):
+        """Serving fast path: same geometry, new tensors."""
+        self.case, self.parents = case, parents
+        if output is not None:
+            self.out, self.lse = output, lse_output
+        self._bind()
+
+    def run(self):
+        """Launch on the current stream of the case's device; returns .out."""
+        if self.args.tokens:
+            self.native.launch("tree_attention", self.argument_address, self.device_index)
+        return self.out

@@ -61,6 +61,86 @@ typedef struct CacheWriteArgs {
     uint32_t tokens, pages, pageSize, int64Slots, pairedSlots;
 } CacheWriteArgs;
 
+/* Tree attention arguments: a tree of drafted tokens per request over the
+ * INT8 caches (no counterpart in the reference).  Request b has the query
+ * tokens cuQ[b] .. cuQ[b + 1] - 1 (T of them) and seqLens[b] rows, the drafted
+ * ones included: C = seqLens[b] - T committed rows, and the row of its drafted
+ * token i is logical row C + i of the original cache.  parents (INT32
+ * [tokens]) names each drafted token's parent by its index in the request; an
+ * index that is not below the token's own makes it a root.  A token of depth d
+ * (a root's is 0) sees
+ *   original rows j < C with j > C + d - window,
+ *   its ancestors and itself, those fewer than `window` steps above it,
+ *   with a compressed cache (ratio > 1) its rows r < C / ratio.
+ * Rows on a page outside [0, oriPages) / [0, cmpPages), or past the block
+ * table, are masked.  q, out BF16 [tokens][heads][512], heads 1..128; sinks
+ * FP32 [heads]; lse FP32 [tokens][heads] or 0; ori / cmp INT8 pages of 32
+ * rows of 512 bytes, page strides in bytes, multiples of 16.  Tokens of
+ * requests with seqLens 0 and past cuQ[batch] are graph padding: their rows
+ * of out and lse are zero-filled. */
+typedef struct TreeAttentionArgs {
+    uint64_t q, ori, cmp, oriScale, cmpScale, oriTable, cmpTable, cuQ;
+    uint64_t seqLens, sinks, parents, out, lse, workspace, partial;
+    uint64_t oriStride, cmpStride;
+    uint32_t tokens, heads, batch, oriPages, cmpPages, oriTableWidth, cmpTableWidth, ratio, window;
+    float softmaxScale;
+} TreeAttentionArgs;
+
+/* One cache of a pool, for the entries below: page i at base + i * pageStride,
+ * its row r at + r * rowStride, `bytes` bytes each (a row's for the path
+ * commit, whose pages have pageRows rows; a page's for fork and compaction,
+ * which read no rowStride).  Everything is a multiple of 16. */
+typedef struct CacheSpan {
+    uint64_t base, pageStride, rowStride, bytes;
+} CacheSpan;
+
+/* Accepted paths of drafted-token trees (no counterpart in the reference).
+ * Requests as in TreeAttentionArgs (cuQ, seqLens, drafted rows behind the C
+ * committed ones).  paths INT32 [batch][depth] names the accepted tokens of a
+ * request by their index, rising; pathLens INT32 [batch] says how many there
+ * are.  A path ends before its first entry that does not rise or is none of
+ * the request's tokens.  Row C + paths[b][k] moves to row C + k in every cache,
+ * and lengths[b] = C + accepted (0 for padding requests, seqLens 0).  Rows on
+ * pages outside [0, pages), or past the block table, do not move.  `caches`
+ * is a device array of CacheSpan; lengths must not overlap seqLens. */
+typedef struct PathCommitArgs {
+    uint64_t caches, table, cuQ, seqLens, paths, pathLens, lengths;
+    uint32_t cacheCount, batch, depth, tokens, tableWidth, pages, pageRows, rowBytes;
+} PathCommitArgs;
+
+/* Rows of a block table that go on as other rows (no counterpart in the
+ * reference): forked, reordered, grown and ended requests.  Every old row is
+ * given up and row i of the new table continues old row parents[i] (outside
+ * [0, rows): an empty row, length 0), with pages for length + room tokens.  A
+ * page holds pageRows tokens.  Its whole pages are shared; of its other pages
+ * the first of a parent's children keeps those that have no other owner
+ * (refs 1), the rest are the lowest free pages (refs 0 when the call begins),
+ * handed out by row, then entry.  The partly filled page is copied where it
+ * was not kept.  Entries behind are -1.  Where free pages run out an entry is
+ * -1, a row without its partly filled page is cut back to its whole pages, and
+ * `missing` counts the entries.  Old entries outside [0, pages) are no pages.
+ * newTable [children][width], newLens, newRefs may be table, seqLens, refs.
+ * workspace: sharedkv_page_fork_workspace bytes, zero before the first launch
+ * (each launch leaves what has to be zero so). */
+typedef struct PageForkArgs {
+    uint64_t caches, table, seqLens, refs, parents, newTable, newLens, newRefs, missing, workspace;
+    uint32_t cacheCount, rows, children, width, pages, pageRows, room;
+    uint32_t unused;
+    uint64_t pageBytes;
+} PageForkArgs;
+
+/* Pool compaction (no counterpart in the reference): with L pages in use
+ * (refs > 0), those from L on move, in order, to the free pages below L, in
+ * order.  moved INT32 [pages]: each page's new place, -1 for free ones; the
+ * table's entries and the refs follow; live INT32 [1] = L.  Entries outside
+ * [0, pages) or on free pages become -1.  newTable and newRefs may be table
+ * and refs.  workspace: sharedkv_page_compact_workspace bytes. */
+typedef struct PageCompactArgs {
+    uint64_t caches, table, refs, newTable, newRefs, moved, live, workspace;
+    uint32_t cacheCount, rows, width, pages;
+    uint64_t pageBytes;
+} PageCompactArgs;
+
 /* Keys per tile of the attention kernels.  Together with SharedKVArgs.splits
  * it fixes the numerics: tile k of a query (kinds in order: original window,
  * then compressed rows) is folded into partition k % splits. */
@@ -145,6 +225,17 @@ int sharedkv_c8_attention_debug(void *stream, const SharedKVArgs *args, const Sh
  * slotColumnStride must fit 32 bits (else hipErrorInvalidValue). */
 int launch_cache_write(uint32_t blocks, void *stream, const CacheWriteArgs *args);
 
+/* Attention of drafted-token trees (TreeAttentionArgs). */
+int launch_sharedkv_tree(void *stream, const TreeAttentionArgs *args);
+
+/* Accepted paths, and pages of a pool (argument blocks above).  pageBytes is
+ * the sum of the caches' bytes and rowBytes the largest row's. */
+int launch_sharedkv_path_commit(void *stream, const PathCommitArgs *args);
+int launch_sharedkv_page_fork(void *stream, const PageForkArgs *args);
+int launch_sharedkv_page_compact(void *stream, const PageCompactArgs *args);
+uint64_t sharedkv_page_fork_workspace(uint32_t children, uint32_t width, uint32_t pages);
+uint64_t sharedkv_page_compact_workspace(uint32_t pages);
+
 /* Scratch sizes in bytes for a launch with `rows` = tokens * ceil(heads / 8)
  * rows (the query token count at eight heads).  partial_bytes(rows, 1) is
  * the partition-state room of a one-partition launch's device re-plan: when
@@ -209,6 +300,12 @@ int sharedkv_c8_set_xcd_local(int enable);
 /* The current device's probe result: 1 XCD-local exchange in use, 0 not
  * (probe failed), -1 not probed yet. */
 int sharedkv_c8_xcd_local(void);
+
+/* sizeof the argument blocks of trees and pages. */
+uint32_t sharedkv_tree_args_size(void);
+uint32_t sharedkv_path_commit_args_size(void);
+uint32_t sharedkv_page_fork_args_size(void);
+uint32_t sharedkv_page_compact_args_size(void);
 
 /* sizeof(SharedKVArgs), sizeof(CacheWriteArgs), library ABI version. */
 uint32_t sharedkv_attention_args_size(void);
