@@ -51,6 +51,7 @@
 #include <type_traits>
 
 #include "sharedkv_hip.h"
+#include "xcd_local.h"
 
 #pragma clang fp contract(off)
 
@@ -4223,6 +4224,8 @@ static_assert(PLAN_CUS * 4 <= NOALLOC_TICKET_BYTES &&
               "a one-partition launch's re-plan fits the allocation-free scratch");
 
 }  // namespace
+
+bool sharedkv::xcd_local(hipStream_t stream) { return xcd_local_dispatch(stream, true); }
 
 extern "C" {
 

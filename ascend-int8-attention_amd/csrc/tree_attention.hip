@@ -15,32 +15,45 @@
 // FP32 result and takes 24.  P V runs on v_mfma_f32_16x16x32_f16: codes are
 // exact in FP16, weights are rounded to its 11 bits (the output has 8).
 //
-// A unit is 64 query rows of one request (a row is a token and a head, heads
-// innermost), which share every key tile of 64 rows (two pages).  Four waves:
-// for Q K each has sixteen of the rows, for P V each has 128 of the channels,
-// the weights passing between them in LDS.
+// A unit is 16 RT query rows of one request (a row is a token and a head, heads
+// innermost), which share every key tile of 64 rows (two pages).  A work-group
+// of four waves takes an item, a run of a unit's tiles: for Q K a wave has
+// sixteen of the rows and 16 RT of the keys, for P V all rows and 128 of the
+// channels, the weights passing between them in LDS.  Tiles come by LDS DMA into
+// a ring of two, one in flight while the other is used.  Every work-group makes
+// the same plan from the live lengths (which requests there are, how many tiles
+// an item gets), and the last item of a unit to finish joins the unit's states.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
+#include "lds_dma.h"
 #include "sharedkv_hip.h"
+#include "xcd_local.h"
 
 namespace {
 
 constexpr int D = 512;
-constexpr int ROWS = 64;           // query rows of a unit
 constexpr int KEYS = 64;           // keys of a tile: two pages
 constexpr int PAGE_ROWS = 32;
 constexpr int THREADS = 256;
 constexpr int WAVES = THREADS / 64;
 constexpr int P_STRIDE = KEYS + 8; // halves; 144 bytes keep the 16-byte reads of 16 rows on different banks
 constexpr int PARENTS = 1024;      // parents kept in LDS; larger trees read theirs from memory
+constexpr int ROOT = 0xffff;
+constexpr int WHOLE = 0x3fffffff;  // tiles of an item where units are not split
 constexpr uint32_t MAX_HEADS = 128;
+constexpr uint32_t ITEMS = 512;    // two work-groups on each of 256 CUs
+constexpr uint32_t XCD_LOCAL = 0x80000000u;   // bit of `split`: work-groups with one blockIdx modulo 8 share an XCD
 constexpr float LOG2E = 1.44269504088896341f, LN2 = 0.69314718055994531f;
 // Weights are 2^(s - m) with m the row's maximum less HEAD when it was last
 // set, so they start at 2^HEAD and m moves only when a score passes it by
 // LIMIT: 2^15 is below FP16's largest, and weights down to 2^-22 of the
 // largest stay normal.
 constexpr float HEAD = 8.0f, LIMIT = 15.0f;
+// Cache policies of the states that items exchange: past the XCD's L2, where items of other XCDs see them, or in it.
+constexpr int SC1 = 16, SC0 = 1;
 
 typedef int v4i __attribute__((ext_vector_type(4)));
 typedef int v2i __attribute__((ext_vector_type(2)));
@@ -48,38 +61,57 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) v2i lds_v2i;
+typedef __attribute__((address_space(3))) v4i lds_v4i;
 
 template <typename T>
 __device__ __forceinline__ const __attribute__((address_space(1))) T *gptr(uint64_t a)
 {
     return reinterpret_cast<const __attribute__((address_space(1))) T *>(a);
 }
+// A value that the compiler takes for another: what is made of it is made anew where it is used and holds no register
+// meanwhile.  (128 of a thread's 256 registers hold the output and 64 the codes of Q where a unit has 64 rows.)
+__device__ __forceinline__ int again(int x)
+{
+    asm volatile("" : "+v"(x));
+    return x;
+}
 __device__ __forceinline__ int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi)
 {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{lo, hi}, bf16x2));
 }
+__device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 
-struct alignas(16) Shared {
-    int8_t tile[KEYS * D];             // key rows, their 16-byte chunks XOR-swizzled with the row
-    _Float16 p[ROWS * P_STRIDE];       // weights [row][key]
-    uint64_t mask[ROWS];               // the tile's keys that each of the unit's tokens sees
-    float factor[ROWS], top[ROWS], sum[ROWS];
-    int32_t moved[WAVES];              // whether a wave's rows moved their maximum in this tile
-    int32_t scan[WAVES];
-    int32_t found[2];
-    int32_t parent[PARENTS];
+// Tile addresses below are made by XOR within a row's 512 bytes.
+template <int RT>
+struct alignas(1024) Shared {
+    static constexpr int ROWS = 16 * RT, PARTS = WAVES / RT;
+    int8_t tile[2][KEYS * D];          // key rows, their 16-byte chunks XOR-swizzled with the row
+    union {
+        _Float16 p[ROWS * P_STRIDE];   // weights [row][key]
+        float scale[2][D];             // channel scales (compressed, original) while Q is encoded
+    };
+    uint64_t mask[ROWS];               // the tile's original rows that each of the unit's tokens sees
+    float factor[ROWS], top[ROWS], sum[PARTS][ROWS], peak[PARTS][ROWS];
+    int32_t moved[RT];                 // whether a row tile moved its maximum in this tile
+    int32_t scan[3][WAVES];
+    int32_t found[7];
+    int32_t walk[ROWS], steps[ROWS], depth[ROWS];   // of the unit's tokens: node that the walk is at, steps to it, depth
+    uint8_t token[ROWS];               // of the unit's rows
+    uint16_t parent[PARENTS];
 };
 
 // A request's rows of the launch, made safe: nothing below reads past the
 // arrays whatever cuQ and seqLens hold.
 struct Request {
-    int32_t first, nodes, committed;   // first token, drafted tokens, committed rows
+    int32_t first, nodes, length, committed;   // first token, drafted tokens, all rows, committed rows
     bool live;
     int32_t compressed;                // visible compressed rows
     int32_t low, end;                  // original rows [low, end), low a multiple of PAGE_ROWS
@@ -92,6 +124,7 @@ __device__ __forceinline__ Request request_of(const TreeAttentionArgs &p, int c0
     const int tokens = (int)p.tokens;
     r.first = min(max(c0, 0), tokens);
     r.nodes = min(max(c1, r.first), tokens) - r.first;
+    r.length = length;
     r.live = length > 0 && r.nodes > 0;
     r.committed = max(0, length - r.nodes);
     const int64_t ori_rows = (int64_t)p.oriTableWidth * PAGE_ROWS, cmp_rows = (int64_t)p.cmpTableWidth * PAGE_ROWS;
@@ -103,73 +136,79 @@ __device__ __forceinline__ Request request_of(const TreeAttentionArgs &p, int c0
     return r;
 }
 
+// Maximum over the four lanes of a query row (lane modulo 16).
+__device__ __forceinline__ float row_max(float v)
+{
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+
+// Largest |q scale| of the lane's row among channels 64 j + 16 g .. + 15, j from j0 on; infinity where there is an
+// infinity or NaN.
+template <int JN>
+__device__ __forceinline__ float largest(const u32x4 (&raw)[JN][2], int j0, const float *scale, int g)
+{
+    float peak = 0.0f;
+    u16x2 bits = {0, 0};
+#pragma unroll
+    for (int j = 0; j < JN; ++j)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t w = raw[j][h][e];
+                const float *s = scale + 64 * (j0 + j) + 16 * g + 8 * h + 2 * e;
+                peak = fmaxf(fmaxf(peak, fabsf(bf16_lo(w) * s[0])), fabsf(bf16_hi(w) * s[1]));
+                bits = __builtin_elementwise_max(bits, __builtin_bit_cast(u16x2, w & 0x7fff7fffu));
+            }
+    if (bits[0] >= 0x7f80 || bits[1] >= 0x7f80) peak = INFINITY;
+    return row_max(peak);
+}
+
+// q * scale as whole numbers of 8 * TERMS bits relative to the row's largest.
 template <int TERMS>
 struct Codes {
-    v4i term[TERMS][8];                // most significant first; channels 64 j + 16 g .. + 15 of row n
-    float step;                        // score (base 2) of one unit
-};
+    static constexpr float LARGEST = TERMS == 2 ? 127.0f * 256.0f : 127.0f * 65536.0f;
+    v4i term[TERMS][8];                // most significant first
+    float inverse, step;               // units of one q * scale; score (base 2) of one unit
 
-// q * scale of the lane's row as whole numbers of 8 * TERMS bits.
-template <int TERMS>
-__device__ __forceinline__ void encode(Codes<TERMS> &c, uint64_t q_row, uint64_t scale, int g, float softmax2)
-{
-    asm volatile("" : "+v"(g));        // keeps the addresses below from being held in registers across tiles
-    constexpr float LARGEST = TERMS == 2 ? 127.0f * 256.0f : 127.0f * 65536.0f;
-    float peak = 0.0f;
-    bool odd = false;                  // an infinity or NaN
-    const auto *qp = gptr<u32x4>(q_row);
-    const auto *sp = gptr<f32x4>(scale);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            const u32x4 w = qp[(64 * j + 16 * g + 8 * half) / 8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float s = sp[(64 * j + 16 * g + 8 * half) / 4 + e / 4][e & 3];
-                const float x = __uint_as_float(e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16) * s;
-                peak = fmaxf(peak, fabsf(x));
-                odd |= !(fabsf(x) < INFINITY);
-            }
-        }
-        __builtin_amdgcn_sched_barrier(0);   // a few loads at a time: registers are short here
+    __device__ __forceinline__ void set(float peak, float softmax2)
+    {
+        // Rows below 2^-90 score zero to FP32 against any code; their inverse would overflow.  The units' sign is the
+        // softmax scale's, so that the largest sum has the largest score.
+        const bool some = !(peak <= 0x1p-90f), odd = !(peak < INFINITY);
+        inverse = some && !odd ? (softmax2 < 0.0f ? -LARGEST : LARGEST) / peak : 0.0f;
+        // Never 0, so that masked keys score -infinity.
+        step = odd ? __builtin_nanf("") : some ? fmaxf(peak / LARGEST * fabsf(softmax2), 0x1p-126f) : 1.0f;
     }
-    peak = fmaxf(peak, __shfl_xor(peak, 16));
-    peak = fmaxf(peak, __shfl_xor(peak, 32));
-    const uint64_t any = __ballot(odd);
-    const int n = threadIdx.x & 15;
-    const bool bad = ((any >> n) | (any >> (n + 16)) | (any >> (n + 32)) | (any >> (n + 48))) & 1;
-    // Rows below 2^-90 score zero to FP32 against any code; their inverse would overflow.
-    asm volatile("" : "+v"(g));
-    const float inverse = peak > 0x1p-90f ? LARGEST / peak : 0.0f;
-    c.step = bad ? __builtin_nanf("") : peak > 0x1p-90f ? peak / LARGEST * softmax2 : 0.0f;
+    // Eight channels' codes: words [term][0 and 1].
+    __device__ __forceinline__ void make(uint32_t (&out)[TERMS][2], const u32x4 &w, const float *s) const
+    {
+        uint32_t v[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            const u32x4 w = qp[(64 * j + 16 * g + 8 * half) / 8];
-#pragma unroll
-            for (int word = 0; word < 2; ++word) {
-                uint32_t packed[TERMS] = {};
-#pragma unroll
-                for (int e = 4 * word; e < 4 * word + 4; ++e) {
-                    const float s = sp[(64 * j + 16 * g + 8 * half) / 4 + e / 4][e & 3];
-                    const float x = __uint_as_float(e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16) * s;
-                    const float y = fminf(fmaxf(x * inverse, -LARGEST), LARGEST);
-                    int v = bad ? 0 : (int)__builtin_rintf(y);
-#pragma unroll
-                    for (int t = TERMS - 1; t >= 0; --t) {
-                        const int low = t ? (int)(int8_t)v : v;
-                        packed[t] |= (uint32_t)(low & 255) << (8 * (e & 3));
-                        v = (v - low) >> 8;
-                    }
-                }
-#pragma unroll
-                for (int t = 0; t < TERMS; ++t) c.term[t][j][2 * half + word] = (int)packed[t];
-            }
-            __builtin_amdgcn_sched_barrier(0);
+        for (int e = 0; e < 8; ++e) {
+            const float x = e & 1 ? bf16_hi(w[e / 2]) : bf16_lo(w[e / 2]);
+            // 1.5 * 2^23 more: the nearest whole number sits in the low bits, the bytes above the lowest
+            // rounded by half of what is below them so that each byte is signed.
+            if (TERMS == 2) v[e] = __float_as_uint(__builtin_fmaf(x * s[e], inverse, 12582912.0f));
+            else v[e] = (uint32_t)(int)__builtin_rintf(x * s[e] * inverse);
         }
-}
+#pragma unroll
+        for (int t = TERMS - 1; t >= 0; --t)
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                uint32_t u[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) u[e] = v[4 * q + e];
+                const uint32_t ab = __builtin_amdgcn_perm(u[1], u[0], 0x0c0c0400u), cd = __builtin_amdgcn_perm(u[3], u[2], 0x04000c0cu);
+                out[t][q] = ab | cd;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[4 * q + e] = (v[4 * q + e] + 128) >> 8;
+            }
+    }
+};
 
 // Eight codes to FP16, exactly: 1024 + (code + 128) has the byte as its low
 // mantissa bits.
@@ -186,71 +225,132 @@ __device__ __forceinline__ f16x8 to_f16(v2i w)
     return out;
 }
 
-// Inclusive sum over the work-group; `total` gets the whole.
-__device__ __forceinline__ int block_scan(Shared &s, int v, int &total)
+// Sum over the lanes up to and with this one.
+__device__ __forceinline__ int wave_upto(int v)
 {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int step = 1; step < 64; step *= 2) {
-        const int other = __shfl_up(v, step);
-        if (lane >= step) v += other;
-    }
-    __syncthreads();
-    if (lane == 63) s.scan[wave] = v;
-    __syncthreads();
-    total = 0;
-    int before = 0;
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-        if (w < wave) before += s.scan[w];
-        total += s.scan[w];
-    }
-    return v + before;
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);    // row_shr 1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);   // row_bcast 15, 31
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+    return v;
+}
+__device__ __forceinline__ int wave_sum(int v) { return __builtin_amdgcn_readlane(wave_upto(v), 63); }
+
+// Floats of an item's state: numerators in the order the waves hold them, then
+// the rows' maxima and sums.
+__host__ __device__ constexpr uint64_t state_floats(int rt) { return 16ull * rt * (D + 2); }
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t state_at(uint64_t partial, uint64_t item, int rt)
+{
+    return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<float *>(partial) + item * state_floats(rt), 0, 0x7fffffff,
+                                             0x00020000);
 }
 
-template <int TERMS>
-__global__ void __launch_bounds__(THREADS, TERMS == 2 ? 2 : 1) tree_attention(const TreeAttentionArgs p)
+template <int TERMS, int RT>
+__global__ void __launch_bounds__(THREADS, TERMS == 2 || RT < 4 ? 2 : 1) tree_attention(const TreeAttentionArgs p, const uint32_t split)
 {
-    __shared__ Shared s;
+    using S = Shared<RT>;
+    constexpr int ROWS = S::ROWS, PARTS = S::PARTS;
+    __shared__ S s;
     const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6), g = lane >> 4, n = lane & 15;
     const int heads = (int)p.heads, batch = (int)p.batch;
     const auto *cu = gptr<int32_t>(p.cuQ), *lens = gptr<int32_t>(p.seqLens);
 
-    // The unit of this work-group: units of the requests in order, then the
-    // rows of graph padding behind the last request.
-    int unit = (int)blockIdx.x, b = -1;
+    // ---- plan: units and tiles of the live requests, tiles of an item, this work-group's item ----
+    auto units_of = [&](const Request &r) { return (r.nodes * heads + ROWS - 1) / ROWS; };
+    Request mine = {};
+    int units = 0, kinds = 0, work = 0;                // units, times their kinds, times their tiles
+    for (int b = tid; b < batch; b += THREADS) {
+        mine = request_of(p, cu[b], cu[b + 1], lens[b]);
+        const int u = units_of(mine);
+        units += u;
+        kinds += u * max(1, (mine.cmp_tiles > 0) + (mine.ori_tiles > 0));
+        work = (int)min((int64_t)u * (mine.cmp_tiles + mine.ori_tiles) + work, (int64_t)0x1ffffff);
+    }
+    const int end = min(max(cu[batch], 0), (int)p.tokens) * heads;
+    const int all_rows = (int)p.tokens * heads, pad_units = (all_rows - end + ROWS - 1) / ROWS;
+    units = wave_sum(units), kinds = wave_sum(kinds), work = wave_sum(work);
+    if (lane == 0) s.scan[0][wave] = units, s.scan[1][wave] = kinds, s.scan[2][wave] = work;
+    if (tid == 0) s.found[0] = -1;
+    __syncthreads();
+    units = kinds = pad_units;
+    int64_t all_work = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) units += s.scan[0][w], kinds += s.scan[1][w], all_work += s.scan[2][w];
+    // Tiles of an item: as many as leave no more than ITEMS items (a unit's last of either kind may be short).
+    // `split` is the number of units that the launch has scratch for: requests that lie one behind the other are never
+    // more, and others are not split.
+    int per_item = WHOLE;
+    if (units <= (int)(split & ~XCD_LOCAL)) {
+        const int64_t room = (int64_t)ITEMS - kinds;
+        per_item = (int)min((int64_t)WHOLE - 1, max((int64_t)1, (all_work + room - 1) / room));
+    }
+    // A unit that is split is split between its kinds too: Q is encoded with a kind's scales.
+    auto parts_of = [&](int tiles) { return (tiles + per_item - 1) / per_item; };
+    auto items_of = [&](const Request &r) {
+        return per_item == WHOLE ? 1 : max(1, parts_of(r.cmp_tiles) + parts_of(r.ori_tiles));
+    };
+    // Work-groups of one XCD (blockIdx modulo 8) take neighbouring items, which read the same rows.
+    int item, items = 0, share = 0, unit = 0, unit0 = 0, b = -1;
     {
-        int done = 0;
-        if (tid < 2) s.found[tid] = -1;
-        for (int at = 0; at < batch && unit >= done; at += THREADS) {
-            const int mine = at + tid;
-            int units = 0;
-            if (mine < batch) units = (request_of(p, cu[mine], cu[mine + 1], 1).nodes * heads + ROWS - 1) / ROWS;
-            int total;
-            const int upto = block_scan(s, units, total) + done;
-            if (unit < upto && unit >= upto - units) s.found[0] = mine, s.found[1] = unit - (upto - units);
-            done += total;
-            __syncthreads();
+        int upto = 0, at_units = 0;
+        for (int pass = 0; pass < 2 && b < 0; ++pass) {
+            // First the number of items (pass 0 ends there where one step holds all requests), then whose this one is.
+            int before = 0, units_before = 0;
+            const bool one_step = batch <= THREADS;
+            for (int at = 0; at < batch; at += THREADS) {
+                const int b0 = at + tid;
+                if (!one_step) mine = b0 < batch ? request_of(p, cu[b0], cu[b0 + 1], lens[b0]) : Request{};
+                const bool there = b0 < batch;
+                const int u = there ? units_of(mine) : 0, n_items = there ? u * items_of(mine) : 0;
+                upto = wave_upto(n_items), at_units = wave_upto(u);
+                __syncthreads();
+                if (lane == 63) s.scan[0][wave] = upto, s.scan[1][wave] = at_units;
+                __syncthreads();
+                int total = 0, total_units = 0;
+#pragma unroll
+                for (int w = 0; w < WAVES; ++w) {
+                    if (w < wave) upto += s.scan[0][w], at_units += s.scan[1][w];
+                    total += s.scan[0][w], total_units += s.scan[1][w];
+                }
+                upto += before, at_units += units_before;
+                before += total, units_before += total_units;
+                if (one_step || pass) {
+                    if (one_step) items = before + pad_units;
+                    share = (items + 7) / 8;
+                    item = (int)(blockIdx.x & 7) * share + (int)(blockIdx.x >> 3);
+                    if ((int)(blockIdx.x >> 3) >= share || item >= items) return;
+                    if (item < upto && item >= upto - n_items) {
+                        s.found[0] = b0, s.found[1] = item - (upto - n_items), s.found[2] = at_units - u;
+                        s.found[3] = mine.first, s.found[4] = mine.first + mine.nodes, s.found[5] = mine.length;
+                    }
+                }
+            }
+            items = before + pad_units;
+            if (one_step) break;
         }
         __syncthreads();
         b = s.found[0];
-        if (b >= 0) unit = s.found[1];
-        else unit -= done;
     }
-    const int all_rows = (int)p.tokens * heads;
     auto zero_rows = [&](int first, int count) {
         for (int i = tid; i < count * (D / 8); i += THREADS)
             reinterpret_cast<u32x4 *>(p.out)[(int64_t)first * (D / 8) + i] = u32x4{0, 0, 0, 0};
         if (p.lse)
             for (int i = tid; i < count; i += THREADS) reinterpret_cast<float *>(p.lse)[first + i] = 0.0f;
     };
-    if (b < 0) {
-        const int live = min(max(cu[batch], 0), (int)p.tokens) * heads;
-        const int64_t first = (int64_t)live + (int64_t)unit * ROWS;
+    if (b < 0) {                                       // rows behind the last request
+        const int64_t first = (int64_t)end + (int64_t)(item - (items - pad_units)) * ROWS;
         if (first < all_rows) zero_rows((int)first, (int)min((int64_t)ROWS, all_rows - first));
         return;
     }
-    const Request r = request_of(p, cu[b], cu[b + 1], lens[b]);
+    b = uni(b);
+    const Request r = request_of(p, uni(s.found[3]), uni(s.found[4]), uni(s.found[5]));
+    const int splits = items_of(r), local = uni(s.found[1]);
+    const int part_no = local % splits;                // which of the unit's items
+    unit = local / splits;
+    unit0 = uni(s.found[2]);
     const int row0 = unit * ROWS;                      // of the request
     const int rows = min(ROWS, r.nodes * heads - row0);
     const int64_t out0 = (int64_t)r.first * heads + row0;
@@ -258,107 +358,279 @@ __global__ void __launch_bounds__(THREADS, TERMS == 2 ? 2 : 1) tree_attention(co
         zero_rows((int)out0, rows);
         return;
     }
-
-    // Tokens of the unit: thread t < tokens walks token t's chain.
-    const int token0 = row0 / heads, tokens = (row0 + rows - 1) / heads - token0 + 1;
-    for (int i = tid; i < min(r.nodes, PARENTS); i += THREADS) s.parent[i] = gptr<int32_t>(p.parents)[r.first + i];
-    __syncthreads();
-    auto parent_of = [&](int node) {
-        const int up = r.nodes <= PARENTS ? s.parent[node] : gptr<int32_t>(p.parents)[r.first + node];
-        return up >= 0 && up < node ? up : -1;
-    };
-    int walk = -1, steps = 0, depth = 0;
-    if (tid < tokens) {
-        walk = token0 + tid;
-        for (int a = parent_of(walk); a >= 0; a = parent_of(a)) ++depth;
+    const int tiles = r.cmp_tiles + r.ori_tiles;
+    int k0 = 0, k1 = tiles;
+    if (splits > 1) {                                  // equal shares of the kind's tiles
+        const int first = parts_of(r.cmp_tiles), second = parts_of(r.ori_tiles);
+        const bool window = part_no >= first;
+        const int at = window ? part_no - first : part_no, of = window ? second : first;
+        const int its_tiles = window ? r.ori_tiles : r.cmp_tiles;
+        k0 = (window ? r.cmp_tiles : 0) + (int)((int64_t)its_tiles * at / of);
+        k1 = (window ? r.cmp_tiles : 0) + (int)((int64_t)its_tiles * (at + 1) / of);
     }
 
-    const int row = 16 * wave + n;                     // the lane's row in Q K
-    const bool there = row < rows;
-    const int token = there ? (row0 + row) / heads - token0 : 0;
-    const uint64_t q_row = p.q + (uint64_t)(out0 + (there ? row : 0)) * (D * 2);
-    const float softmax2 = p.softmaxScale * LOG2E;
-
-    Codes<TERMS> q;
-    f32x4 acc[8][4] = {};
-    float m = -INFINITY, sum = 0.0f;
-    const int tiles = r.cmp_tiles + r.ori_tiles;
-    auto run_tile = [&](int k, const bool window) {
-        // Original tiles run from the last to the first: the walks go from a token up.
-        const int base = window ? r.low + (tiles - 1 - k) * KEYS : k * KEYS;
-        uint64_t seen = 0;                             // the tile's rows that lie on a page of the pool
-        {
-            const uint64_t table = window ? p.oriTable : p.cmpTable;
-            const int width = (int)(window ? p.oriTableWidth : p.cmpTableWidth);
-            const uint32_t pages = window ? p.oriPages : p.cmpPages;
-            const uint64_t pool = window ? p.ori : p.cmp, stride = window ? p.oriStride : p.cmpStride;
-            __syncthreads();
+    // ---- tiles: k < cmp_tiles compressed rows upwards, then the original rows downwards (walks go up the tree) ----
+    auto base_of = [&](int k) { return k < r.cmp_tiles ? k * KEYS : r.low + (tiles - 1 - k) * KEYS; };
+    int entries = -1;                                  // page of half (lane & 1) of tile 32 block + lane / 2
+    auto read_entries = [&](int block) {
+        const int k = 32 * block + (lane >> 1);
+        const bool window = k >= r.cmp_tiles;
+        const int e = base_of(k) / PAGE_ROWS + (lane & 1), width = (int)(window ? p.oriTableWidth : p.cmpTableWidth);
+        entries = k < k1 && e < width ? gptr<int32_t>(window ? p.oriTable : p.cmpTable)[(int64_t)b * width + e] : -1;
+    };
+    // Starts the copies of tile k and returns its rows that lie on a page.  Wave w moves rows 4 w .. 4 w + 3 of every
+    // sixteen, two an instruction, so that a lane's place in a row (the swizzle goes by the row modulo 16) is the same
+    // for all sixteens, and differs by one bit between the pairs.
+    auto copy_tile = [&](int k) -> uint64_t {
+        const int at = 2 * (k & 31);
+        const bool window = k >= r.cmp_tiles;
+        const uint64_t pool = window ? p.ori : p.cmp, stride = window ? p.oriStride : p.cmpStride;
+        const uint32_t pages = window ? p.oriPages : p.cmpPages;
+        const int lx = again(lane);
+        const uint32_t lane_offset =
+            (uint32_t)((4 * wave + (lx >> 5)) * D + (((lx & 31) ^ (4 * wave + (lx >> 5))) << 4));
+        const uint32_t to = (uint32_t)(uintptr_t)s.tile[k & 1] + 4 * wave * D;
+        uint64_t rows_there = 0;
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const int e = base / PAGE_ROWS + half;
-                const int page = e < width ? gptr<int32_t>(table)[(int64_t)b * width + e] : -1;
-                const bool good = (uint32_t)page < pages;
-                if (good) seen |= 0xffffffffull << (32 * half);
-                const auto *from = gptr<v4i>(pool + (good ? (uint64_t)page : 0) * stride);
+        for (int half = 0; half < 2; ++half) {
+            const int page = __builtin_amdgcn_readlane(entries, at + half);
+            if ((uint32_t)page >= pages) continue;
+            rows_there |= 0xffffffffull << (32 * half);
+            const uint64_t from = pool + (uint64_t)page * stride;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int at = tid + i * THREADS, slot = PAGE_ROWS * half + at / 32, chunk = at & 31;
-                    *reinterpret_cast<v4i *>(s.tile + slot * D + ((chunk ^ (slot & 15)) << 4)) = from[at];
-                }
+            for (int i = 0; i < 2; ++i) {
+                const uint32_t lds = (uint32_t)uni((int)(to + (32 * half + 16 * i) * D));
+                lds_dma16(from + 16 * i * D, lane_offset, lds);
+                lds_dma16(from + 16 * i * D, (lane_offset ^ 32u) + 2 * D, lds + 2 * D);
             }
         }
-        if (!window) {
-            const int left = r.compressed - base;
-            if (left < KEYS) seen &= (1ull << left) - 1;
-            if (tid < ROWS) s.mask[tid] = seen;
-        } else if (tid < tokens) {
-            // Committed rows (C + depth - window, C), then the ancestors.
-            uint64_t mine = 0;
-            const int64_t from = max((int64_t)0, (int64_t)r.committed + depth - p.window + 1 - base);
-            const int64_t to = min((int64_t)KEYS, (int64_t)r.committed - base);
-            if (from < to) mine = (to == KEYS ? ~0ull : (1ull << to) - 1) & ~((1ull << from) - 1);
-            for (; walk >= 0 && r.committed + walk >= base && (uint32_t)steps < p.window; walk = parent_of(walk), ++steps)
-                if (r.committed + walk < base + KEYS) mine |= 1ull << (r.committed + walk - base);
-            s.mask[tid] = mine & seen;
-        }
-        __syncthreads();
+        return rows_there;
+    };
 
-        // S = Q K^T: query row n, keys 16 kt + 4 g + i.
-        int lx = lane;
-        asm volatile("" : "+v"(lx));   // addresses from here on are made anew: registers are short
-        const int gx = lx >> 4, nx = lx & 15;
-        const int8_t *at = s.tile + nx * D;
-        const uint64_t mask = s.mask[token];
-        float w[4][4], peak = -INFINITY;
+    // ---- Q, scales and parents; the first tile is on its way while Q is encoded ----
+    const int row = 16 * (wave % RT) + n;              // the lane's row in Q K
+    const int key0 = wave / RT * 16 * RT;              // the wave's first key there
+    auto q_at = [&](int j) {                           // its channels 64 j + 16 g on; rows past the unit's take the first's
+        const int lx = again(lane), at = 16 * (wave % RT) + (lx & 15);
+        return gptr<u32x4>(p.q + (uint64_t)(out0 + (at < rows ? at : 0)) * (D * 2)) + 2 * (lx >> 4) + 8 * j;
+    };
+    const int token0 = row0 / heads, tokens = (row0 + rows - 1) / heads - token0 + 1;
+    const float softmax2 = p.softmaxScale * LOG2E;
+    const bool has_cmp = k0 < r.cmp_tiles && k0 < k1, has_ori = k1 > r.cmp_tiles;
+    // The waves of a row tile encode a share of its channels each (64 j .. 64 j + 63, j from j0 on) and pass the codes
+    // round in the tile buffer that is free.
+    constexpr bool SHARE = PARTS > 1 && RT * TERMS * 8 * 64 * 16 <= KEYS * D;
+    constexpr int JN = SHARE ? 8 / PARTS : 8;
+    const int j0 = SHARE ? wave / RT * JN : 0;
+    auto load_scales = [&]() {
+        for (int i = tid; i < D / 4; i += THREADS) {
+            if (has_cmp) reinterpret_cast<f32x4 *>(s.scale[0])[i] = gptr<f32x4>(p.cmpScale)[i];
+            if (has_ori) reinterpret_cast<f32x4 *>(s.scale[1])[i] = gptr<f32x4>(p.oriScale)[i];
+        }
+    };
+    auto row_peak = [&](float mine_peak) {             // over the waves of the row tile
+        if (!SHARE) return mine_peak;
+        if (g == 0) s.peak[wave / RT][row] = mine_peak;
+        lds_barrier();
+        float peak = s.peak[0][row];
 #pragma unroll
-        for (int kp = 0; kp < 2; ++kp) {
-            v4i dots[TERMS][2] = {};
+        for (int part = 1; part < PARTS; ++part) peak = fmaxf(peak, s.peak[part][row]);
+        lds_barrier();
+        return peak;
+    };
+    Codes<TERMS> q = {};
+    auto stage_at = [&](int8_t *stage, int t, int j) { return stage + ((((wave % RT) * TERMS + t) * 8 + j) * 64 + lane) * 16; };
+    // Codes of eight channels; where waves share a row tile they go to the staging buffer, whence all read them.
+    auto put = [&](int8_t *stage, int j, int h, const u32x4 &w, const float *scale) {
+        uint32_t out[TERMS][2];
+        q.make(out, w, scale + 64 * j + 16 * g + 8 * h);
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
+        for (int t = 0; t < TERMS; ++t)
+            if (!SHARE) q.term[t][j][2 * h] = (int)out[t][0], q.term[t][j][2 * h + 1] = (int)out[t][1];
+            else *reinterpret_cast<u32x2 *>(stage_at(stage, t, j) + 8 * h) = u32x2{out[t][0], out[t][1]};
+    };
+    auto take = [&](int8_t *stage) {
+        if (!SHARE) return;
+        lds_barrier();
 #pragma unroll
-                for (int kt = 0; kt < 2; ++kt) {
-                    const v4i key =
-                        *reinterpret_cast<const v4i *>(at + 16 * (2 * kp + kt) * D + (((4 * j + gx) ^ nx) << 4));
+        for (int t = 0; t < TERMS; ++t)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) q.term[t][j] = *reinterpret_cast<const v4i *>(stage_at(stage, t, j));
+    };
+    uint64_t seen = 0, next_seen = 0;
+    float ori_peak = 0.0f;
+    if (k0 < k1) {
+        u32x4 raw[JN][2];
+#pragma unroll
+        for (int j = 0; j < JN; ++j) raw[j][0] = q_at(j0 + j)[0], raw[j][1] = q_at(j0 + j)[1];
+        read_entries(k0 >> 5);
+        load_scales();
+        if (tid < ROWS) s.token[tid] = (uint8_t)((row0 + min(tid, rows - 1)) / heads - token0);
+        if (has_ori)
+            for (int i = tid; i < min(r.nodes, PARENTS); i += THREADS) {
+                const int up = gptr<int32_t>(p.parents)[r.first + i];
+                s.parent[i] = (uint16_t)(up >= 0 && up < i ? up : ROOT);
+            }
+        // The copies come last: a wait for an earlier load does not wait for them.
+#pragma unroll
+        for (int j = 0; j < JN; ++j) asm volatile("" : "+v"(raw[j][0]), "+v"(raw[j][1]));
+        next_seen = copy_tile(k0);
+        lds_barrier();
+        const float *scale = s.scale[has_cmp ? 0 : 1];
+        const float first_peak = row_peak(largest<JN>(raw, j0, scale, g));
+        if (has_cmp && has_ori) ori_peak = row_peak(largest<JN>(raw, j0, s.scale[1], g));
+        q.set(first_peak, softmax2);
+        int8_t *stage = s.tile[(k0 + 1) & 1];
+#pragma unroll
+        for (int j = 0; j < JN; ++j)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                if (!SHARE) put(stage, j, h, raw[j][h], scale);
+                else put(stage, j0 + j, h, raw[j][h], scale);
+            }
+        take(stage);
+    }
+    auto parent_of = [&](int node) {
+        if (r.nodes <= PARENTS) {
+            const int up = s.parent[node];
+            return up == ROOT ? -1 : up;
+        }
+        const int up = gptr<int32_t>(p.parents)[r.first + node];
+        return up >= 0 && up < node ? up : -1;
+    };
+    // Thread t < tokens walks token t's chain, and says which of an original tile's rows the token sees.
+    if (has_ori && tid < tokens) {
+        int depth = 0;
+        for (int a = parent_of(token0 + tid); a >= 0; a = parent_of(a)) ++depth;
+        s.walk[tid] = token0 + tid, s.steps[tid] = 0, s.depth[tid] = depth;
+    }
+    auto make_mask = [&](int k, uint64_t rows_there) {
+        if (tid >= tokens) return;
+        // Committed rows (C + depth - window, C), then the ancestors.
+        const int base = base_of(k);
+        const int from = max(0, max(0, r.committed + s.depth[tid] + 1 - (int)min(p.window, 0x7fffffffu)) - base);
+        const int to = min(KEYS, r.committed - base);
+        uint64_t bits = 0;
+        if (from < to) bits = (~0ull >> (KEYS - to)) & (~0ull << from);
+        if (r.committed + r.nodes > base) {
+            int walk = s.walk[tid], steps = s.steps[tid];
+            for (; walk >= 0 && r.committed + walk >= base && (uint32_t)steps < p.window; walk = parent_of(walk), ++steps)
+                if (r.committed + walk < base + KEYS) bits |= 1ull << (r.committed + walk - base);
+            s.walk[tid] = walk, s.steps[tid] = steps;
+        }
+        s.mask[tid] = bits & rows_there;
+    };
+    if (k0 < k1 && k0 >= r.cmp_tiles) make_mask(k0, next_seen);
+
+    f32x4 acc[8][RT] = {};
+    float m = -INFINITY, sum = 0.0f;
+#pragma nounroll
+    for (int k = k0; k < k1; ++k) {
+        const bool window = k >= r.cmp_tiles;
+        seen = next_seen;
+        vm_wait_all();
+        lds_barrier();                                 // tile k is there; nobody uses tile k - 1 or its weights any more
+        if (window && k == r.cmp_tiles && k > k0) {
+            // From the compressed rows' channel scales to the original ones'.
+            load_scales();
+            lds_barrier();
+#pragma unroll
+            for (int ct = 0; ct < 8; ++ct) {
+                const int at = 128 * wave + 16 * ct + 4 * (again(lane) >> 4);
+                const f32x4 ratio = *reinterpret_cast<const f32x4 *>(s.scale[0] + at) / *reinterpret_cast<const f32x4 *>(s.scale[1] + at);
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) acc[ct][rt] *= ratio;
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            q.set(ori_peak, softmax2);
+            int8_t *stage = s.tile[(k + 1) & 1];
+#pragma unroll
+            for (int c = 0; c < JN; c += 2) {          // a few loads at a time: registers are short
+                u32x4 raw[2][2];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) raw[j][0] = q_at(j0 + c + j)[0], raw[j][1] = q_at(j0 + c + j)[1];
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        if (!SHARE) put(stage, c + j, h, raw[j][h], s.scale[1]);
+                        else put(stage, j0 + c + j, h, raw[j][h], s.scale[1]);
+                    }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            take(stage);
+            lds_barrier();
+        }
+        if (k + 1 < k1) {
+            if (!((k + 1) & 31)) read_entries((k + 1) >> 5);
+            next_seen = copy_tile(k + 1);
+        }
+        const int lx = again(lane), its_row = 16 * (wave % RT) + (lx & 15);
+        const uint32_t tile = (uint32_t)(uintptr_t)s.tile[k & 1];
+
+        // S = Q K^T: query row n, keys key0 + 16 kt + 4 g + i.
+        if (!window) {
+            const int left = r.compressed - k * KEYS;
+            if (left < KEYS) seen &= (1ull << left) - 1;
+        } else
+            seen = s.mask[s.token[its_row]];
+        float w[RT][4];
+        {
+            const uint32_t at = tile + (uint32_t)((key0 + (lx & 15)) * D + (((lx >> 4) ^ (lx & 15)) << 4));
+            constexpr int PAIR = RT == 2 ? 2 : 1, STEPS = 8 * RT / PAIR, AHEAD = 3;
+            // Step st: keys of tiles PAIR (st / 8) on, channels 64 (st % 8) on; reads run two steps ahead.
+            v4i key[AHEAD][PAIR];
+            auto fetch = [&](int st) {
+#pragma unroll
+                for (int kt = 0; kt < PAIR; ++kt)
+                    key[st % AHEAD][kt] = *(const lds_v4i *)(uintptr_t)((at ^ (uint32_t)(64 * (st & 7))) +
+                                                                       (uint32_t)(16 * (PAIR * (st >> 3) + kt) * D));
+            };
+            fetch(0);
+            fetch(1);
+            v4i dots[TERMS][PAIR];
+#pragma unroll
+            for (int st = 0; st < STEPS; ++st) {
+                if (st + 2 < STEPS) fetch(st + 2);
+                const int j = st & 7;
+#pragma unroll
+                for (int kt = 0; kt < PAIR; ++kt)
 #pragma unroll
                     for (int t = 0; t < TERMS; ++t)
-                        dots[t][kt] = __builtin_amdgcn_mfma_i32_16x16x64_i8(key, q.term[t][j], dots[t][kt], 0, 0, 0);
-                }
+                        dots[t][kt] = __builtin_amdgcn_mfma_i32_16x16x64_i8(key[st % AHEAD][kt], q.term[t][j],
+                                                                            j ? dots[t][kt] : v4i{0, 0, 0, 0}, 0, 0, 0);
+                if (j == 7)
 #pragma unroll
-            for (int kt = 0; kt < 2; ++kt) {
-                const uint32_t bits = (uint32_t)(mask >> (16 * (2 * kp + kt) + 4 * g)) & 15u;
+                    for (int kt = 0; kt < PAIR; ++kt)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    // At most 512 * 32512 * 128 + 512 * 128 * 128: within 32 bits.
-                    float x = (float)(dots[0][kt][i] * 256 + dots[1][kt][i]);
-                    if (TERMS == 3) x = __builtin_fmaf(x, 256.0f, (float)dots[TERMS - 1][kt][i]);
-                    w[2 * kp + kt][i] = bits >> i & 1 ? x * q.step : -INFINITY;
-                    peak = fmaxf(peak, w[2 * kp + kt][i]);
-                }
+                        for (int i = 0; i < 4; ++i) {
+                            // At most 512 * 32512 * 128 + 512 * 128 * 128: within 32 bits.
+                            float x = (float)(dots[0][kt][i] * 256 + dots[1][kt][i]);
+                            if (TERMS == 3) x = __builtin_fmaf(x, 256.0f, (float)dots[TERMS - 1][kt][i]);
+                            w[PAIR * (st >> 3) + kt][i] = x;
+                        }
+                __builtin_amdgcn_sched_barrier(0);
             }
-            __builtin_amdgcn_sched_barrier(0);
         }
-        peak = fmaxf(peak, __shfl_xor(peak, 16));
-        peak = fmaxf(peak, __shfl_xor(peak, 32));
+        if (__ballot(seen != ~0ull)) {
+#pragma unroll
+            for (int kt = 0; kt < RT; ++kt) {
+                const uint32_t bits = (uint32_t)(seen >> (key0 + 16 * kt + 4 * (lx >> 4))) & 15u;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[kt][i] = bits >> i & 1 ? w[kt][i] : -INFINITY;
+            }
+        }
+        float peak = -INFINITY;
+#pragma unroll
+        for (int kt = 0; kt < RT; ++kt) peak = fmaxf(fmaxf(fmaxf(peak, w[kt][0]), fmaxf(w[kt][1], w[kt][2])), w[kt][3]);
+        peak = row_max(peak);
+        if (PARTS > 1) {                               // the row's keys are spread over waves
+            if (lx < 16) s.peak[wave / RT][its_row] = peak;
+            lds_barrier();
+#pragma unroll
+            for (int part = 0; part < PARTS; ++part) peak = fmaxf(peak, s.peak[part][its_row]);
+        }
+        peak *= q.step;
         float factor = 1.0f;
         const bool move = peak > m + LIMIT;            // and where m is still -infinity
         if (move) {
@@ -367,100 +639,217 @@ __global__ void __launch_bounds__(THREADS, TERMS == 2 ? 2 : 1) tree_attention(co
             sum *= factor;
         }
         const bool any = __ballot(move) != 0;
-        if (lane == 0) s.moved[wave] = any;
-        if (any && g == 0) s.factor[row] = factor;
-#pragma unroll
-        for (int kt = 0; kt < 4; ++kt) {
-            const uint32_t bits = (uint32_t)(mask >> (16 * kt + 4 * g)) & 15u;
-            f16x4 half;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float x = bits >> i & 1 ? __builtin_amdgcn_exp2f(w[kt][i] - m) : 0.0f;
-                sum += x;
-                half[i] = (_Float16)x;
-            }
-            *reinterpret_cast<f16x4 *>(s.p + row * P_STRIDE + 16 * kt + 4 * g) = half;
+        if (wave < RT) {
+            if (lx == 0) s.moved[wave] = any;
+            if (any && lx < 16) s.factor[its_row] = factor;
         }
-        __syncthreads();
+        {
+            // Weights 2^(x step - m): 0 for masked keys, also where all have been masked so far.
+            const float from = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+            for (int kt = 0; kt < RT; ++kt) {
+                f16x4 half;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(w[kt][i], q.step, -from));
+                    sum += x;
+                    half[i] = (_Float16)x;
+                }
+                *reinterpret_cast<f16x4 *>(s.p + its_row * P_STRIDE + key0 + 16 * kt + 4 * (lx >> 4)) = half;
+            }
+        }
+        lds_barrier();
+        if (k + 1 < k1 && k + 1 >= r.cmp_tiles) make_mask(k + 1, next_seen);
 
         // acc[ct][rt]: channels 128 wave + 16 ct + 4 g + i, row 16 rt + n.
-        if (uni(s.moved[0] | s.moved[1] | s.moved[2] | s.moved[3])) {
-            f32x4 f;
+        int moved = 0;
 #pragma unroll
-            for (int rt = 0; rt < 4; ++rt) f[rt] = s.moved[rt] ? s.factor[16 * rt + n] : 1.0f;
+        for (int rt = 0; rt < RT; ++rt) moved |= s.moved[rt];
+        if (uni(moved)) {
+            float f[RT];
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) f[rt] = s.moved[rt] ? s.factor[16 * rt + (lx & 15)] : 1.0f;
 #pragma unroll
             for (int ct = 0; ct < 8; ++ct)
 #pragma unroll
-                for (int rt = 0; rt < 4; ++rt) acc[ct][rt] *= f[rt];
+                for (int rt = 0; rt < RT; ++rt) acc[ct][rt] *= f[rt];
         }
         __builtin_amdgcn_sched_barrier(0);
-        asm volatile("" : "+v"(lx));
+        {
+            const int lx = again(lane);
+            const int slot = 8 * (lx >> 4) + ((lx & 15) >> 1);
+            const uint32_t from = tile + (uint32_t)(slot * D + 8 * (lx & 1) + (((8 * wave) ^ (slot & 15)) << 4));
+            const _Float16 *its = s.p + (lx & 15) * P_STRIDE + 8 * (lx >> 4);
+            // Step st: channels 16 (st % 8) on of keys 32 (st / 8) on; reads run AHEAD steps ahead.
+            constexpr int AHEAD = 4;
+            v2i code[AHEAD];
+            auto fetch = [&](int st) {
+                code[st % AHEAD] = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                    (lds_v2i *)(uintptr_t)((from ^ (uint32_t)((st & 7) << 4)) + (uint32_t)(32 * (st >> 3) * D)));
+            };
+            f16x8 weight[RT];
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-            const int gx = lx >> 4, nx = lx & 15;
-            f16x8 weight[4];
+            for (int rt = 0; rt < RT; ++rt) weight[rt] = *reinterpret_cast<const f16x8 *>(its + 16 * rt * P_STRIDE);
 #pragma unroll
-            for (int rt = 0; rt < 4; ++rt)
-                weight[rt] = *reinterpret_cast<const f16x8 *>(s.p + (16 * rt + nx) * P_STRIDE + 32 * kb + 8 * gx);
-            const int slot = 32 * kb + 8 * gx + (nx >> 1);
-            const int8_t *from = s.tile + slot * D + 8 * (nx & 1);
+            for (int st = 0; st < AHEAD; ++st) fetch(st);
 #pragma unroll
-            for (int ct = 0; ct < 8; ++ct) {
-                const v2i code = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-                    (lds_v2i *)(from + (((8 * wave + ct) ^ (slot & 15)) << 4)));
-                const f16x8 value = to_f16(code);
+            for (int st = 0; st < 16; ++st) {
+                if (st == 8)
 #pragma unroll
-                for (int rt = 0; rt < 4; ++rt)
-                    acc[ct][rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(value, weight[rt], acc[ct][rt], 0, 0, 0);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-        }
-    };
-    if (r.cmp_tiles) {
-        encode<TERMS>(q, q_row, p.cmpScale, g, softmax2);
-        for (int k = 0; k < r.cmp_tiles; ++k) run_tile(k, false);
-    }
-    if (r.ori_tiles) {
-        encode<TERMS>(q, q_row, p.oriScale, g, softmax2);
-        if (r.cmp_tiles) {
-            // From the compressed rows' channel scales to the original ones'.
+                    for (int rt = 0; rt < RT; ++rt) weight[rt] = *reinterpret_cast<const f16x8 *>(its + 16 * rt * P_STRIDE + 32);
+                const f16x8 value = to_f16(code[st % AHEAD]);
+                if (st + AHEAD < 16) fetch(st + AHEAD);
 #pragma unroll
-            for (int ct = 0; ct < 8; ++ct) {
-                const int at = (128 * wave + 16 * ct + 4 * g) / 4;
-                const f32x4 ratio = gptr<f32x4>(p.cmpScale)[at] / gptr<f32x4>(p.oriScale)[at];
-#pragma unroll
-                for (int rt = 0; rt < 4; ++rt) acc[ct][rt] *= ratio;
+                for (int rt = 0; rt < RT; ++rt)
+                    acc[st & 7][rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(value, weight[rt], acc[st & 7][rt], 0, 0, 0);
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
-        for (int k = r.cmp_tiles; k < tiles; ++k) run_tile(k, true);
     }
     sum += __shfl_xor(sum, 16);
     sum += __shfl_xor(sum, 32);
-    if (g == 0) s.top[row] = m, s.sum[row] = sum;
-    __syncthreads();
-    const uint64_t scales = r.ori_tiles ? p.oriScale : p.cmpScale;
+    if (g == 0) {
+        s.sum[wave / RT][row] = sum;
+        if (wave < RT) s.top[row] = m;
+    }
+    lds_barrier();
+    auto row_sum = [&](int at) {
+        float total = s.sum[0][at];
 #pragma unroll
-    for (int rt = 0; rt < 4; ++rt) {
-        const int mine = 16 * rt + n;
-        if (mine >= rows) continue;
-        const float sink = gptr<float>(p.sinks)[(row0 + mine) % heads] * LOG2E;
-        const float most = s.top[mine];
-        const float top = fmaxf(most, sink);
-        // Where both are -infinity no key was seen and there is no sink; an infinite sink takes everything.
-        const float share = most == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(most - top);
-        const float rest = sink == top ? (top == -INFINITY ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(sink - top);
-        const float total = s.sum[mine] * share + rest;
-        const float give = share == 0.0f && !(total != total) ? 0.0f : share / total;
+        for (int part = 1; part < PARTS; ++part) total += s.sum[part][at];
+        return total;
+    };
+    // Values from code units.
+    {
+        const uint64_t scales = has_ori ? p.oriScale : p.cmpScale;
 #pragma unroll
         for (int ct = 0; ct < 8; ++ct) {
-            const int c = 128 * wave + 16 * ct + 4 * g;
-            const f32x4 v = acc[ct][rt] * give * gptr<f32x4>(scales)[c / 4];
-            *reinterpret_cast<u32x2 *>(p.out + (uint64_t)(out0 + mine) * (D * 2) + c * 2) =
+            const f32x4 scale = gptr<f32x4>(has_ori || has_cmp ? scales : p.oriScale)[(128 * wave + 16 * ct + 4 * g) / 4];
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) acc[ct][rt] *= scale;
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    float top[RT], total[RT];
+    if (splits == 1) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) top[rt] = s.top[16 * rt + n], total[rt] = row_sum(16 * rt + n);
+    } else {
+        // ---- states of the unit's items, joined by the last of them to finish ----
+        // Every store has completed (at the point where all XCDs see it) before the ticket is taken, and the states
+        // are added in the items' order, whichever is last.
+        const uint64_t first_item = (uint64_t)(item - part_no);
+        const bool near = (split & XCD_LOCAL) && (item - part_no) / share == (item - part_no + splits - 1) / share;
+        auto exchange = [&](auto policy_c) {
+            constexpr int POLICY = decltype(policy_c)::value;
+            {
+                const auto to = state_at(p.partial, (uint64_t)item, RT);
+#pragma unroll
+                for (int ct = 0; ct < 8; ++ct)
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt)
+                        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, acc[ct][rt]), to,
+                                                               ((ct * RT + rt) * THREADS + tid) * 16, 0, POLICY);
+                if (tid < ROWS) {
+                    __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(s.top[tid]), to, (ROWS * D + tid) * 4, 0, POLICY);
+                    __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(row_sum(tid)), to, (ROWS * (D + 1) + tid) * 4, 0,
+                                                          POLICY);
+                }
+            }
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+            __builtin_amdgcn_s_waitcnt(0);
+            __syncthreads();
+            uint32_t *ticket = reinterpret_cast<uint32_t *>(p.workspace) + unit0 + unit;
+            if (tid == 0) s.found[6] = (int)__hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __syncthreads();
+            if (s.found[6] != splits - 1) return false;
+            if (tid == 0) __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+            auto statistic = [&](int part, int rt, int which) {
+                return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
+                    state_at(p.partial, first_item + (uint64_t)part, RT), (ROWS * (D + which) + 16 * rt + n) * 4, 0, POLICY));
+            };
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) top[rt] = -INFINITY, total[rt] = 0.0f;
+            // Several states' loads at a time, as many as there are registers for.
+            constexpr int LOOK = RT == 4 ? 2 : 4, GROUP = RT == 1 ? 4 : RT == 2 ? 2 : 1;
+            for (int part = 0; part < splits; part += LOOK) {
+                float v[LOOK][RT];
+#pragma unroll
+                for (int u = 0; u < LOOK; ++u)
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) v[u][rt] = statistic(min(part + u, splits - 1), rt, 0);
+#pragma unroll
+                for (int u = 0; u < LOOK; ++u)
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) top[rt] = fmaxf(top[rt], v[u][rt]);
+            }
+#pragma unroll
+            for (int ct = 0; ct < 8; ++ct)
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) acc[ct][rt] = f32x4{0, 0, 0, 0};
+#pragma nounroll
+            for (int part = 0; part < splits; part += GROUP) {
+                float its[GROUP][RT], its_sum[GROUP][RT];
+#pragma unroll
+                for (int u = 0; u < GROUP; ++u)
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) {
+                        its[u][rt] = statistic(min(part + u, splits - 1), rt, 0);
+                        its_sum[u][rt] = statistic(min(part + u, splits - 1), rt, 1);
+                    }
+                constexpr int HALF = RT == 4 ? 2 : 8;
+#pragma unroll
+                for (int c0 = 0; c0 < 8; c0 += HALF) {
+                    f32x4 v[GROUP][HALF][RT];
+#pragma unroll
+                    for (int u = 0; u < GROUP; ++u) {
+                        const auto from = state_at(p.partial, first_item + (uint64_t)min(part + u, splits - 1), RT);
+#pragma unroll
+                        for (int ct = 0; ct < HALF; ++ct)
+#pragma unroll
+                            for (int rt = 0; rt < RT; ++rt)
+                                v[u][ct][rt] = __builtin_bit_cast(
+                                    f32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                               from, (((c0 + ct) * RT + rt) * THREADS + tid) * 16, 0, POLICY));
+                    }
+#pragma unroll
+                    for (int u = 0; u < GROUP; ++u)
+#pragma unroll
+                        for (int rt = 0; rt < RT; ++rt) {
+                            const bool some = part + u < splits && its[u][rt] != -INFINITY;
+                            const float f = some ? __builtin_amdgcn_exp2f(its[u][rt] - top[rt]) : 0.0f;
+                            if (part + u >= splits) continue;
+                            if (c0 == 0) total[rt] += its_sum[u][rt] * f;
+#pragma unroll
+                            for (int ct = 0; ct < HALF; ++ct) acc[c0 + ct][rt] += v[u][ct][rt] * f;
+                        }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+            return true;
+        };
+        if (!(near ? exchange(std::integral_constant<int, SC0>{}) : exchange(std::integral_constant<int, SC1>{}))) return;
+    }
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        const int at = 16 * rt + n;
+        if (at >= rows) continue;
+        const float sink = gptr<float>(p.sinks)[(row0 + at) % heads] * LOG2E;
+        const float most = top[rt], higher = fmaxf(most, sink);
+        // Where both are -infinity no key was seen and there is no sink; an infinite sink takes everything.
+        const float share = most == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(most - higher);
+        const float rest = sink == higher ? (higher == -INFINITY ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(sink - higher);
+        const float whole = total[rt] * share + rest;
+        const float give = share == 0.0f && !(whole != whole) ? 0.0f : share / whole;
+#pragma unroll
+        for (int ct = 0; ct < 8; ++ct) {
+            const f32x4 v = acc[ct][rt] * give;
+            *reinterpret_cast<u32x2 *>(p.out + (uint64_t)(out0 + at) * (D * 2) + (128 * wave + 16 * ct + 4 * g) * 2) =
                 u32x2{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
         }
         if (p.lse && wave == 0 && g == 0)
-            reinterpret_cast<float *>(p.lse)[out0 + mine] = top * LN2 + (total == 0.0f ? 0.0f : logf(total));
+            reinterpret_cast<float *>(p.lse)[out0 + at] = higher * LN2 + (whole == 0.0f ? 0.0f : logf(whole));
     }
 }
 
@@ -475,7 +864,37 @@ bool rejected(const TreeAttentionArgs *a)
                          (a->cmpStride & 15) || a->cmpStride < (uint64_t)PAGE_ROWS * D || ((a->cmp | a->cmpScale) & 15)))
         return true;
     // Rows and pages are counted in 32 bits.
-    return (uint64_t)a->tokens * a->heads > 0x7fff0000ull || a->oriTableWidth > 0x3ffffffu || a->cmpTableWidth > 0x3ffffffu;
+    return a->batch > 0xffffffu || (uint64_t)a->tokens * a->heads > 0x7fff0000ull || a->oriTableWidth > 0x3ffffffu ||
+           a->cmpTableWidth > 0x3ffffffu;
+}
+
+struct Plan {
+    int rt;
+    bool split;
+    uint32_t units, grid;
+};
+Plan plan_of(const TreeAttentionArgs *a)
+{
+    Plan plan;
+    const uint64_t rows = (uint64_t)a->tokens * a->heads;
+    const uint64_t cmp_tiles = a->ratio > 1 ? (a->cmpTableWidth + 1) / 2 : 0;
+    // Tiles that a request is likely to have: the window and trees of twice the average size, as far as the tables go.
+    const uint64_t near = (uint64_t)a->window + 2 * (a->tokens / a->batch + 1) + PAGE_ROWS;
+    const uint64_t ori_pages = near / PAGE_ROWS + 1 < a->oriTableWidth ? near / PAGE_ROWS + 1 : a->oriTableWidth;
+    const uint64_t work = (rows + 63) / 64 * (cmp_tiles + (ori_pages + 1) / 2);
+    // Units of 16 rows spread few rows over more work-groups and join smaller states; units of 64 rows read and convert
+    // a key's row for more of them.  In tiles of 64 rows and 64 keys (microseconds of 16, 32 and 64 rows a unit): 1
+    // request of 8 nodes, 4 tiles 14.2, 18.5, 34; 32 requests of 4-16 nodes, 400 tiles 26, 30, 66; 48 of 25 nodes, 750
+    // tiles 32, 30, 31; 16 of 24 nodes and 64 heads, 5400 tiles 147, 105, 94; 4 of 61 over 32 K rows, 31000 tiles 917,
+    // 311, 252.
+    plan.rt = work <= 600 ? 1 : work <= 2000 ? 2 : 4;
+    // A request's last unit may be short, and so may the padding's.
+    plan.units = (uint32_t)(rows / (16 * plan.rt)) + a->batch + 1;
+    const uint64_t tiles = cmp_tiles + (a->oriTableWidth + 1) / 2;
+    plan.split = plan.units <= ITEMS * 3 / 8 && tiles > 1;
+    const uint64_t items = plan.split ? plan.units * tiles : plan.units;
+    plan.grid = (uint32_t)((plan.split && items > ITEMS ? ITEMS : items) + 7) & ~7u;
+    return plan;
 }
 
 }  // namespace
@@ -486,11 +905,23 @@ int launch_sharedkv_tree(void *stream, const TreeAttentionArgs *a)
 {
     if (rejected(a)) return (int)hipErrorInvalidValue;
     if (!a->tokens) return (int)hipSuccess;
-    // A request's last unit may be short, and so may the padding's.
-    const uint32_t units = (uint32_t)((uint64_t)a->tokens * a->heads / ROWS) + a->batch + 1;
-    const auto kernel = a->lse ? &tree_attention<3> : &tree_attention<2>;
-    hipLaunchKernelGGL(kernel, dim3(units), dim3(THREADS), 0, static_cast<hipStream_t>(stream), *a);
+    const Plan plan = plan_of(a);
+    if (plan.split && (!a->workspace || !a->partial || ((a->workspace | a->partial) & 15))) return (int)hipErrorInvalidValue;
+    const auto kernel = plan.rt == 4   ? (a->lse ? &tree_attention<3, 4> : &tree_attention<2, 4>)
+                        : plan.rt == 2 ? (a->lse ? &tree_attention<3, 2> : &tree_attention<2, 2>)
+                                       : (a->lse ? &tree_attention<3, 1> : &tree_attention<2, 1>);
+    hipLaunchKernelGGL(kernel, dim3(plan.grid), dim3(THREADS), 0, static_cast<hipStream_t>(stream), *a,
+                       plan.split ? plan.units | (sharedkv::xcd_local(static_cast<hipStream_t>(stream)) ? XCD_LOCAL : 0u) : 0u);
     return (int)hipGetLastError();
+}
+
+int sharedkv_tree_scratch(const TreeAttentionArgs *a, uint64_t *workspace, uint64_t *partial)
+{
+    if (!workspace || !partial || rejected(a)) return (int)hipErrorInvalidValue;
+    const Plan plan = plan_of(a);
+    *workspace = plan.split ? plan.units * 4ull : 0;
+    *partial = plan.split ? plan.grid * state_floats(plan.rt) * 4 : 0;
+    return (int)hipSuccess;
 }
 
 uint32_t sharedkv_tree_args_size(void) { return (uint32_t)sizeof(TreeAttentionArgs); }

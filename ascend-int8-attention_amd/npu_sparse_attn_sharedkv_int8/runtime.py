@@ -97,7 +97,7 @@ EXPORTS = ("launch_sharedkv_c8_sparse", "launch_sharedkv_c8_dense", "launch_shar
            "sharedkv_c8_workspace_bytes", "sharedkv_c8_partial_bytes", "sharedkv_c8_noalloc_scratch_bytes",
            "sharedkv_c8_noalloc_layout", "sharedkv_c8_set_merge_mode", "sharedkv_c8_set_xcd_local",
            "sharedkv_c8_xcd_local", "sharedkv_attention_args_size", "sharedkv_cache_args_size",
-           "sharedkv_abi_version", "sharedkv_page_fork_workspace", "sharedkv_page_compact_workspace",
+           "sharedkv_abi_version", "sharedkv_tree_scratch", "sharedkv_page_fork_workspace", "sharedkv_page_compact_workspace",
            *(name for launch, _, size in BLOCK_LAUNCHES.values() for name in (launch, size)))
 
 
@@ -148,6 +148,9 @@ def library():
         getattr(lib, size).restype = ctypes.c_uint32
         if getattr(lib, size)() != ctypes.sizeof(block):
             raise RuntimeError(f"Native {block.__name__} ABI changed; rebuild the library")
+    lib.sharedkv_tree_scratch.argtypes = [ctypes.c_void_p, ctypes.POINTER(ctypes.c_uint64),
+                                          ctypes.POINTER(ctypes.c_uint64)]
+    lib.sharedkv_tree_scratch.restype = ctypes.c_int
     for name, count in (("sharedkv_page_fork_workspace", 3), ("sharedkv_page_compact_workspace", 1)):
         getattr(lib, name).argtypes = [ctypes.c_uint32] * count
         getattr(lib, name).restype = ctypes.c_uint64

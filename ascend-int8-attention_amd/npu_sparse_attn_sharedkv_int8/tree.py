@@ -27,7 +27,7 @@ import torch
 
 from .attention import _check_cache
 from .c8_attention import BLOCK, MAX_HEADS
-from .runtime import TreeAttentionArgs, native_launcher
+from .runtime import TreeAttentionArgs, library, native_launcher
 
 RATIOS = (1, 128)
 MAX_WINDOW = 2 ** 31 - 1
@@ -35,8 +35,10 @@ MAX_WINDOW = 2 ** 31 - 1
 
 class PreparedTreeAttention:
     """run() launches on the current stream of the inputs' device, allocates
-    nothing and reads nothing back.  Launches of one operator that may overlap
-    need an operator each.
+    nothing and reads nothing back.  Its scratch comes from
+    scratch_allocator(name, shape, dtype, device), by default a new tensor;
+    launches that may overlap must not share it (an operator each, or an
+    allocator by stream).
 
     Protocol: BF16 q[T, H, 512], 1..128 heads; INT8 caches [P, 32, 1, 512] with
     any page stride that is a multiple of 16 bytes; frozen FP32[512] scales;
@@ -46,7 +48,8 @@ class PreparedTreeAttention:
     with seq_lens 0, are graph padding: their outputs are zero.
     """
 
-    def __init__(self, case, parents, ori_scale, cmp_scale=None, *, output=None, return_lse=False, lse_output=None):
+    def __init__(self, case, parents, ori_scale, cmp_scale=None, *, output=None, return_lse=False, lse_output=None,
+                 scratch_allocator=None):
         q = case.q
         if q.device.type != "cuda" or q.dtype != torch.bfloat16 or q.ndim != 3 or q.shape[-1] != 512:
             raise ValueError("Expected BF16 Q[T,H,512] on a GPU")
@@ -90,6 +93,7 @@ class PreparedTreeAttention:
             self.args.cmpPages, self.args.cmpStride = case.cmp.shape[0], case.cmp.stride(0)
             self.args.cmpTableWidth, self.args.cmpScale = case.cmp_block_table.shape[1], cmp_scale.data_ptr()
         self._bind()
+        self._take_scratch(scratch_allocator, device)
         self.native = native_launcher()
         self.argument_address = ctypes.addressof(self.args)
         self.device_index = device.index if device.index is not None else torch.cuda.current_device()
@@ -102,6 +106,21 @@ class PreparedTreeAttention:
         if lse is not None and (tuple(lse.shape) != tuple(q.shape[:2]) or lse.dtype != torch.float32
                                 or lse.device != q.device or not lse.is_contiguous()):
             raise ValueError("Invalid FP32 LSE[T,H] output buffer")
+
+    def _take_scratch(self, allocator, device):
+        sizes = ctypes.c_uint64(), ctypes.c_uint64()
+        if self.args.tokens and library().sharedkv_tree_scratch(ctypes.addressof(self.args), *map(ctypes.byref, sizes)):
+            raise ValueError("This launch is outside the tree kernel's limits (2^31 query rows)")
+        allocate = allocator or (lambda name, shape, dtype, dev: torch.empty(shape, dtype=dtype, device=dev))
+        tickets, states = (size.value // 4 for size in sizes)
+        self.workspace = self.partial = None
+        if states:
+            # Merge tickets, which every launch leaves zero, and partition states.
+            self.workspace = allocate("tree_workspace", (tickets,), torch.int32, device)
+            self.partial = allocate("tree_partial", (states,), torch.float32, device)
+            self.workspace.zero_()
+            torch.cuda.current_stream(device).synchronize()      # run() may come on another stream
+            self.args.workspace, self.args.partial = self.workspace.data_ptr(), self.partial.data_ptr()
 
     def _bind(self):
         case, args = self.case, self.args

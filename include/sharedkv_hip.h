@@ -77,7 +77,9 @@ typedef struct CacheWriteArgs {
  * FP32 [heads]; lse FP32 [tokens][heads] or 0; ori / cmp INT8 pages of 32
  * rows of 512 bytes, page strides in bytes, multiples of 16.  Tokens of
  * requests with seqLens 0 and past cuQ[batch] are graph padding: their rows
- * of out and lse are zero-filled. */
+ * of out and lse are zero-filled.  workspace and partial: the scratch that
+ * sharedkv_tree_scratch names; the workspace is zero before the first launch,
+ * and each launch leaves it zero, so launches that may overlap need their own. */
 typedef struct TreeAttentionArgs {
     uint64_t q, ori, cmp, oriScale, cmpScale, oriTable, cmpTable, cuQ;
     uint64_t seqLens, sinks, parents, out, lse, workspace, partial;
@@ -225,8 +227,11 @@ int sharedkv_c8_attention_debug(void *stream, const SharedKVArgs *args, const Sh
  * slotColumnStride must fit 32 bits (else hipErrorInvalidValue). */
 int launch_cache_write(uint32_t blocks, void *stream, const CacheWriteArgs *args);
 
-/* Attention of drafted-token trees (TreeAttentionArgs). */
+/* Attention of drafted-token trees (TreeAttentionArgs), and the bytes of its
+ * scratch (0: none needed), a host-only query that reads everything but the
+ * workspace and partial fields. */
 int launch_sharedkv_tree(void *stream, const TreeAttentionArgs *args);
+int sharedkv_tree_scratch(const TreeAttentionArgs *args, uint64_t *workspace, uint64_t *partial);
 
 /* Accepted paths, and pages of a pool (argument blocks above).  pageBytes is
  * the sum of the caches' bytes and rowBytes the largest row's. */
