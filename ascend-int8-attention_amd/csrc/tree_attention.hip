@@ -81,6 +81,12 @@ __device__ __forceinline__ int again(int x)
     asm volatile("" : "+v"(x));
     return x;
 }
+// For stores: a flat store, which may reach LDS too, makes every later wait for an LDS read wait for all of them.
+template <typename T>
+__device__ __forceinline__ __attribute__((address_space(1))) T *gout(uint64_t a)
+{
+    return reinterpret_cast<__attribute__((address_space(1))) T *>(a);
+}
 __device__ __forceinline__ int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi)
 {
@@ -145,26 +151,16 @@ __device__ __forceinline__ float row_max(float v)
     return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
 }
 
-// Largest |q scale| of the lane's row among channels 64 j + 16 g .. + 15, j from j0 on; infinity where there is an
-// infinity or NaN.
-template <int JN>
-__device__ __forceinline__ float largest(const u32x4 (&raw)[JN][2], int j0, const float *scale, int g)
+// Products q * scale of the lane's channels 64 j + 16 g + 8 h on.
+struct Products {
+    float x[8];
+};
+__device__ __forceinline__ Products products(const u32x4 &w, const float *scale)
 {
-    float peak = 0.0f;
-    u16x2 bits = {0, 0};
+    Products out;
 #pragma unroll
-    for (int j = 0; j < JN; ++j)
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const uint32_t w = raw[j][h][e];
-                const float *s = scale + 64 * (j0 + j) + 16 * g + 8 * h + 2 * e;
-                peak = fmaxf(fmaxf(peak, fabsf(bf16_lo(w) * s[0])), fabsf(bf16_hi(w) * s[1]));
-                bits = __builtin_elementwise_max(bits, __builtin_bit_cast(u16x2, w & 0x7fff7fffu));
-            }
-    if (bits[0] >= 0x7f80 || bits[1] >= 0x7f80) peak = INFINITY;
-    return row_max(peak);
+    for (int e = 0; e < 8; ++e) out.x[e] = (e & 1 ? bf16_hi(w[e / 2]) : bf16_lo(w[e / 2])) * scale[e];
+    return out;
 }
 
 // q * scale as whole numbers of 8 * TERMS bits relative to the row's largest.
@@ -184,34 +180,42 @@ struct Codes {
         step = odd ? __builtin_nanf("") : some ? fmaxf(peak / LARGEST * fabsf(softmax2), 0x1p-126f) : 1.0f;
     }
     // Eight channels' codes: words [term][0 and 1].
-    __device__ __forceinline__ void make(uint32_t (&out)[TERMS][2], const u32x4 &w, const float *s) const
+    __device__ __forceinline__ void make(uint32_t (&out)[TERMS][2], const Products &from) const
     {
         uint32_t v[8];
+        if (TERMS == 2) {
+            // With 1.5 * 2^23 more, the nearest whole number sits in the low bits; with half of a byte's range more too,
+            // the second byte is rounded as the first, signed, byte wants it, and that one has its sign bit flipped.
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float x = e & 1 ? bf16_hi(w[e / 2]) : bf16_lo(w[e / 2]);
-            // 1.5 * 2^23 more: the nearest whole number sits in the low bits, the bytes above the lowest
-            // rounded by half of what is below them so that each byte is signed.
-            if (TERMS == 2) v[e] = __float_as_uint(__builtin_fmaf(x * s[e], inverse, 12582912.0f));
-            else v[e] = (uint32_t)(int)__builtin_rintf(x * s[e] * inverse);
+            for (int e = 0; e < 8; ++e)
+                v[e] = __float_as_uint(__builtin_fmaf(from.x[e], inverse, 12582912.0f + 128.0f));
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                const uint32_t *u = v + 4 * q;
+                const uint32_t ab = __builtin_amdgcn_perm(u[1], u[0], 0x05040100u), cd = __builtin_amdgcn_perm(u[3], u[2], 0x05040100u);
+                out[0][q] = __builtin_amdgcn_perm(cd, ab, 0x07050301u);
+                out[1][q] = __builtin_amdgcn_perm(cd, ab, 0x06040200u) ^ 0x80808080u;
+            }
+            return;
         }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = (uint32_t)(int)__builtin_rintf(from.x[e] * inverse);
 #pragma unroll
         for (int t = TERMS - 1; t >= 0; --t)
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
-                uint32_t u[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) u[e] = v[4 * q + e];
+                uint32_t *u = v + 4 * q;
                 const uint32_t ab = __builtin_amdgcn_perm(u[1], u[0], 0x0c0c0400u), cd = __builtin_amdgcn_perm(u[3], u[2], 0x04000c0cu);
                 out[t][q] = ab | cd;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[4 * q + e] = (v[4 * q + e] + 128) >> 8;
+                for (int e = 0; e < 4; ++e) u[e] = (u[e] + 128) >> 8;
             }
     }
 };
 
-// Eight codes to FP16, exactly: 1024 + (code + 128) has the byte as its low
-// mantissa bits.
+// Eight codes to FP16, exactly: 1024 + (code + 128) has the byte as its low mantissa bits.  (Left unsubtracted, as a
+// subnormal code + 128, the offset would save two fifths of these instructions, and round the sums of a long context
+// at 128 times their size.)
 __device__ __forceinline__ f16x8 to_f16(v2i w)
 {
     f16x8 out;
@@ -336,9 +340,9 @@ __global__ void __launch_bounds__(THREADS, TERMS == 2 || RT < 4 ? 2 : 1) tree_at
     }
     auto zero_rows = [&](int first, int count) {
         for (int i = tid; i < count * (D / 8); i += THREADS)
-            reinterpret_cast<u32x4 *>(p.out)[(int64_t)first * (D / 8) + i] = u32x4{0, 0, 0, 0};
+            gout<u32x4>(p.out)[(int64_t)first * (D / 8) + i] = u32x4{0, 0, 0, 0};
         if (p.lse)
-            for (int i = tid; i < count; i += THREADS) reinterpret_cast<float *>(p.lse)[first + i] = 0.0f;
+            for (int i = tid; i < count; i += THREADS) gout<float>(p.lse)[first + i] = 0.0f;
     };
     if (b < 0) {                                       // rows behind the last request
         const int64_t first = (int64_t)end + (int64_t)(item - (items - pad_units)) * ROWS;
@@ -441,9 +445,9 @@ __global__ void __launch_bounds__(THREADS, TERMS == 2 || RT < 4 ? 2 : 1) tree_at
     Codes<TERMS> q = {};
     auto stage_at = [&](int8_t *stage, int t, int j) { return stage + ((((wave % RT) * TERMS + t) * 8 + j) * 64 + lane) * 16; };
     // Codes of eight channels; where waves share a row tile they go to the staging buffer, whence all read them.
-    auto put = [&](int8_t *stage, int j, int h, const u32x4 &w, const float *scale) {
+    auto put = [&](int8_t *stage, int j, int h, const Products &x) {
         uint32_t out[TERMS][2];
-        q.make(out, w, scale + 64 * j + 16 * g + 8 * h);
+        q.make(out, x);
 #pragma unroll
         for (int t = 0; t < TERMS; ++t)
             if (!SHARE) q.term[t][j][2 * h] = (int)out[t][0], q.term[t][j][2 * h + 1] = (int)out[t][1];
@@ -476,17 +480,50 @@ __global__ void __launch_bounds__(THREADS, TERMS == 2 || RT < 4 ? 2 : 1) tree_at
         for (int j = 0; j < JN; ++j) asm volatile("" : "+v"(raw[j][0]), "+v"(raw[j][1]));
         next_seen = copy_tile(k0);
         lds_barrier();
-        const float *scale = s.scale[has_cmp ? 0 : 1];
-        const float first_peak = row_peak(largest<JN>(raw, j0, scale, g));
-        if (has_cmp && has_ori) ori_peak = row_peak(largest<JN>(raw, j0, s.scale[1], g));
-        q.set(first_peak, softmax2);
+        const float *scale = s.scale[has_cmp ? 0 : 1] + 64 * j0 + 16 * g;
         int8_t *stage = s.tile[(k0 + 1) & 1];
+        constexpr bool KEEP = JN <= 4;                 // few enough products to hold them
+        Products x[KEEP ? JN : 1][2];
+        float first_peak = 0.0f, second_peak = 0.0f;
+        u16x2 bits = {0, 0};
 #pragma unroll
         for (int j = 0; j < JN; ++j)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                if (!SHARE) put(stage, j, h, raw[j][h], scale);
-                else put(stage, j0 + j, h, raw[j][h], scale);
+                Products &at = x[KEEP ? j : 0][h];
+                at = products(raw[j][h], scale + 64 * j + 8 * h);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) first_peak = fmaxf(first_peak, fabsf(at.x[e]));
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    bits = __builtin_elementwise_max(bits, __builtin_bit_cast(u16x2, raw[j][h][e] & 0x7fff7fffu));
+                if (!KEEP) __builtin_amdgcn_sched_barrier(0);
+            }
+        if (has_cmp && has_ori)
+#pragma unroll
+            for (int j = 0; j < JN; ++j)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const Products at = products(raw[j][h], s.scale[1] + 64 * (j0 + j) + 16 * g + 8 * h);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) second_peak = fmaxf(second_peak, fabsf(at.x[e]));
+                    if (!KEEP) __builtin_amdgcn_sched_barrier(0);
+                }
+        if (bits[0] >= 0x7f80 || bits[1] >= 0x7f80) first_peak = second_peak = INFINITY;   // an infinity or NaN in the row
+        first_peak = row_peak(row_max(first_peak));
+        if (has_cmp && has_ori) ori_peak = row_peak(row_max(second_peak));
+        q.set(first_peak, softmax2);
+#pragma unroll
+        for (int j = 0; j < JN; ++j)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                if (!KEEP) {
+                    asm volatile("" : "+v"(raw[j][h]));   // made again, not held
+                    x[0][h] = products(raw[j][h], scale + 64 * j + 8 * h);
+                }
+                if (!SHARE) put(stage, j, h, x[KEEP ? j : 0][h]);
+                else put(stage, j0 + j, h, x[KEEP ? j : 0][h]);
+                if (!KEEP) __builtin_amdgcn_sched_barrier(0);
             }
         take(stage);
     }
@@ -504,8 +541,14 @@ __global__ void __launch_bounds__(THREADS, TERMS == 2 || RT < 4 ? 2 : 1) tree_at
         for (int a = parent_of(token0 + tid); a >= 0; a = parent_of(a)) ++depth;
         s.walk[tid] = token0 + tid, s.steps[tid] = 0, s.depth[tid] = depth;
     }
+    // Original tiles of committed rows that the deepest token's window still holds need no masks.
+    const int plain_from = max(0, r.committed + r.nodes - (int)min(p.window, 0x7fffffffu));
+    auto is_plain = [&](int k) {
+        const int base = base_of(k);
+        return k < r.cmp_tiles || (base >= plain_from && base + KEYS <= r.committed);
+    };
     auto make_mask = [&](int k, uint64_t rows_there) {
-        if (tid >= tokens) return;
+        if (is_plain(k) || tid >= tokens) return;
         // Committed rows (C + depth - window, C), then the ancestors.
         const int base = base_of(k);
         const int from = max(0, max(0, r.committed + s.depth[tid] + 1 - (int)min(p.window, 0x7fffffffu)) - base);
@@ -520,7 +563,7 @@ __global__ void __launch_bounds__(THREADS, TERMS == 2 || RT < 4 ? 2 : 1) tree_at
         }
         s.mask[tid] = bits & rows_there;
     };
-    if (k0 < k1 && k0 >= r.cmp_tiles) make_mask(k0, next_seen);
+    if (k0 < k1) make_mask(k0, next_seen);
 
     f32x4 acc[8][RT] = {};
     float m = -INFINITY, sum = 0.0f;
@@ -553,8 +596,9 @@ __global__ void __launch_bounds__(THREADS, TERMS == 2 || RT < 4 ? 2 : 1) tree_at
                 for (int j = 0; j < 2; ++j)
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        if (!SHARE) put(stage, c + j, h, raw[j][h], s.scale[1]);
-                        else put(stage, j0 + c + j, h, raw[j][h], s.scale[1]);
+                        const Products x = products(raw[j][h], s.scale[1] + 64 * (j0 + c + j) + 16 * g + 8 * h);
+                        if (!SHARE) put(stage, c + j, h, x);
+                        else put(stage, j0 + c + j, h, x);
                     }
                 __builtin_amdgcn_sched_barrier(0);
             }
@@ -569,11 +613,11 @@ __global__ void __launch_bounds__(THREADS, TERMS == 2 || RT < 4 ? 2 : 1) tree_at
         const uint32_t tile = (uint32_t)(uintptr_t)s.tile[k & 1];
 
         // S = Q K^T: query row n, keys key0 + 16 kt + 4 g + i.
+        const bool plain = is_plain(k);
         if (!window) {
             const int left = r.compressed - k * KEYS;
             if (left < KEYS) seen &= (1ull << left) - 1;
-        } else
-            seen = s.mask[s.token[its_row]];
+        }
         float w[RT][4];
         {
             const uint32_t at = tile + (uint32_t)((key0 + (lx & 15)) * D + (((lx >> 4) ^ (lx & 15)) << 4));
@@ -589,6 +633,7 @@ __global__ void __launch_bounds__(THREADS, TERMS == 2 || RT < 4 ? 2 : 1) tree_at
             fetch(0);
             fetch(1);
             v4i dots[TERMS][PAIR];
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int st = 0; st < STEPS; ++st) {
                 if (st + 2 < STEPS) fetch(st + 2);
@@ -612,10 +657,12 @@ __global__ void __launch_bounds__(THREADS, TERMS == 2 || RT < 4 ? 2 : 1) tree_at
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
-        if (__ballot(seen != ~0ull)) {
+        __builtin_amdgcn_s_setprio(0);
+        if (!plain || seen != ~0ull) {
+            const uint64_t its = plain ? seen : s.mask[s.token[its_row]];
 #pragma unroll
             for (int kt = 0; kt < RT; ++kt) {
-                const uint32_t bits = (uint32_t)(seen >> (key0 + 16 * kt + 4 * (lx >> 4))) & 15u;
+                const uint32_t bits = (uint32_t)(its >> (key0 + 16 * kt + 4 * (lx >> 4))) & 15u;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) w[kt][i] = bits >> i & 1 ? w[kt][i] : -INFINITY;
             }
@@ -652,58 +699,72 @@ __global__ void __launch_bounds__(THREADS, TERMS == 2 || RT < 4 ? 2 : 1) tree_at
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(w[kt][i], q.step, -from));
-                    sum += x;
+                    if (TERMS == 3) sum += x;          // the log-sum-exp's sum is of the weights before rounding
                     half[i] = (_Float16)x;
+                }
+                if (TERMS == 2) {                      // the output's, of the weights as P V takes them
+                    const f16x2 ones = {(_Float16)1.0f, (_Float16)1.0f};
+                    sum = __builtin_amdgcn_fdot2(f16x2{half[0], half[1]}, ones, sum, false);
+                    sum = __builtin_amdgcn_fdot2(f16x2{half[2], half[3]}, ones, sum, false);
                 }
                 *reinterpret_cast<f16x4 *>(s.p + its_row * P_STRIDE + key0 + 16 * kt + 4 * (lx >> 4)) = half;
             }
         }
         lds_barrier();
-        if (k + 1 < k1 && k + 1 >= r.cmp_tiles) make_mask(k + 1, next_seen);
+        if (k + 1 < k1) make_mask(k + 1, next_seen);
 
         // acc[ct][rt]: channels 128 wave + 16 ct + 4 g + i, row 16 rt + n.
-        int moved = 0;
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) moved |= s.moved[rt];
-        if (uni(moved)) {
-            float f[RT];
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) f[rt] = s.moved[rt] ? s.factor[16 * rt + (lx & 15)] : 1.0f;
-#pragma unroll
-            for (int ct = 0; ct < 8; ++ct)
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt) acc[ct][rt] *= f[rt];
-        }
-        __builtin_amdgcn_sched_barrier(0);
         {
             const int lx = again(lane);
             const int slot = 8 * (lx >> 4) + ((lx & 15) >> 1);
             const uint32_t from = tile + (uint32_t)(slot * D + 8 * (lx & 1) + (((8 * wave) ^ (slot & 15)) << 4));
             const _Float16 *its = s.p + (lx & 15) * P_STRIDE + 8 * (lx >> 4);
-            // Step st: channels 16 (st % 8) on of keys 32 (st / 8) on; reads run AHEAD steps ahead.
+            // Step st: channels 16 (st % 8) on of keys 32 (st / 8) on.  Reads run AHEAD steps ahead, and the next step's
+            // codes are converted between this step's matrix instructions.
             constexpr int AHEAD = 4;
             v2i code[AHEAD];
             auto fetch = [&](int st) {
                 code[st % AHEAD] = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
                     (lds_v2i *)(uintptr_t)((from ^ (uint32_t)((st & 7) << 4)) + (uint32_t)(32 * (st >> 3) * D)));
             };
-            f16x8 weight[RT];
+            f16x8 weight[RT], value[2];
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) weight[rt] = *reinterpret_cast<const f16x8 *>(its + 16 * rt * P_STRIDE);
 #pragma unroll
             for (int st = 0; st < AHEAD; ++st) fetch(st);
+            int moved = 0;
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) moved |= s.moved[rt];
+            if (uni(moved)) {
+                float f[RT];
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) f[rt] = s.moved[rt] ? s.factor[16 * rt + (lx & 15)] : 1.0f;
+#pragma unroll
+                for (int ct = 0; ct < 8; ++ct)
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) acc[ct][rt] *= f[rt];
+            }
+            value[0] = to_f16(code[0]);
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int st = 0; st < 16; ++st) {
                 if (st == 8)
 #pragma unroll
                     for (int rt = 0; rt < RT; ++rt) weight[rt] = *reinterpret_cast<const f16x8 *>(its + 16 * rt * P_STRIDE + 32);
-                const f16x8 value = to_f16(code[st % AHEAD]);
                 if (st + AHEAD < 16) fetch(st + AHEAD);
+                if (st + 1 < 16) value[(st + 1) & 1] = to_f16(code[(st + 1) % AHEAD]);
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt)
-                    acc[st & 7][rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(value, weight[rt], acc[st & 7][rt], 0, 0, 0);
+                    acc[st & 7][rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(value[st & 1], weight[rt], acc[st & 7][rt], 0, 0, 0);
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
+                    __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);              // one matrix instruction,
+                    __builtin_amdgcn_sched_group_barrier(0x2, 12 / RT, 0);         // then others
+                }
                 __builtin_amdgcn_sched_barrier(0);
             }
+            __builtin_amdgcn_s_setprio(0);
         }
     }
     sum += __shfl_xor(sum, 16);
@@ -721,10 +782,10 @@ __global__ void __launch_bounds__(THREADS, TERMS == 2 || RT < 4 ? 2 : 1) tree_at
     };
     // Values from code units.
     {
-        const uint64_t scales = has_ori ? p.oriScale : p.cmpScale;
+        const uint64_t scales = has_cmp && !has_ori ? p.cmpScale : p.oriScale;
 #pragma unroll
         for (int ct = 0; ct < 8; ++ct) {
-            const f32x4 scale = gptr<f32x4>(has_ori || has_cmp ? scales : p.oriScale)[(128 * wave + 16 * ct + 4 * g) / 4];
+            const f32x4 scale = gptr<f32x4>(scales)[(128 * wave + 16 * ct + 4 * g) / 4];
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) acc[ct][rt] *= scale;
             __builtin_amdgcn_sched_barrier(0);
@@ -759,7 +820,7 @@ __global__ void __launch_bounds__(THREADS, TERMS == 2 || RT < 4 ? 2 : 1) tree_at
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
             __builtin_amdgcn_s_waitcnt(0);
             __syncthreads();
-            uint32_t *ticket = reinterpret_cast<uint32_t *>(p.workspace) + unit0 + unit;
+            auto *ticket = gout<uint32_t>(p.workspace) + unit0 + unit;
             if (tid == 0) s.found[6] = (int)__hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             __syncthreads();
             if (s.found[6] != splits - 1) return false;
@@ -769,42 +830,27 @@ __global__ void __launch_bounds__(THREADS, TERMS == 2 || RT < 4 ? 2 : 1) tree_at
                 return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
                     state_at(p.partial, first_item + (uint64_t)part, RT), (ROWS * (D + which) + 16 * rt + n) * 4, 0, POLICY));
             };
+            // One pass, some channels and several states at a time: as many loads in flight as there are registers for.
+            constexpr int GROUP = RT == 4 ? 1 : 4 / RT, HALF = 8 / RT;
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) top[rt] = -INFINITY, total[rt] = 0.0f;
-            // Several states' loads at a time, as many as there are registers for.
-            constexpr int LOOK = RT == 4 ? 2 : 4, GROUP = RT == 1 ? 4 : RT == 2 ? 2 : 1;
-            for (int part = 0; part < splits; part += LOOK) {
-                float v[LOOK][RT];
+            for (int c0 = 0; c0 < 8; c0 += HALF) {
+                float high[RT], whole[RT];
 #pragma unroll
-                for (int u = 0; u < LOOK; ++u)
+                for (int rt = 0; rt < RT; ++rt) {
+                    high[rt] = -INFINITY, whole[rt] = 0.0f;
 #pragma unroll
-                    for (int rt = 0; rt < RT; ++rt) v[u][rt] = statistic(min(part + u, splits - 1), rt, 0);
-#pragma unroll
-                for (int u = 0; u < LOOK; ++u)
-#pragma unroll
-                    for (int rt = 0; rt < RT; ++rt) top[rt] = fmaxf(top[rt], v[u][rt]);
-            }
-#pragma unroll
-            for (int ct = 0; ct < 8; ++ct)
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt) acc[ct][rt] = f32x4{0, 0, 0, 0};
+                    for (int ct = 0; ct < HALF; ++ct) acc[c0 + ct][rt] = f32x4{0, 0, 0, 0};
+                }
 #pragma nounroll
-            for (int part = 0; part < splits; part += GROUP) {
-                float its[GROUP][RT], its_sum[GROUP][RT];
-#pragma unroll
-                for (int u = 0; u < GROUP; ++u)
-#pragma unroll
-                    for (int rt = 0; rt < RT; ++rt) {
-                        its[u][rt] = statistic(min(part + u, splits - 1), rt, 0);
-                        its_sum[u][rt] = statistic(min(part + u, splits - 1), rt, 1);
-                    }
-                constexpr int HALF = RT == 4 ? 2 : 8;
-#pragma unroll
-                for (int c0 = 0; c0 < 8; c0 += HALF) {
+                for (int part = 0; part < splits; part += GROUP) {
+                    float its[GROUP][RT], its_sum[GROUP][RT];
                     f32x4 v[GROUP][HALF][RT];
 #pragma unroll
                     for (int u = 0; u < GROUP; ++u) {
-                        const auto from = state_at(p.partial, first_item + (uint64_t)min(part + u, splits - 1), RT);
+                        const int at = min(part + u, splits - 1);
+                        const auto from = state_at(p.partial, first_item + (uint64_t)at, RT);
+#pragma unroll
+                        for (int rt = 0; rt < RT; ++rt) its[u][rt] = statistic(at, rt, 0), its_sum[u][rt] = statistic(at, rt, 1);
 #pragma unroll
                         for (int ct = 0; ct < HALF; ++ct)
 #pragma unroll
@@ -814,18 +860,28 @@ __global__ void __launch_bounds__(THREADS, TERMS == 2 || RT < 4 ? 2 : 1) tree_at
                                                from, (((c0 + ct) * RT + rt) * THREADS + tid) * 16, 0, POLICY));
                     }
 #pragma unroll
-                    for (int u = 0; u < GROUP; ++u)
+                    for (int rt = 0; rt < RT; ++rt) {
+                        float most = high[rt];
 #pragma unroll
-                        for (int rt = 0; rt < RT; ++rt) {
-                            const bool some = part + u < splits && its[u][rt] != -INFINITY;
-                            const float f = some ? __builtin_amdgcn_exp2f(its[u][rt] - top[rt]) : 0.0f;
+                        for (int u = 0; u < GROUP; ++u) most = fmaxf(most, its[u][rt]);
+                        const float from = most == -INFINITY ? 0.0f : most, keep = __builtin_amdgcn_exp2f(high[rt] - from);
+                        whole[rt] *= keep;
+#pragma unroll
+                        for (int ct = 0; ct < HALF; ++ct) acc[c0 + ct][rt] *= keep;
+#pragma unroll
+                        for (int u = 0; u < GROUP; ++u) {
                             if (part + u >= splits) continue;
-                            if (c0 == 0) total[rt] += its_sum[u][rt] * f;
+                            const float f = __builtin_amdgcn_exp2f(its[u][rt] - from);
+                            whole[rt] += its_sum[u][rt] * f;
 #pragma unroll
                             for (int ct = 0; ct < HALF; ++ct) acc[c0 + ct][rt] += v[u][ct][rt] * f;
                         }
+                        high[rt] = most;
+                    }
                     __builtin_amdgcn_sched_barrier(0);
                 }
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) top[rt] = high[rt], total[rt] = whole[rt];
             }
             return true;
         };
@@ -845,11 +901,11 @@ __global__ void __launch_bounds__(THREADS, TERMS == 2 || RT < 4 ? 2 : 1) tree_at
 #pragma unroll
         for (int ct = 0; ct < 8; ++ct) {
             const f32x4 v = acc[ct][rt] * give;
-            *reinterpret_cast<u32x2 *>(p.out + (uint64_t)(out0 + at) * (D * 2) + (128 * wave + 16 * ct + 4 * g) * 2) =
+            *gout<u32x2>(p.out + (uint64_t)(out0 + at) * (D * 2) + (128 * wave + 16 * ct + 4 * g) * 2) =
                 u32x2{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
         }
         if (p.lse && wave == 0 && g == 0)
-            reinterpret_cast<float *>(p.lse)[out0 + at] = higher * LN2 + (whole == 0.0f ? 0.0f : logf(whole));
+            gout<float>(p.lse)[out0 + at] = higher * LN2 + (whole == 0.0f ? 0.0f : logf(whole));
     }
 }
 
