@@ -330,7 +330,7 @@ def run_compact(rng, pages, share, rows=7, width=31, layers=2, gap=4096, inplace
     np.testing.assert_array_equal(flat.cpu().numpy(), want[4])
 
 
-@pytest.mark.parametrize("pages", [1, 2, 40, 2047, 2048, 2049, 6144, 10001])
+@pytest.mark.parametrize("pages", [1, 2, 40, 2047, 2048, 2049, 6144, 10001, 20001])
 @pytest.mark.parametrize("share", [0.0, 0.05, 0.5, 0.97, 1.0])
 def test_compact(pages, share):
     say(f"[compact] {pages} pages, {share} in use")
@@ -341,7 +341,8 @@ def test_compact(pages, share):
 @pytest.mark.parametrize("flatten", [False, True])
 def test_compact_in_place_and_flat_backing(inplace, flatten):
     say(f"[compact] in place {inplace}, flat {flatten}")
-    run_compact(np.random.default_rng(1), 3001, 0.4, rows=100, width=77, inplace=inplace, flatten=flatten)
+    for pages in (1500, 3001, 17000):
+        run_compact(np.random.default_rng(1), pages, 0.4, rows=100, width=77, inplace=inplace, flatten=flatten)
 
 
 def test_compact_pages_of_many_slices():
