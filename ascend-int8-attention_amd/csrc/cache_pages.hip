@@ -42,6 +42,19 @@ __device__ __forceinline__ __attribute__((address_space(1))) T *gout(uint64_t a)
     return reinterpret_cast<__attribute__((address_space(1))) T *>(a);
 }
 
+// Eight words from `at` on of an array of `count`, `other` past its end; in two loads where they may be.
+__device__ __forceinline__ void load_words(int (&v)[PER_THREAD], uint64_t array, int64_t at, int64_t count, int other)
+{
+    if (at + PER_THREAD <= count && !(array & 15)) {
+        const u32x4 a = gptr<u32x4>(array)[at / 4], b = gptr<u32x4>(array)[at / 4 + 1];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = (int)a[i], v[4 + i] = (int)b[i];
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < PER_THREAD; ++i) v[i] = at + i < count ? gptr<int32_t>(array)[at + i] : other;
+}
+
 // Sum over the work-group, in every thread.
 __device__ __forceinline__ int block_sum(int v)
 {
@@ -297,17 +310,14 @@ __global__ void __launch_bounds__(THREADS) fork_plan(const PageForkArgs p)
     }
     at -= p.rows;
     const int64_t page = (int64_t)at * CHUNK + tid * PER_THREAD;
-    bool spare[PER_THREAD];
-    int mine = 0;
+    int held[PER_THREAD], mine = 0;
+    load_words(held, p.refs, page, p.pages, 1);
 #pragma unroll
-    for (int i = 0; i < PER_THREAD; ++i) {
-        spare[i] = page + i < p.pages && refs[page + i] == 0;
-        mine += spare[i];
-    }
+    for (int i = 0; i < PER_THREAD; ++i) mine += held[i] == 0;
     int total, rank = block_before(mine, total);
 #pragma unroll
     for (int i = 0; i < PER_THREAD; ++i)
-        if (spare[i]) w.freed[(int64_t)at * CHUNK + rank++] = (int32_t)(page + i);
+        if (held[i] == 0) w.freed[(int64_t)at * CHUNK + rank++] = (int32_t)(page + i);
     if (tid == 0) w.count[at] = total;
 }
 
@@ -375,34 +385,31 @@ __global__ void __launch_bounds__(THREADS) fork_apply(const PageForkArgs p, uint
         return;
     }
     at -= p.children * slices;
-    int needed = 0;
+    const int64_t page = (int64_t)at * CHUNK + tid * PER_THREAD;
+    int held[PER_THREAD], change[PER_THREAD], mine = 0;
+    load_words(held, p.refs, page, p.pages, 1);
+    load_words(change, (uint64_t)(uintptr_t)w.delta, page, p.pages, 0);
+    int needed = 0, before = 0, free_pages = 0;
     for (int i = tid; i < (int)p.children; i += THREADS) needed += w.need[i];
-    needed = block_sum(needed);
-    int before = 0, free_pages = 0;
     for (int c = tid; c < chunks; c += THREADS) {
         free_pages += w.count[c];
         if (c < (int)at) before += w.count[c];
     }
+    needed = block_sum(needed);
     before = block_sum(before);
     if (at == 0) {
         free_pages = block_sum(free_pages);
         if (tid == 0) gout<int32_t>(p.missing)[0] = max(0, needed - free_pages);
     }
-    const int64_t page = (int64_t)at * CHUNK + tid * PER_THREAD;
-    int held[PER_THREAD], mine = 0;
 #pragma unroll
-    for (int i = 0; i < PER_THREAD; ++i) {
-        held[i] = page + i < p.pages ? gptr<int32_t>(p.refs)[page + i] : 1;
-        mine += held[i] == 0;
-    }
+    for (int i = 0; i < PER_THREAD; ++i) mine += held[i] == 0;
     int total, rank = before + block_before(mine, total);
 #pragma unroll
     for (int i = 0; i < PER_THREAD; ++i)
         if (page + i < p.pages) {
-            const int change = w.delta[page + i];
-            if (change) w.delta[page + i] = 0;
+            if (change[i]) w.delta[page + i] = 0;
             const int given = held[i] == 0 && rank++ < needed;
-            gout<int32_t>(p.newRefs)[page + i] = held[i] + change + given;
+            gout<int32_t>(p.newRefs)[page + i] = held[i] + change[i] + given;
         }
 }
 
@@ -476,11 +483,9 @@ __global__ void __launch_bounds__(THREADS) compact_plan(const PageCompactArgs p)
     }
     const int64_t page = (int64_t)chunk * CHUNK + tid * PER_THREAD;
     int held[PER_THREAD], mine = 0;
+    load_words(held, p.refs, page, p.pages, 0);
 #pragma unroll
-    for (int i = 0; i < PER_THREAD; ++i) {
-        held[i] = page + i < p.pages ? gptr<int32_t>(p.refs)[page + i] : 0;
-        mine += held[i] > 0;
-    }
+    for (int i = 0; i < PER_THREAD; ++i) mine += held[i] > 0;
     int total, rank = before + block_before(mine, total);
     if (few && tid == 0) w.count[chunk] = total;
 #pragma unroll
@@ -535,8 +540,7 @@ __global__ void __launch_bounds__(THREADS) compact_apply(const PageCompactArgs p
     const int live = gptr<int32_t>(p.live)[0];
     const int64_t page = (int64_t)at * CHUNK + tid * PER_THREAD;
     int held[PER_THREAD];
-#pragma unroll
-    for (int i = 0; i < PER_THREAD; ++i) held[i] = page + i < p.pages ? gptr<int32_t>(p.refs)[page + i] : 0;
+    load_words(held, p.refs, page, p.pages, 0);
     // Free pages of the chunk below L take the pages that move, in order: their rank is what is left of their index.
     int spare = 0;
 #pragma unroll
@@ -573,12 +577,9 @@ __global__ void __launch_bounds__(THREADS) compact_small(const PageCompactArgs p
     const bool has_entry = at >= copies && at < copies + table_groups && first < entries;
     const int entry = has_entry ? gptr<int32_t>(p.table)[first] : -1;
     int held[PER_THREAD], mine = 0;
+    load_words(held, p.refs, tid * PER_THREAD, p.pages, 0);
 #pragma unroll
-    for (int i = 0; i < PER_THREAD; ++i) {
-        const int page = tid * PER_THREAD + i;
-        held[i] = page < (int)p.pages ? gptr<int32_t>(p.refs)[page] : 0;
-        mine += held[i] > 0;
-    }
+    for (int i = 0; i < PER_THREAD; ++i) mine += held[i] > 0;
     int live, rank = block_before(mine, live), inside = 0;
 #pragma unroll
     for (int i = 0; i < PER_THREAD; ++i) inside += held[i] > 0 && tid * PER_THREAD + i < live;
