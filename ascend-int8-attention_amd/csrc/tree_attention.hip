@@ -44,7 +44,9 @@ constexpr int PARENTS = 1024;      // parents kept in LDS; larger trees read the
 constexpr int ROOT = 0xffff;
 constexpr int WHOLE = 0x3fffffff;  // tiles of an item where units are not split
 constexpr uint32_t MAX_HEADS = 128;
-constexpr uint32_t ITEMS = 512;    // two work-groups on each of 256 CUs
+// Items of a launch: two work-groups on each of 256 CUs; of small units, whose items differ most, half as many again (32
+// requests of 4-16 nodes: 25.7 us in at most 512 items, 23.1 in 768, 30.9 in 1024).
+__host__ __device__ constexpr uint32_t items_for(int rt) { return rt == 1 ? 768 : 512; }
 constexpr uint32_t XCD_LOCAL = 0x80000000u;   // bit of `split`: work-groups with one blockIdx modulo 8 share an XCD
 constexpr float LOG2E = 1.44269504088896341f, LN2 = 0.69314718055994531f;
 // Weights are 2^(s - m) with m the row's maximum less HEAD when it was last
@@ -124,7 +126,11 @@ struct Request {
     int32_t cmp_tiles, ori_tiles;
 };
 
-__device__ __forceinline__ Request request_of(const TreeAttentionArgs &p, int c0, int c1, int length)
+// The launch's sizes.
+struct Sizes {
+    uint32_t tokens, ratio, window, oriTableWidth, cmpTableWidth;
+};
+__device__ __forceinline__ Request request_of(const Sizes &p, int c0, int c1, int length)
 {
     Request r;
     const int tokens = (int)p.tokens;
@@ -253,28 +259,32 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t state_at(uint64_t partial, uin
 }
 
 template <int TERMS, int RT>
-__global__ void __launch_bounds__(THREADS, TERMS == 2 || RT < 4 ? 2 : 1) tree_attention(const TreeAttentionArgs p, const uint32_t split)
+__global__ void __launch_bounds__(THREADS, TERMS == 2 || RT < 4 ? 2 : 1) tree_attention(const uint64_t cu_q, const uint64_t seq_lens, const uint32_t batch_arg, const uint32_t heads_arg,
+               const uint32_t split, const uint32_t tokens_arg, const uint32_t ratio, const uint32_t window_rows,
+               const uint32_t ori_width, const uint32_t cmp_width, const TreeAttentionArgs p)
 {
+    const Sizes size = {tokens_arg, ratio, window_rows, ori_width, cmp_width};
     using S = Shared<RT>;
     constexpr int ROWS = S::ROWS, PARTS = S::PARTS;
     __shared__ S s;
     const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6), g = lane >> 4, n = lane & 15;
-    const int heads = (int)p.heads, batch = (int)p.batch;
-    const auto *cu = gptr<int32_t>(p.cuQ), *lens = gptr<int32_t>(p.seqLens);
+    // The leading arguments are the ones that the first loads need: the build preloads them into SGPRs.
+    const int heads = (int)heads_arg, batch = (int)batch_arg;
+    const auto *cu = gptr<int32_t>(cu_q), *lens = gptr<int32_t>(seq_lens);
 
     // ---- plan: units and tiles of the live requests, tiles of an item, this work-group's item ----
     auto units_of = [&](const Request &r) { return (r.nodes * heads + ROWS - 1) / ROWS; };
     Request mine = {};
     int units = 0, kinds = 0, work = 0;                // units, times their kinds, times their tiles
     for (int b = tid; b < batch; b += THREADS) {
-        mine = request_of(p, cu[b], cu[b + 1], lens[b]);
+        mine = request_of(size, cu[b], cu[b + 1], lens[b]);
         const int u = units_of(mine);
         units += u;
         kinds += u * max(1, (mine.cmp_tiles > 0) + (mine.ori_tiles > 0));
         work = (int)min((int64_t)u * (mine.cmp_tiles + mine.ori_tiles) + work, (int64_t)0x1ffffff);
     }
-    const int end = min(max(cu[batch], 0), (int)p.tokens) * heads;
-    const int all_rows = (int)p.tokens * heads, pad_units = (all_rows - end + ROWS - 1) / ROWS;
+    const int end = min(max(cu[batch], 0), (int)size.tokens) * heads;
+    const int all_rows = (int)size.tokens * heads, pad_units = (all_rows - end + ROWS - 1) / ROWS;
     units = wave_sum(units), kinds = wave_sum(kinds), work = wave_sum(work);
     if (lane == 0) s.scan[0][wave] = units, s.scan[1][wave] = kinds, s.scan[2][wave] = work;
     if (tid == 0) s.found[0] = -1;
@@ -283,12 +293,12 @@ __global__ void __launch_bounds__(THREADS, TERMS == 2 || RT < 4 ? 2 : 1) tree_at
     int64_t all_work = 0;
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) units += s.scan[0][w], kinds += s.scan[1][w], all_work += s.scan[2][w];
-    // Tiles of an item: as many as leave no more than ITEMS items (a unit's last of either kind may be short).
+    // Tiles of an item: as many as leave no more than items_for items (a unit's last of either kind may be short).
     // `split` is the number of units that the launch has scratch for: requests that lie one behind the other are never
     // more, and others are not split.
     int per_item = WHOLE;
     if (units <= (int)(split & ~XCD_LOCAL)) {
-        const int64_t room = (int64_t)ITEMS - kinds;
+        const int64_t room = (int64_t)items_for(RT) - kinds;
         per_item = (int)min((int64_t)WHOLE - 1, max((int64_t)1, (all_work + room - 1) / room));
     }
     // A unit that is split is split between its kinds too: Q is encoded with a kind's scales.
@@ -306,7 +316,7 @@ __global__ void __launch_bounds__(THREADS, TERMS == 2 || RT < 4 ? 2 : 1) tree_at
             const bool one_step = batch <= THREADS;
             for (int at = 0; at < batch; at += THREADS) {
                 const int b0 = at + tid;
-                if (!one_step) mine = b0 < batch ? request_of(p, cu[b0], cu[b0 + 1], lens[b0]) : Request{};
+                if (!one_step) mine = b0 < batch ? request_of(size, cu[b0], cu[b0 + 1], lens[b0]) : Request{};
                 const bool there = b0 < batch;
                 const int u = there ? units_of(mine) : 0, n_items = there ? u * items_of(mine) : 0;
                 upto = wave_upto(n_items), at_units = wave_upto(u);
@@ -350,7 +360,7 @@ __global__ void __launch_bounds__(THREADS, TERMS == 2 || RT < 4 ? 2 : 1) tree_at
         return;
     }
     b = uni(b);
-    const Request r = request_of(p, uni(s.found[3]), uni(s.found[4]), uni(s.found[5]));
+    const Request r = request_of(size, uni(s.found[3]), uni(s.found[4]), uni(s.found[5]));
     const int splits = items_of(r), local = uni(s.found[1]);
     const int part_no = local % splits;                // which of the unit's items
     unit = local / splits;
@@ -423,7 +433,8 @@ __global__ void __launch_bounds__(THREADS, TERMS == 2 || RT < 4 ? 2 : 1) tree_at
     const bool has_cmp = k0 < r.cmp_tiles && k0 < k1, has_ori = k1 > r.cmp_tiles;
     // The waves of a row tile encode a share of its channels each (64 j .. 64 j + 63, j from j0 on) and pass the codes
     // round in the tile buffer that is free.
-    constexpr bool SHARE = PARTS > 1 && RT * TERMS * 8 * 64 * 16 <= KEYS * D;
+    constexpr bool SHARE = PARTS > 1;
+    constexpr int AT_ONCE = KEYS * D / (RT * 8 * 64 * 16) > 0 ? KEYS * D / (RT * 8 * 64 * 16) : 1;   // terms that the buffer holds
     constexpr int JN = SHARE ? 8 / PARTS : 8;
     const int j0 = SHARE ? wave / RT * JN : 0;
     auto load_scales = [&]() {
@@ -432,6 +443,7 @@ __global__ void __launch_bounds__(THREADS, TERMS == 2 || RT < 4 ? 2 : 1) tree_at
             if (has_ori) reinterpret_cast<f32x4 *>(s.scale[1])[i] = gptr<f32x4>(p.oriScale)[i];
         }
     };
+    auto kept = [](float peak) { return peak == peak ? peak : INFINITY; };   // from here on infinity stands for both
     auto row_peak = [&](float mine_peak) {             // over the waves of the row tile
         if (!SHARE) return mine_peak;
         if (g == 0) s.peak[wave / RT][row] = mine_peak;
@@ -443,23 +455,34 @@ __global__ void __launch_bounds__(THREADS, TERMS == 2 || RT < 4 ? 2 : 1) tree_at
         return peak;
     };
     Codes<TERMS> q = {};
-    auto stage_at = [&](int8_t *stage, int t, int j) { return stage + ((((wave % RT) * TERMS + t) * 8 + j) * 64 + lane) * 16; };
-    // Codes of eight channels; where waves share a row tile they go to the staging buffer, whence all read them.
-    auto put = [&](int8_t *stage, int j, int h, const Products &x) {
+    auto stage_at = [&](int8_t *stage, int t, int j) { return stage + ((((wave % RT) * AT_ONCE + t) * 8 + j) * 64 + lane) * 16; };
+    // Codes of eight of the wave's channels; `own` are the wave's shares, j from j0 on.
+    v4i own[SHARE ? TERMS : 1][SHARE ? JN : 1];
+    auto put = [&](int j, int h, const Products &x) {
         uint32_t out[TERMS][2];
         q.make(out, x);
 #pragma unroll
-        for (int t = 0; t < TERMS; ++t)
-            if (!SHARE) q.term[t][j][2 * h] = (int)out[t][0], q.term[t][j][2 * h + 1] = (int)out[t][1];
-            else *reinterpret_cast<u32x2 *>(stage_at(stage, t, j) + 8 * h) = u32x2{out[t][0], out[t][1]};
+        for (int t = 0; t < TERMS; ++t) {
+            v4i &to = SHARE ? own[SHARE ? t : 0][SHARE ? j : 0] : q.term[t][j];
+            to[2 * h] = (int)out[t][0], to[2 * h + 1] = (int)out[t][1];
+        }
     };
+    // Every wave of a row tile gets all codes, some terms at a time through the staging buffer.
     auto take = [&](int8_t *stage) {
         if (!SHARE) return;
-        lds_barrier();
 #pragma unroll
-        for (int t = 0; t < TERMS; ++t)
+        for (int t0 = 0; t0 < TERMS; t0 += AT_ONCE) {
+            if (t0) lds_barrier();
 #pragma unroll
-            for (int j = 0; j < 8; ++j) q.term[t][j] = *reinterpret_cast<const v4i *>(stage_at(stage, t, j));
+            for (int t = t0; t < TERMS && t < t0 + AT_ONCE; ++t)
+#pragma unroll
+                for (int j = 0; j < JN; ++j) *reinterpret_cast<v4i *>(stage_at(stage, t - t0, j0 + j)) = own[SHARE ? t : 0][SHARE ? j : 0];
+            lds_barrier();
+#pragma unroll
+            for (int t = t0; t < TERMS && t < t0 + AT_ONCE; ++t)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) q.term[t][j] = *reinterpret_cast<const v4i *>(stage_at(stage, t - t0, j));
+        }
     };
     uint64_t seen = 0, next_seen = 0;
     float ori_peak = 0.0f;
@@ -484,8 +507,7 @@ __global__ void __launch_bounds__(THREADS, TERMS == 2 || RT < 4 ? 2 : 1) tree_at
         int8_t *stage = s.tile[(k0 + 1) & 1];
         constexpr bool KEEP = JN <= 4;                 // few enough products to hold them
         Products x[KEEP ? JN : 1][2];
-        float first_peak = 0.0f, second_peak = 0.0f;
-        u16x2 bits = {0, 0};
+        float first_peak = 0.0f, second_peak = 0.0f;   // maxima that keep a NaN
 #pragma unroll
         for (int j = 0; j < JN; ++j)
 #pragma unroll
@@ -493,10 +515,7 @@ __global__ void __launch_bounds__(THREADS, TERMS == 2 || RT < 4 ? 2 : 1) tree_at
                 Products &at = x[KEEP ? j : 0][h];
                 at = products(raw[j][h], scale + 64 * j + 8 * h);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) first_peak = fmaxf(first_peak, fabsf(at.x[e]));
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    bits = __builtin_elementwise_max(bits, __builtin_bit_cast(u16x2, raw[j][h][e] & 0x7fff7fffu));
+                for (int e = 0; e < 8; ++e) first_peak = __builtin_elementwise_maximum(first_peak, fabsf(at.x[e]));
                 if (!KEEP) __builtin_amdgcn_sched_barrier(0);
             }
         if (has_cmp && has_ori)
@@ -506,12 +525,11 @@ __global__ void __launch_bounds__(THREADS, TERMS == 2 || RT < 4 ? 2 : 1) tree_at
                 for (int h = 0; h < 2; ++h) {
                     const Products at = products(raw[j][h], s.scale[1] + 64 * (j0 + j) + 16 * g + 8 * h);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) second_peak = fmaxf(second_peak, fabsf(at.x[e]));
+                    for (int e = 0; e < 8; ++e) second_peak = __builtin_elementwise_maximum(second_peak, fabsf(at.x[e]));
                     if (!KEEP) __builtin_amdgcn_sched_barrier(0);
                 }
-        if (bits[0] >= 0x7f80 || bits[1] >= 0x7f80) first_peak = second_peak = INFINITY;   // an infinity or NaN in the row
-        first_peak = row_peak(row_max(first_peak));
-        if (has_cmp && has_ori) ori_peak = row_peak(row_max(second_peak));
+        first_peak = row_peak(row_max(kept(first_peak)));
+        if (has_cmp && has_ori) ori_peak = row_peak(row_max(kept(second_peak)));
         q.set(first_peak, softmax2);
 #pragma unroll
         for (int j = 0; j < JN; ++j)
@@ -521,8 +539,7 @@ __global__ void __launch_bounds__(THREADS, TERMS == 2 || RT < 4 ? 2 : 1) tree_at
                     asm volatile("" : "+v"(raw[j][h]));   // made again, not held
                     x[0][h] = products(raw[j][h], scale + 64 * j + 8 * h);
                 }
-                if (!SHARE) put(stage, j, h, x[KEEP ? j : 0][h]);
-                else put(stage, j0 + j, h, x[KEEP ? j : 0][h]);
+                put(j, h, x[KEEP ? j : 0][h]);
                 if (!KEEP) __builtin_amdgcn_sched_barrier(0);
             }
         take(stage);
@@ -597,8 +614,7 @@ __global__ void __launch_bounds__(THREADS, TERMS == 2 || RT < 4 ? 2 : 1) tree_at
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const Products x = products(raw[j][h], s.scale[1] + 64 * (j0 + c + j) + 16 * g + 8 * h);
-                        if (!SHARE) put(stage, c + j, h, x);
-                        else put(stage, j0 + c + j, h, x);
+                        put(c + j, h, x);
                     }
                 __builtin_amdgcn_sched_barrier(0);
             }
@@ -943,13 +959,14 @@ Plan plan_of(const TreeAttentionArgs *a)
     // request of 8 nodes, 4 tiles 14.2, 18.5, 34; 32 requests of 4-16 nodes, 400 tiles 26, 30, 66; 48 of 25 nodes, 750
     // tiles 32, 30, 31; 16 of 24 nodes and 64 heads, 5400 tiles 147, 105, 94; 4 of 61 over 32 K rows, 31000 tiles 917,
     // 311, 252.
-    plan.rt = work <= 600 ? 1 : work <= 2000 ? 2 : 4;
+    plan.rt = work <= 500 ? 1 : work <= 2000 ? 2 : 4;
     // A request's last unit may be short, and so may the padding's.
     plan.units = (uint32_t)(rows / (16 * plan.rt)) + a->batch + 1;
     const uint64_t tiles = cmp_tiles + (a->oriTableWidth + 1) / 2;
-    plan.split = plan.units <= ITEMS * 3 / 8 && tiles > 1;
+    const uint32_t most = items_for(plan.rt);
+    plan.split = plan.units <= most * 3 / 8 && tiles > 1;
     const uint64_t items = plan.split ? plan.units * tiles : plan.units;
-    plan.grid = (uint32_t)((plan.split && items > ITEMS ? ITEMS : items) + 7) & ~7u;
+    plan.grid = (uint32_t)((plan.split && items > most ? most : items) + 7) & ~7u;
     return plan;
 }
 
@@ -966,8 +983,10 @@ int launch_sharedkv_tree(void *stream, const TreeAttentionArgs *a)
     const auto kernel = plan.rt == 4   ? (a->lse ? &tree_attention<3, 4> : &tree_attention<2, 4>)
                         : plan.rt == 2 ? (a->lse ? &tree_attention<3, 2> : &tree_attention<2, 2>)
                                        : (a->lse ? &tree_attention<3, 1> : &tree_attention<2, 1>);
-    hipLaunchKernelGGL(kernel, dim3(plan.grid), dim3(THREADS), 0, static_cast<hipStream_t>(stream), *a,
-                       plan.split ? plan.units | (sharedkv::xcd_local(static_cast<hipStream_t>(stream)) ? XCD_LOCAL : 0u) : 0u);
+    const bool local = plan.split && sharedkv::xcd_local(static_cast<hipStream_t>(stream));
+    hipLaunchKernelGGL(kernel, dim3(plan.grid), dim3(THREADS), 0, static_cast<hipStream_t>(stream), a->cuQ, a->seqLens,
+                       a->batch, a->heads, (plan.split ? plan.units : 0u) | (local ? XCD_LOCAL : 0u), a->tokens, a->ratio,
+                       a->window, a->oriTableWidth, a->ratio > 1 ? a->cmpTableWidth : 0u, *a);
     return (int)hipGetLastError();
 }
 
