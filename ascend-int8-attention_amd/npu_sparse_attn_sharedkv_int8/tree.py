@@ -119,7 +119,8 @@ class PreparedTreeAttention:
             self.workspace = allocate("tree_workspace", (tickets,), torch.int32, device)
             self.partial = allocate("tree_partial", (states,), torch.float32, device)
             self.workspace.zero_()
-            torch.cuda.current_stream(device).synchronize()      # run() may come on another stream
+            if not torch.cuda.is_current_stream_capturing():
+                torch.cuda.current_stream(device).synchronize()  # run() may come on another stream
             self.args.workspace, self.args.partial = self.workspace.data_ptr(), self.partial.data_ptr()
 
     def _bind(self):

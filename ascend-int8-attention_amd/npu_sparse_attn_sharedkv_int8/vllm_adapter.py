@@ -37,6 +37,7 @@ from .cache import PreparedCacheWrite
 from .calibration import load_scale_file
 from .contract import SharedKVCase
 from .runtime import native_launcher
+from .tree import PreparedTreeAttention
 
 ARCH = "gfx950"
 OPERATORS_PER_LAYER = 8
@@ -255,13 +256,21 @@ class SharedKVLayer:
     # -- attention
     def attention(self, q, **kw):
         """The sparse attention call (keyword contract above); returns
-        (out BF16 [T, H, 512], lse FP32 [T, H, 1]) or (out, empty FP32)."""
+        (out BF16 [T, H, 512], lse FP32 [T, H, 1]) or (out, empty FP32).
+        With tree_parents (INT32 [T], each token's parent by its index in the
+        request) the tokens are the drafted trees of PreparedTreeAttention."""
         case, return_lse = parse_attention_call(q, kw)
+        parents = kw.get("tree_parents")
         out = torch.empty_like(q)
         lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
-        key = (launch_shape(case, return_lse), stream_key(q.device))
+        key = (launch_shape(case, return_lse), parents is not None, stream_key(q.device))
         op = self.operators.get(key)
-        if op is None:
+        if op is None and parents is not None:
+            op = PreparedTreeAttention(case, parents, self.scale("ori", q.device)[0],
+                                       self.scale("cmp", q.device)[0] if case.ratio > 1 else None, output=out,
+                                       lse_output=lse, scratch_allocator=scratch_allocator)
+            self.operators.put(key, op)
+        elif op is None:
             op = PreparedAttention(case, self.scale("ori", q.device)[0],
                                    self.scale("cmp", q.device)[0] if case.ratio > 1 else None,
                                    return_lse=return_lse, output=out, lse_output=lse,
@@ -270,6 +279,8 @@ class SharedKVLayer:
             if _rank_zero():
                 LOG.info("sharedKV attention %s: ratio %d, %d tokens x %d heads, %d KV partitions", self.prefix,
                          case.ratio, q.shape[0], q.shape[1], op.splits)
+        elif parents is not None:
+            op._rebind_same_geometry(case, parents, output=out, lse_output=lse)
         else:
             op._rebind_same_geometry(case, output=out, lse_output=lse)
         if torch.cuda.is_current_stream_capturing() and all(op is not c for c in self.captured):
@@ -277,7 +288,7 @@ class SharedKVLayer:
         op.run()
         # The caller owns the outputs (under capture: the graph's pool);
         # the operator keeps only its argument block and scratch.
-        op.case = op.out = op.lse = None
+        op.case = op.out = op.lse = op.parents = None
         if lse is not None:
             return out, lse.unsqueeze(-1)
         empty = self._empty_lse.get(q.device)
