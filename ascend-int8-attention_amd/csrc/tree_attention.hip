@@ -592,6 +592,9 @@ __global__ void __launch_bounds__(THREADS, TERMS == 2 || RT < 4 ? 2 : 1) tree_at
         lds_barrier();                                 // tile k is there; nobody uses tile k - 1 or its weights any more
         if (window && k == r.cmp_tiles && k > k0) {
             // From the compressed rows' channel scales to the original ones'.
+            u32x4 raw[JN][2];                          // in the registers of the compressed kind's codes
+#pragma unroll
+            for (int j = 0; j < JN; ++j) raw[j][0] = q_at(j0 + j)[0], raw[j][1] = q_at(j0 + j)[1];
             load_scales();
             lds_barrier();
 #pragma unroll
@@ -605,17 +608,10 @@ __global__ void __launch_bounds__(THREADS, TERMS == 2 || RT < 4 ? 2 : 1) tree_at
             q.set(ori_peak, softmax2);
             int8_t *stage = s.tile[(k + 1) & 1];
 #pragma unroll
-            for (int c = 0; c < JN; c += 2) {          // a few loads at a time: registers are short
-                u32x4 raw[2][2];
+            for (int j = 0; j < JN; ++j) {
 #pragma unroll
-                for (int j = 0; j < 2; ++j) raw[j][0] = q_at(j0 + c + j)[0], raw[j][1] = q_at(j0 + c + j)[1];
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const Products x = products(raw[j][h], s.scale[1] + 64 * (j0 + c + j) + 16 * g + 8 * h);
-                        put(c + j, h, x);
-                    }
+                for (int h = 0; h < 2; ++h)
+                    put(j, h, products(raw[j][h], s.scale[1] + 64 * (j0 + j) + 16 * (again(lane) >> 4) + 8 * h));
                 __builtin_amdgcn_sched_barrier(0);
             }
             take(stage);
