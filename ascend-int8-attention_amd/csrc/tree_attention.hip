@@ -47,6 +47,8 @@ constexpr uint32_t MAX_HEADS = 128;
 // Items of a launch: two work-groups on each of 256 CUs; of small units, whose items differ most, half as many again (32
 // requests of 4-16 nodes: 25.7 us in at most 512 items, 23.1 in 768, 30.9 in 1024).
 __host__ __device__ constexpr uint32_t items_for(int rt) { return rt == 1 ? 768 : 512; }
+// Tiles of a launch's units together, up to which a launch is split: they are summed over 64 lanes in 32 bits.
+constexpr uint64_t MAX_SPLIT_WORK = 0x1ffffff;
 constexpr uint32_t XCD_LOCAL = 0x80000000u;   // bit of `split`: work-groups with one blockIdx modulo 8 share an XCD
 constexpr float LOG2E = 1.44269504088896341f, LN2 = 0.69314718055994531f;
 // Weights are 2^(s - m) with m the row's maximum less HEAD when it was last
@@ -96,6 +98,17 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi)
 }
 __device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+
+// Scale in which a channel's numerator is held once original rows have joined the compressed ones: the original one,
+// unless that is so far below the compressed one that the quotient could overflow.  Raised, it is at most 2^-60 of the
+// compressed one, and so is what the original codes add.
+__device__ __forceinline__ f32x4 joint_scale(f32x4 cmp, f32x4 ori)
+{
+    f32x4 out;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out[i] = fmaxf(fmaxf(ori[i], cmp[i] * 0x1p-60f), 0x1p-149f);
+    return out;
+}
 
 // Tile addresses below are made by XOR within a row's 512 bytes.
 template <int RT>
@@ -281,7 +294,7 @@ __global__ void __launch_bounds__(THREADS, TERMS == 2 || RT < 4 ? 2 : 1) tree_at
         const int u = units_of(mine);
         units += u;
         kinds += u * max(1, (mine.cmp_tiles > 0) + (mine.ori_tiles > 0));
-        work = (int)min((int64_t)u * (mine.cmp_tiles + mine.ori_tiles) + work, (int64_t)0x1ffffff);
+        work = (int)min((int64_t)u * (mine.cmp_tiles + mine.ori_tiles) + work, (int64_t)MAX_SPLIT_WORK);
     }
     const int end = min(max(cu[batch], 0), (int)size.tokens) * heads;
     const int all_rows = (int)size.tokens * heads, pad_units = (all_rows - end + ROWS - 1) / ROWS;
@@ -600,7 +613,8 @@ __global__ void __launch_bounds__(THREADS, TERMS == 2 || RT < 4 ? 2 : 1) tree_at
 #pragma unroll
             for (int ct = 0; ct < 8; ++ct) {
                 const int at = 128 * wave + 16 * ct + 4 * (again(lane) >> 4);
-                const f32x4 ratio = *reinterpret_cast<const f32x4 *>(s.scale[0] + at) / *reinterpret_cast<const f32x4 *>(s.scale[1] + at);
+                const f32x4 cmp = *reinterpret_cast<const f32x4 *>(s.scale[0] + at);
+                const f32x4 ratio = cmp / joint_scale(cmp, *reinterpret_cast<const f32x4 *>(s.scale[1] + at));
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) acc[ct][rt] *= ratio;
                 __builtin_amdgcn_sched_barrier(0);
@@ -797,7 +811,8 @@ __global__ void __launch_bounds__(THREADS, TERMS == 2 || RT < 4 ? 2 : 1) tree_at
         const uint64_t scales = has_cmp && !has_ori ? p.cmpScale : p.oriScale;
 #pragma unroll
         for (int ct = 0; ct < 8; ++ct) {
-            const f32x4 scale = gptr<f32x4>(scales)[(128 * wave + 16 * ct + 4 * g) / 4];
+            f32x4 scale = gptr<f32x4>(scales)[(128 * wave + 16 * ct + 4 * g) / 4];
+            if (has_cmp && has_ori) scale = joint_scale(gptr<f32x4>(p.cmpScale)[(128 * wave + 16 * ct + 4 * g) / 4], scale);
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) acc[ct][rt] *= scale;
             __builtin_amdgcn_sched_barrier(0);
@@ -960,7 +975,7 @@ Plan plan_of(const TreeAttentionArgs *a)
     plan.units = (uint32_t)(rows / (16 * plan.rt)) + a->batch + 1;
     const uint64_t tiles = cmp_tiles + (a->oriTableWidth + 1) / 2;
     const uint32_t most = items_for(plan.rt);
-    plan.split = plan.units <= most * 3 / 8 && tiles > 1;
+    plan.split = plan.units <= most * 3 / 8 && tiles > 1 && plan.units * tiles <= MAX_SPLIT_WORK;
     const uint64_t items = plan.split ? plan.units * tiles : plan.units;
     plan.grid = (uint32_t)((plan.split && items > most ? most : items) + 7) & ~7u;
     return plan;

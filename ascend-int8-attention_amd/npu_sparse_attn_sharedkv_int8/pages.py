@@ -49,6 +49,46 @@ def _inner(cache, first):
     return run * cache.element_size()
 
 
+def _runs(c, dims):
+    """(start, strides of the first `dims` dimensions, bytes from the first to
+    the last of the dimensions from each on), all in bytes."""
+    size = c.element_size()
+    steps = tuple(s * size for s in c.stride()[:dims])
+    spans = [_inner(c, dims)]
+    for n, step in zip(reversed(c.shape[:dims]), reversed(steps)):
+        spans.append(spans[-1] + (n - 1) * step)
+    return c.data_ptr(), steps, spans[::-1]
+
+
+def _apart(a, b):
+    """Whether two caches (as _runs) share no byte: separate memory, or runs
+    that lie side by side in the same strides (layers interleaved in a pool's
+    pages, parts of its rows)."""
+    (at_a, steps, spans_a), (at_b, steps_b, spans_b) = a, b
+    ahead = at_b - at_a
+    if ahead >= spans_a[0] or -ahead >= spans_b[0]:
+        return True
+    if steps != steps_b:
+        return False
+    # In steps of one stride that every run of both keeps to.
+    return any(step and not any(s % step for s in steps[:level])
+               and spans_a[level + 1] <= ahead % step <= step - spans_b[level + 1]
+               for level, step in enumerate(steps))
+
+
+def _all_apart(caches, dims):
+    runs = sorted(_runs(c, dims) for c in caches)
+    if all(a[0] + a[2][0] <= b[0] for a, b in zip(runs, runs[1:])):
+        return True                                     # memory of their own
+    step = runs[0][1][0]
+    if step and all(r[1] == runs[0][1] for r in runs):
+        # Pages interleaved in one backing: neighbours within a stride, and the last to the next stride's first.
+        places = sorted((r[0] % step, r[2][1]) for r in runs)
+        if all(at + size <= after for (at, size), (after, _) in zip(places, places[1:] + [(places[0][0] + step, 0)])):
+            return True
+    return all(_apart(a, b) for i, a in enumerate(runs) for b in runs[:i])
+
+
 def _check_caches(caches, dims):
     """The caches as a list, after the checks all operators share: on one GPU,
     the same number of pages, each page (dims = 1) or row of a page (2) one run
@@ -68,6 +108,8 @@ def _check_caches(caches, dims):
             raise ValueError(f"Cache pages and rows must be contiguous in whole {UNIT}-byte units")
         if (c.shape[0] > 1 and c.stride(0) * size < span) or (dims == 2 and c.shape[1] > 1 and c.stride(1) * size < inner):
             raise ValueError("Cache pages and rows must not overlap")
+    if not _all_apart(caches, dims):
+        raise ValueError("Caches must not overlap")
     if not 1 <= leading[0] <= MAX_PAGES:
         raise ValueError(f"Expected 1..{MAX_PAGES} pages")
     return caches

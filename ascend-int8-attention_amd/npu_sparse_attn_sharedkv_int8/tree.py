@@ -27,6 +27,7 @@ import torch
 
 from .attention import _check_cache
 from .c8_attention import BLOCK, MAX_HEADS
+from .pages import _overlap
 from .runtime import TreeAttentionArgs, library, native_launcher
 
 RATIOS = (1, 128)
@@ -106,6 +107,10 @@ class PreparedTreeAttention:
         if lse is not None and (tuple(lse.shape) != tuple(q.shape[:2]) or lse.dtype != torch.float32
                                 or lse.device != q.device or not lse.is_contiguous()):
             raise ValueError("Invalid FP32 LSE[T,H] output buffer")
+        inputs = [q, self.parents, self.case.cu_q, self.case.seq_lens, self.case.sink]
+        if any(_overlap(out, x) for x in inputs + ([lse] if lse is not None else [])) \
+                or lse is not None and any(_overlap(lse, x) for x in inputs):
+            raise ValueError("Outputs must not overlap inputs or each other")
 
     def _take_scratch(self, allocator, device):
         sizes = ctypes.c_uint64(), ctypes.c_uint64()

@@ -464,6 +464,7 @@ def test_refusals():
     refuse("16-byte", lambda: PreparedPathCommit(cache.view(-1)[8:-504].view(-1, 1, 512), table, cu, seq, paths, lens))
     refuse("contiguous", lambda: PreparedPathCommit(cache.transpose(1, 3), table, cu, seq, paths, lens))
     refuse("overlap", lambda: PreparedPathCommit(cache.as_strided((9, 32, 512), (512, 512, 1)), table, cu, seq, paths, lens))
+    refuse("not overlap", lambda: PreparedPathCommit([cache, cache], table, cu, seq, paths, lens))
     refuse("cu_q", lambda: PreparedPathCommit(cache, table, cu[:2], seq, paths, lens))
     refuse("INT32", lambda: PreparedPathCommit(cache, table, cu, seq.long(), paths, lens))
     refuse("block_table", lambda: PreparedPathCommit(cache, table[:1], cu, seq, paths, lens))

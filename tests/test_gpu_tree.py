@@ -12,11 +12,17 @@ A = sum_j p_j |v_j|; the output's rounding adds 2^-8 |out|.  FP16 weights start
 at 2^8 for a row's largest and are multiples of 2^-24 at the low end, so each is
 off by 2^-25 besides, at most 2^-33 of the largest (which is at most the sum):
 2^-33 sum_j |v_j|, all that is left in a channel where every heavy key's code
-is 0.  The log-sum-exp is
+is 0.  Where a channel's original scale is below 2^-60 of the compressed one, a
+unit of both kinds takes 2^-60 of the compressed one, r, for it: with s the
+true scale, 0 < s < r, what the original rows add is off by
+(r - s) |sum_j p_j code_j| < r sum_j p_j |code_j| over the original rows, times
+1 + 2^-8 for the output's rounding and 1 + 2^-9 for the weights' (2^-6
+together); no term for other channels.  The log-sum-exp is
 off by d + 2^-22 (max|s| + |lse|) + 2^-20.
 """
 import math
 import sys
+import zlib
 
 import numpy as np
 import pytest
@@ -117,6 +123,7 @@ class Trees:
                     kinds.append((self.cmp, np.arange(c // self.ratio)))
                 t = self.cu[b] + i
                 scores, values, d = [], [], np.zeros(self.heads)
+                raised = []                     # |value| of the rows whose scale is raised, as raised
                 for kind, rows in kinds:
                     codes, good = self.rows(kind, b, rows)
                     codes, scale = codes[good], kind["scale"].astype(np.float64)
@@ -125,6 +132,8 @@ class Trees:
                     qs = q[t] * scale
                     scores.append(qs @ codes.T * self.softmax_scale)
                     values.append(codes * scale)
+                    least = self.cmp["scale"].astype(np.float64) * 2.0 ** -60 if self.cmp and kind is self.ori else scale
+                    raised.append(np.abs(codes) * np.where(scale < least, least, 0))
                     step = np.abs(qs).max(1) / (127 * 256 ** (terms - 1))
                     d = np.maximum(d, abs(self.softmax_scale) * step / 2 * np.abs(codes).sum(1).max())
                 sink = self.sink.astype(np.float64)
@@ -140,7 +149,8 @@ class Trees:
                 out[t] = p @ v
                 size = np.abs(s).max(1)
                 slack = 2 * (d + 2 ** -22 * size) + 2 ** -11 + 2 ** -18
-                near[t] = 2 ** -8 * np.abs(out[t]) + slack[:, None] * (p @ np.abs(v)) + 2 ** -33 * np.abs(v).sum(0)
+                near[t] = 2 ** -8 * np.abs(out[t]) + slack[:, None] * (p @ np.abs(v)) + 2 ** -33 * np.abs(v).sum(0) \
+                    + (1 + 2 ** -6) * (p @ np.concatenate(raised))
                 lse[t] = top + np.log(total)
                 lse_near[t] = d + 2 ** -22 * (size + np.abs(lse[t])) + 2 ** -20
         return out, near, lse, lse_near
@@ -194,7 +204,42 @@ SHAPES = [
 def test_matches_64_bits(shape, lse):
     nodes, committed, heads, ratio, window = shape
     say(f"[tree] {shape} lse={lse}")
-    check(Trees(hash(str(shape)) % 1000, nodes, committed, heads=heads, ratio=ratio, window=window), lse)
+    check(Trees(zlib.crc32(str(shape).encode()) % 1000, nodes, committed, heads=heads, ratio=ratio, window=window), lse)
+
+
+LAUNCHES = [
+    # split, nodes, committed, heads, ratio, window: units of 16, 32 and 64 rows
+    (False, [3] * 24, [0, 5, 127, 128, 200, 9000] * 4, 64, 128, 128),
+    (True, [12, 11], [6000, 4100], 128, 128, 1024),
+    (False, [14] * 10, [31, 4096, 127, 300, 9000, 1, 0, 640, 129, 8500], 64, 128, 128),
+    (True, [61, 57], [2000, 1531], 64, 1, ALL),
+    (False, [16] * 30, [0, 17, 128, 500, 9000, 700] * 5, 64, 128, 128),
+    (True, [61], [33000], 16, 1, ALL),             # many items of a unit
+    (True, [30, 1], [20000, 70], 128, 128, 1000),
+]
+
+
+@pytest.mark.parametrize("launch", LAUNCHES, ids=lambda s: f"{len(s[1])}x{max(s[1])}_c{max(s[2])}_h{s[3]}_r{s[4]}_w{s[5]}")
+@pytest.mark.parametrize("lse", [False, True], ids=["out", "lse"])
+def test_units_of_every_size(launch, lse):
+    """Units split over items and whole ones, which change from the compressed rows' scales to the original ones'."""
+    split, nodes, committed, heads, ratio, window = launch
+    say(f"[tree] {launch} lse={lse}")
+    op = check(Trees(zlib.crc32(str(launch).encode()) % 1000, nodes, committed, heads=heads, ratio=ratio, window=window), lse)
+    assert (op.partial is not None) == split
+
+
+@pytest.mark.parametrize("nodes,heads,batch", [(3, 64, 24), (14, 64, 10), (16, 64, 30)])
+def test_scales_far_apart(nodes, heads, batch):
+    """Channels whose original scale is far below the compressed one (their quotient passes FP32's range), and the other
+    way round, in units that hold both kinds."""
+    trees = Trees(22, [nodes] * batch, [200, 9000] * (batch // 2), heads=heads)
+    trees.ori["scale"][::7] = 1e-38
+    trees.ori["scale"][1::7] = 1e-8
+    trees.cmp["scale"][2::7] = 1e-38
+    trees.ori["scale"][3::7] = trees.cmp["scale"][3::7] = 1e-38
+    say(f"[tree] scales far apart, {batch} requests of {nodes} tokens")
+    assert check(trees, False).partial is None
 
 
 def test_chains_and_stars():
@@ -478,3 +523,5 @@ def test_refusals():
     refuse("metadata", case_field("cu_q", lambda t: t[:2].contiguous()))
     refuse("output", lambda a: a.update(output=torch.empty(8, 8, 512, device="cuda")))
     refuse("LSE", lambda a: a.update(lse_output=torch.empty(8, 7, device="cuda")))
+    refuse("overlap", lambda a: a.update(output=a["case"].q))
+    refuse("overlap", lambda a: a.update(lse_output=a["case"].q.view(torch.float32).reshape(-1)[:64].view(8, 8)))

@@ -80,6 +80,43 @@ def test_tree_scratch_covers_the_plan():
         assert fits, (tokens, heads, batch, width, sizes[0].value, sizes[1].value)
 
 
+def test_contexts_past_the_plans_sums_are_not_split():
+    """90 tokens of 128 heads over 12.8 M rows have 36 M tiles, more than the work-groups' sums hold."""
+    lib, a = runtime.library(), good_tree()
+    a.tokens, a.heads, a.ratio, a.window = 90, 128, 1, 2 ** 30
+    sizes = ctypes.c_uint64(), ctypes.c_uint64()
+    for width, split in ((100_000, True), (400_000, False)):
+        a.oriTableWidth = width
+        assert lib.sharedkv_tree_scratch(ctypes.addressof(a), *map(ctypes.byref, sizes)) == 0
+        assert (sizes[1].value > 0) == split
+
+
+def test_caches_of_a_pool_are_told_apart():
+    from npu_sparse_attn_sharedkv_int8.pages import _all_apart
+
+    def _apart(a, b, dims):
+        return _all_apart([a, b], dims)
+
+    flat = torch.zeros(22 * 4096, dtype=torch.int8)
+    layers = [flat.as_strided((20, 4, 512), (4096, 512, 1), k * 2048) for k in range(2)]
+    halves = [flat.as_strided((20, 8, 256), (4096, 512, 1), k * 256) for k in range(2)]
+    odd = [flat.as_strided((19, 8, 256), (4096 - 256, 512, 1), k * 256) for k in range(2)]
+    for dims in (1, 2):
+        assert _apart(*layers, dims) and _apart(*layers[::-1], dims)
+        assert not _apart(layers[0], layers[0], dims)
+        assert not _apart(layers[0], flat.as_strided((20, 4, 512), (4096, 512, 1), 1536), dims)
+        assert not _apart(layers[0], flat.as_strided((20, 4, 512), (4096, 512, 1), 4096 + 512), dims)
+        assert _apart(layers[0], torch.zeros(20, 4, 512, dtype=torch.int8), dims)
+        assert _apart(flat[:8192].view(2, 4096), flat[8192:].view(20, 4096), 1)
+    assert _apart(*halves, 2) and _apart(*halves[::-1], 2)
+    own = torch.zeros(20, 4, 512, dtype=torch.int8)
+    assert _all_apart([*layers, own], 2) and not _all_apart([*layers, own, layers[1]], 2)
+    many = [flat.as_strided((20, 4, 64), (4096, 64, 1), k * 256) for k in range(16)]
+    assert _all_apart(many[::-1], 1) and not _all_apart(many + [flat.as_strided((20, 4, 64), (4096, 64, 1), 128)], 2)
+    # Rows that lie side by side in a page, but not from page to page.
+    assert not _apart(*odd, 2) and not _apart(*odd[::-1], 2)
+
+
 def good_commit():
     a = runtime.PathCommitArgs(cacheCount=2, batch=3, depth=4, tokens=30, tableWidth=4, pages=9, pageRows=32, rowBytes=512)
     for name in "caches table cuQ seqLens paths pathLens lengths".split():
