@@ -44,7 +44,7 @@ class PreparedTreeAttention:
     Protocol: BF16 q[T, H, 512], 1..128 heads; INT8 caches [P, 32, 1, 512] with
     any page stride that is a multiple of 16 bytes; frozen FP32[512] scales;
     ratio 1 (window only) or 128 (and every compressed row); any window >= 1
-    (2**30 attends the whole context).  Rows on pages outside the pool or past
+    (2**30 attends the whole context); cu_q rises from 0.  Rows on pages outside the pool or past
     the block table are masked.  Tokens past cu_q[batch], and those of requests
     with seq_lens 0, are graph padding: their outputs are zero.
     """
@@ -119,12 +119,15 @@ class PreparedTreeAttention:
         allocate = allocator or (lambda name, shape, dtype, dev: torch.empty(shape, dtype=dtype, device=dev))
         tickets, states = (size.value // 4 for size in sizes)
         self.workspace = self.partial = None
+        self._unclear = False
         if states:
             # Merge tickets, which every launch leaves zero, and partition states.
             self.workspace = allocate("tree_workspace", (tickets,), torch.int32, device)
             self.partial = allocate("tree_partial", (states,), torch.float32, device)
-            self.workspace.zero_()
-            if not torch.cuda.is_current_stream_capturing():
+            # Under capture a clear only becomes part of that graph: run() then clears too, until it has done so eagerly.
+            self._unclear = torch.cuda.is_current_stream_capturing()
+            if not self._unclear:
+                self.workspace.zero_()
                 torch.cuda.current_stream(device).synchronize()  # run() may come on another stream
             self.args.workspace, self.args.partial = self.workspace.data_ptr(), self.partial.data_ptr()
 
@@ -146,6 +149,9 @@ class PreparedTreeAttention:
 
     def run(self):
         """Launch on the current stream of the case's device; returns .out."""
+        if self._unclear:
+            self.workspace.zero_()
+            self._unclear = torch.cuda.is_current_stream_capturing()
         if self.args.tokens:
             self.native.launch("tree_attention", self.argument_address, self.device_index)
         return self.out

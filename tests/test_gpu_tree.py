@@ -451,6 +451,32 @@ def test_graph_replays_and_rebinding():
     torch.cuda.synchronize()
 
 
+def test_made_under_capture():
+    """Scratch that is not clear, first seen under capture: an eager run and a second graph before the first's replay."""
+    import torch
+    from npu_sparse_attn_sharedkv_int8 import PreparedTreeAttention
+    trees = Trees(23, [7, 12], [500, 4000])
+    case, parents, scale, cmp_scale = trees.device()
+    PreparedTreeAttention(case, parents, scale, cmp_scale, return_lse=True).run()
+    dirty = {"tree_workspace": torch.full((1 << 10,), 7, dtype=torch.int32, device="cuda"),
+             "tree_partial": torch.full((1 << 23,), float("nan"), device="cuda")}
+    torch.cuda.synchronize()
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    with torch.cuda.graph(graphs[0]):
+        op = PreparedTreeAttention(case, parents, scale, cmp_scale, return_lse=True,
+                                   scratch_allocator=lambda name, shape, dtype, device: dirty[name][:shape[0]])
+        op.run()
+    with torch.cuda.graph(graphs[1]):
+        op.run()
+    assert op.partial is not None
+    for step in (graphs[1].replay, op.run, graphs[0].replay, op.run, graphs[1].replay):
+        op.out.fill_(float("nan"))
+        say("[tree] a run of an operator made under capture")
+        step()
+        torch.cuda.synchronize()
+        compare(op, trees, True)
+
+
 def test_another_stream():
     import torch
     from npu_sparse_attn_sharedkv_int8 import PreparedTreeAttention
