@@ -23,6 +23,15 @@
 // a ring of two, one in flight while the other is used.  Every work-group makes
 // the same plan from the live lengths (which requests there are, how many tiles
 // an item gets), and the last item of a unit to finish joins the unit's states.
+//
+// What bounds it.  4 * 512 flops for every 512-byte key and query row: from some
+// hundred rows a request on, the matrix instructions and the vector ones beside
+// them (a key's codes to FP16, the softmax).  4 requests of 57-61 tokens and 16
+// heads over 20-32 K rows take 236 us, 860 TFLOP/s, three quarters of a large
+// library FP16 product's rate; 2048 of the 4900 cycles that a wave spends on a
+// tile are matrix instructions, about 1850 vector ones.  Small launches are a chain of
+// round trips (lengths, Q and tables, tiles, states): one request of 8 tokens and
+// 4096 rows takes 13.5 us, 32 of 4-16 tokens 22.6.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -46,7 +55,7 @@ constexpr int WHOLE = 0x3fffffff;  // tiles of an item where units are not split
 constexpr uint32_t MAX_HEADS = 128;
 constexpr int CUS = 256;
 // Items of a launch: two work-groups on each of 256 CUs; of small units, whose items differ most, half as many again (32
-// requests of 4-16 nodes: 25.7 us in at most 512 items, 23.1 in 768, 30.9 in 1024).
+// requests of 4-16 nodes: 24.8 us in at most 512 items, 22.7 in 768, 30.1 in 1024).
 __host__ __device__ constexpr uint32_t items_for(int rt) { return rt == 1 ? 768 : 512; }
 // Tiles of a launch's units together, up to which a launch is split: they are summed over 64 lanes in 32 bits.
 constexpr uint64_t MAX_SPLIT_WORK = 0x1ffffff;
@@ -476,7 +485,7 @@ __global__ void __launch_bounds__(THREADS, TERMS == 2 || RT < 4 ? 2 : 1) tree_at
     constexpr int JN = SHARE ? 8 / PARTS : 8;
     const int j0 = SHARE ? wave / RT * JN : 0;
     auto load_scales = [&]() {
-        for (int i = tid; i < D / 4; i += THREADS) {
+        for (int i = RT == 4 ? again(tid) : tid; i < D / 4; i += THREADS) {
             if (has_cmp) reinterpret_cast<f32x4 *>(s.scale[0])[i] = gptr<f32x4>(p.cmpScale)[i];
             if (has_ori) reinterpret_cast<f32x4 *>(s.scale[1])[i] = gptr<f32x4>(p.oriScale)[i];
         }
@@ -603,20 +612,21 @@ __global__ void __launch_bounds__(THREADS, TERMS == 2 || RT < 4 ? 2 : 1) tree_at
         return k < r.cmp_tiles || (base >= plain_from && base + KEYS <= r.committed);
     };
     auto make_mask = [&](int k, uint64_t rows_there) {
-        if (is_plain(k) || tid >= tokens) return;
+        const int at = tid;
+        if (is_plain(k) || at >= tokens) return;
         // Committed rows (C + depth - window, C), then the ancestors.
         const int base = base_of(k);
-        const int from = max(0, max(0, r.committed + s.depth[tid] + 1 - (int)min(p.window, 0x7fffffffu)) - base);
+        const int from = max(0, max(0, r.committed + s.depth[at] + 1 - (int)min(p.window, 0x7fffffffu)) - base);
         const int to = min(KEYS, r.committed - base);
         uint64_t bits = 0;
         if (from < to) bits = (~0ull >> (KEYS - to)) & (~0ull << from);
         if (r.committed + r.nodes > base) {
-            int walk = s.walk[tid], steps = s.steps[tid];
+            int walk = s.walk[at], steps = s.steps[at];
             for (; walk >= 0 && r.committed + walk >= base && (uint32_t)steps < p.window; walk = parent_of(walk), ++steps)
                 if (r.committed + walk < base + KEYS) bits |= 1ull << (r.committed + walk - base);
-            s.walk[tid] = walk, s.steps[tid] = steps;
+            s.walk[at] = walk, s.steps[at] = steps;
         }
-        s.mask[tid] = bits & rows_there;
+        s.mask[at] = bits & rows_there;
     };
     if (k0 < k1) make_mask(k0, next_seen);
 
@@ -684,6 +694,8 @@ __global__ void __launch_bounds__(THREADS, TERMS == 2 || RT < 4 ? 2 : 1) tree_at
             fetch(0);
             fetch(1);
             v4i dots[TERMS][PAIR];
+            // Matrix instructions before the other work-group's vector ones, here and in P V (16 requests of 24 nodes and
+            // 64 heads, and 4 of 61 over 32 K rows: 80.6 and 236 us, 83.7 and 252 without).
             __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int st = 0; st < STEPS; ++st) {
@@ -718,9 +730,11 @@ __global__ void __launch_bounds__(THREADS, TERMS == 2 || RT < 4 ? 2 : 1) tree_at
                 for (int i = 0; i < 4; ++i) w[kt][i] = bits >> i & 1 ? w[kt][i] : -INFINITY;
             }
         }
-        float peak = -INFINITY;
+        float peak = -INFINITY;                        // scores are no NaN: units, or -infinity
 #pragma unroll
-        for (int kt = 0; kt < RT; ++kt) peak = fmaxf(fmaxf(fmaxf(peak, w[kt][0]), fmaxf(w[kt][1], w[kt][2])), w[kt][3]);
+        for (int kt = 0; kt < RT; ++kt)
+#pragma unroll
+            for (int i = 0; i < 4; i += 2) peak = __builtin_elementwise_maxnum(__builtin_elementwise_maxnum(peak, w[kt][i]), w[kt][i + 1]);
         peak = row_max(peak);
         if (PARTS > 1) {                               // the row's keys are spread over waves
             if (lx < 16) s.peak[wave / RT][its_row] = peak;
@@ -992,9 +1006,9 @@ Plan plan_of(const TreeAttentionArgs *a)
     const uint64_t work = (rows + 63) / 64 * (cmp_tiles + (ori_pages + 1) / 2);
     // Units of 16 rows spread few rows over more work-groups and join smaller states; units of 64 rows read and convert
     // a key's row for more of them.  In tiles of 64 rows and 64 keys (microseconds of 16, 32 and 64 rows a unit): 1
-    // request of 8 nodes, 4 tiles 14.2, 18.5, 34; 32 requests of 4-16 nodes, 400 tiles 26, 30, 66; 48 of 25 nodes, 750
-    // tiles 32, 30, 31; 16 of 24 nodes and 64 heads, 5400 tiles 147, 105, 94; 4 of 61 over 32 K rows, 31000 tiles 917,
-    // 311, 252.
+    // request of 8 nodes, 4 tiles 13.5, 18.2, 34.7; 32 requests of 4-16 nodes, 400 tiles 22.7, 28.8, 64; 48 of 25 nodes,
+    // 750 tiles 31.5, 24.6, 33.4; 16 of 24 nodes and 64 heads, 5400 tiles 140, 112, 79; 4 of 61 over 32 K rows, 31000
+    // tiles 626, 284, 236.
     plan.rt = work <= 500 ? 1 : work <= 2000 ? 2 : 4;
     // A request's last unit may be short, and so may the padding's.
     plan.units = (uint32_t)(rows / (16 * plan.rt)) + a->batch + 1;
