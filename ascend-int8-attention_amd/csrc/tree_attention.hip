@@ -28,8 +28,8 @@
 // hundred rows a request on, the matrix instructions and the vector ones beside
 // them (a key's codes to FP16, the softmax).  4 requests of 57-61 tokens and 16
 // heads over 20-32 K rows take 236 us, 860 TFLOP/s, three quarters of a large
-// library FP16 product's rate; 2048 of the 4900 cycles that a wave spends on a
-// tile are matrix instructions, about 1850 vector ones.  Small launches are a chain of
+// library FP16 product's rate; a SIMD takes about 4960 cycles for a wave's tile,
+// 2048 of them busy with matrix instructions, beside some 420 vector ones.  Small launches are a chain of
 // round trips (lengths, Q and tables, tiles, states): one request of 8 tokens and
 // 4096 rows takes 13.5 us, 32 of 4-16 tokens 22.6.
 #include <hip/hip_runtime.h>
