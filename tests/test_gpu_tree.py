@@ -242,6 +242,38 @@ def test_scales_far_apart(nodes, heads, batch):
     assert check(trees, False).partial is None
 
 
+@pytest.mark.parametrize("batch,heads", [(40, 64), (20, 64), (70, 32)])
+def test_whole_units_beside_padding(batch, heads):
+    """Units of 64 rows in the order of their length (more than 512 of them, fewer, and more requests than a wave has
+    lanes, in their own order), with requests that are padding between live ones and tokens behind them."""
+    import torch
+    from npu_sparse_attn_sharedkv_int8 import PreparedTreeAttention
+    committed = [0, 17, 128, 500, 9000, 700, 3, 1290, 8000, 65]
+    trees = Trees(24, [16] * batch, [committed[b % 10] for b in range(batch)], heads=heads, pad_tokens=9, pad_batch=2)
+    case, parents, scale, cmp_scale = trees.device()
+    dead = list(range(3, batch, 7))
+    case.seq_lens[dead] = 0
+    op = PreparedTreeAttention(case, parents, scale, cmp_scale)
+    assert op.partial is None
+    op.out.fill_(float("nan"))
+    say(f"[tree] {batch} requests of 16 tokens, {heads} heads, {len(dead)} of them padding")
+    op.run()
+    torch.cuda.synchronize()
+    out, near, _, _ = trees.expect(2)
+    for b in dead:
+        out[16 * b:16 * b + 16], near[16 * b:16 * b + 16] = 0, 0
+    got = op.out.double().cpu().numpy()
+    assert not np.isnan(got).any() and (np.abs(got - out) <= near).all()
+    assert (op.out[16 * batch:] == 0).all()
+
+
+@pytest.mark.parametrize("softmax_scale", [-0.05, 0.0, 1.5])
+def test_softmax_scales(softmax_scale):
+    say(f"[tree] softmax scale {softmax_scale}")
+    check(Trees(25, [9, 5], [700, 6000], softmax_scale=softmax_scale), True)
+    check(Trees(26, [9, 5], [700, 6000], softmax_scale=softmax_scale), False)
+
+
 def test_chains_and_stars():
     chain = [[i - 1 for i in range(20)], [-1] * 20, [-1] + [0] * 19]
     say("[tree] chain, roots only, star")
@@ -490,6 +522,28 @@ def test_another_stream():
         op.run()
     side.synchronize()
     compare(op, trees, True)
+
+
+def test_two_operators_at_once():
+    """Split launches of two operators on two streams, over the same caches."""
+    import torch
+    from npu_sparse_attn_sharedkv_int8 import PreparedTreeAttention
+    trees = Trees(27, [7, 12, 16], [500, 4000, 12000])
+    case, parents, scale, cmp_scale = trees.device()
+    ops = [PreparedTreeAttention(case, parents, scale, cmp_scale, return_lse=True) for _ in range(2)]
+    assert all(op.partial is not None for op in ops)
+    for op in ops:
+        op.out.fill_(float("nan"))
+    torch.cuda.synchronize()
+    say("[tree] two streams at once")
+    streams = [torch.cuda.Stream() for _ in ops]
+    for _ in range(20):
+        for op, stream in zip(ops, streams):
+            with torch.cuda.stream(stream):
+                op.run()
+    torch.cuda.synchronize()
+    for op in ops:
+        compare(op, trees, True)
 
 
 def test_equals_the_window_operator_on_a_chain():
