@@ -34,6 +34,64 @@ RATIOS = (1, 128)
 MAX_WINDOW = 2 ** 31 - 1
 
 
+def _check_query(q):
+    if q.device.type != "cuda" or q.dtype != torch.bfloat16 or q.ndim != 3 or q.shape[-1] != 512:
+        raise ValueError("Expected BF16 Q[T,H,512] on a GPU")
+    if not 1 <= q.shape[1] <= MAX_HEADS or not q.is_contiguous() or q.data_ptr() % 16:
+        raise ValueError(f"Expected 1..{MAX_HEADS} heads and contiguous, 16-byte aligned Q")
+
+
+def _check_inputs(case, parents, ori_scale, cmp_scale):
+    """Refuses what the kernel cannot take; returns the launch's geometry, (device, the argument block's sizes)."""
+    q = case.q
+    _check_query(q)
+    tokens, heads, _ = q.shape
+    if case.ratio not in RATIOS or case.cmp_indices is not None or case.ori_indices is not None:
+        raise ValueError("Trees attend a window (ratio 1) or a window and every compressed row (ratio 128); "
+                         "layers with lists per token (ratio 4, explicit slots) go through PreparedAttention")
+    if not 1 <= case.window <= MAX_WINDOW:
+        raise ValueError("Expected a positive window")
+    device, batch = q.device, case.seq_lens.numel()
+    caches = [(case.ori, case.ori_block_table, ori_scale)]
+    if case.ratio != 1:
+        caches.append((case.cmp, case.cmp_block_table, cmp_scale))
+    for cache, table, scale in caches:
+        _check_cache(cache, table, scale, batch, device)
+        if (cache.shape[1] != BLOCK or cache.stride(0) % 16 or cache.data_ptr() % 16 or scale.data_ptr() % 16
+                or not table.shape[1]):
+            raise ValueError(f"Expected pages of {BLOCK} rows, 16-byte aligned, and a block table of one page or more")
+    if not batch or tuple(case.cu_q.shape) != (batch + 1,) or case.seq_lens.ndim != 1 \
+            or tuple(case.sink.shape) != (heads,):
+        raise ValueError("Invalid sequence metadata or sink shape")
+    if not isinstance(parents, torch.Tensor) or tuple(parents.shape) != (tokens,):
+        raise ValueError("Expected INT32 parents[T]")
+    for x, dtype in ((case.cu_q, torch.int32), (case.seq_lens, torch.int32), (case.sink, torch.float32),
+                     (parents, torch.int32)):
+        if x.dtype != dtype or x.device != device or not x.is_contiguous():
+            raise ValueError("Invalid metadata dtype, device or contiguity")
+    sizes = dict(tokens=tokens, heads=heads, batch=batch, oriPages=case.ori.shape[0], oriStride=case.ori.stride(0),
+                 oriTableWidth=case.ori_block_table.shape[1], ratio=case.ratio, window=case.window,
+                 softmaxScale=case.softmax_scale)
+    if case.ratio != 1:
+        sizes.update(cmpPages=case.cmp.shape[0], cmpStride=case.cmp.stride(0),
+                     cmpTableWidth=case.cmp_block_table.shape[1])
+    return device, sizes
+
+
+def _check_outputs(out, lse, case, parents):
+    q = case.q
+    if (out is None or tuple(out.shape) != tuple(q.shape) or out.device != q.device or out.dtype != torch.bfloat16
+            or not out.is_contiguous() or out.data_ptr() % 16):
+        raise ValueError("Invalid output buffer")
+    if lse is not None and (tuple(lse.shape) != tuple(q.shape[:2]) or lse.dtype != torch.float32
+                            or lse.device != q.device or not lse.is_contiguous()):
+        raise ValueError("Invalid FP32 LSE[T,H] output buffer")
+    inputs = [q, parents, case.cu_q, case.seq_lens, case.sink]
+    if any(_overlap(out, x) for x in inputs + ([lse] if lse is not None else [])) \
+            or lse is not None and any(_overlap(lse, x) for x in inputs):
+        raise ValueError("Outputs must not overlap inputs or each other")
+
+
 class PreparedTreeAttention:
     """run() launches on the current stream of the inputs' device, allocates
     nothing and reads nothing back.  Its scratch comes from
@@ -51,66 +109,22 @@ class PreparedTreeAttention:
 
     def __init__(self, case, parents, ori_scale, cmp_scale=None, *, output=None, return_lse=False, lse_output=None,
                  scratch_allocator=None):
-        q = case.q
-        if q.device.type != "cuda" or q.dtype != torch.bfloat16 or q.ndim != 3 or q.shape[-1] != 512:
-            raise ValueError("Expected BF16 Q[T,H,512] on a GPU")
-        tokens, heads, _ = q.shape
-        if not 1 <= heads <= MAX_HEADS or not q.is_contiguous() or q.data_ptr() % 16:
-            raise ValueError(f"Expected 1..{MAX_HEADS} heads and contiguous, 16-byte aligned Q")
-        if case.ratio not in RATIOS or case.cmp_indices is not None or case.ori_indices is not None:
-            raise ValueError("Trees attend a window (ratio 1) or a window and every compressed row (ratio 128); "
-                             "layers with lists per token (ratio 4, explicit slots) go through PreparedAttention")
-        if not 1 <= case.window <= MAX_WINDOW:
-            raise ValueError("Expected a positive window")
-        device, batch = q.device, case.seq_lens.numel()
-        caches = [(case.ori, case.ori_block_table, ori_scale)]
-        if case.ratio != 1:
-            caches.append((case.cmp, case.cmp_block_table, cmp_scale))
-        for cache, table, scale in caches:
-            _check_cache(cache, table, scale, batch, device)
-            if (cache.shape[1] != BLOCK or cache.stride(0) % 16 or cache.data_ptr() % 16 or scale.data_ptr() % 16
-                    or not table.shape[1]):
-                raise ValueError(f"Expected pages of {BLOCK} rows, 16-byte aligned, and a block table of one page or more")
-        if not batch or tuple(case.cu_q.shape) != (batch + 1,) or case.seq_lens.ndim != 1 \
-                or tuple(case.sink.shape) != (heads,):
-            raise ValueError("Invalid sequence metadata or sink shape")
-        if tuple(parents.shape) != (tokens,):
-            raise ValueError("Expected INT32 parents[T]")
-        for x, dtype in ((case.cu_q, torch.int32), (case.seq_lens, torch.int32), (case.sink, torch.float32),
-                         (parents, torch.int32)):
-            if x.dtype != dtype or x.device != device or not x.is_contiguous():
-                raise ValueError("Invalid metadata dtype, device or contiguity")
+        self.geometry = _check_inputs(case, parents, ori_scale, cmp_scale)
+        q, device = case.q, case.q.device
         self.case, self.parents, self.scales = case, parents, (ori_scale, cmp_scale)
         self.out = output if output is not None else torch.empty_like(q)
         self.lse = lse_output
         if lse_output is None and return_lse:
-            self.lse = torch.empty((tokens, heads), dtype=torch.float32, device=device)
-        self._check_outputs(q)
-        self.args = TreeAttentionArgs(
-            tokens=tokens, heads=heads, batch=batch, oriPages=case.ori.shape[0], oriStride=case.ori.stride(0),
-            oriTableWidth=case.ori_block_table.shape[1], ratio=case.ratio, window=case.window,
-            softmaxScale=case.softmax_scale, oriScale=ori_scale.data_ptr())
-        if case.ratio != 1:
-            self.args.cmpPages, self.args.cmpStride = case.cmp.shape[0], case.cmp.stride(0)
-            self.args.cmpTableWidth, self.args.cmpScale = case.cmp_block_table.shape[1], cmp_scale.data_ptr()
+            self.lse = torch.empty(q.shape[:2], dtype=torch.float32, device=device)
+        _check_outputs(self.out, self.lse, case, parents)
+        _, sizes = self.geometry
+        self.args = TreeAttentionArgs(**sizes, oriScale=ori_scale.data_ptr(),
+                                      cmpScale=cmp_scale.data_ptr() if case.ratio != 1 else 0)
         self._bind()
         self._take_scratch(scratch_allocator, device)
         self.native = native_launcher()
         self.argument_address = ctypes.addressof(self.args)
         self.device_index = device.index if device.index is not None else torch.cuda.current_device()
-
-    def _check_outputs(self, q):
-        out, lse = self.out, self.lse
-        if (tuple(out.shape) != tuple(q.shape) or out.device != q.device or out.dtype != torch.bfloat16
-                or not out.is_contiguous() or out.data_ptr() % 16):
-            raise ValueError("Invalid output buffer")
-        if lse is not None and (tuple(lse.shape) != tuple(q.shape[:2]) or lse.dtype != torch.float32
-                                or lse.device != q.device or not lse.is_contiguous()):
-            raise ValueError("Invalid FP32 LSE[T,H] output buffer")
-        inputs = [q, self.parents, self.case.cu_q, self.case.seq_lens, self.case.sink]
-        if any(_overlap(out, x) for x in inputs + ([lse] if lse is not None else [])) \
-                or lse is not None and any(_overlap(lse, x) for x in inputs):
-            raise ValueError("Outputs must not overlap inputs or each other")
 
     def _take_scratch(self, allocator, device):
         sizes = ctypes.c_uint64(), ctypes.c_uint64()
@@ -141,10 +155,12 @@ class PreparedTreeAttention:
             setattr(args, name, tensor.data_ptr() if tensor is not None else 0)
 
     def _rebind_same_geometry(self, case, parents, *, output=None, lse_output=None):
-        """Serving fast path: same geometry, new tensors."""
-        self.case, self.parents = case, parents
-        if output is not None:
-            self.out, self.lse = output, lse_output
+        """Serving fast path: same geometry, new tensors, under the constructor's checks (the kernel reads them by it)."""
+        if _check_inputs(case, parents, *self.scales) != self.geometry:
+            raise ValueError("Rebinding keeps the device and every size of the launch")
+        out, lse = (output, lse_output) if output is not None else (self.out, self.lse)
+        _check_outputs(out, lse, case, parents)
+        self.case, self.parents, self.out, self.lse = case, parents, out, lse
         self._bind()
 
     def run(self):

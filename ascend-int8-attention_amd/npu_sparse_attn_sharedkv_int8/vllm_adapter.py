@@ -263,7 +263,7 @@ class SharedKVLayer:
         parents = kw.get("tree_parents")
         out = torch.empty_like(q)
         lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
-        key = (launch_shape(case, return_lse), parents is not None, stream_key(q.device))
+        key = (launch_shape(case, return_lse), parents is not None, q.device, stream_key(q.device))
         op = self.operators.get(key)
         if op is None and parents is not None:
             op = PreparedTreeAttention(case, parents, self.scale("ori", q.device)[0],
