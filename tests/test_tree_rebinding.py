@@ -15,6 +15,10 @@ def aligned(x):
     return room[at:at + x.numel() * x.element_size()].view(x.dtype).view(x.shape).copy_(x)
 
 
+def off_by(x, count):
+    return aligned(torch.empty(x.numel() + count, dtype=x.dtype))[count:].view(x.shape)
+
+
 def inputs(ratio=128):
     cache = lambda pages: aligned(torch.zeros((pages, 32, 1, 512), dtype=torch.int8))  # noqa: E731
     table = lambda width: torch.zeros((BATCH, width), dtype=torch.int32)  # noqa: E731
@@ -34,7 +38,7 @@ def bound(monkeypatch):
     op.scales = tuple(aligned(torch.ones(512)) for _ in range(2))
     op.args = runtime.TreeAttentionArgs()
     if hasattr(tree, "_check_inputs"):
-        op.geometry = tree._check_inputs(case, parents, *op.scales)
+        op.geometry, op.layout = tree._check_inputs(case, parents, *op.scales), tree._layout(case, parents)
     op.case, op.parents, op.out, op.lse = case, parents, aligned(torch.empty_like(case.q)), None
     op._bind()
     return op
@@ -76,7 +80,8 @@ def test_parents_are_checked(bound, match, make):
     ("cmp_block_table", "block table", lambda t: torch.zeros((1, BATCH), dtype=torch.int32).T.expand(BATCH, 2)[:, :1].T),
     ("ori_block_table", "every size", lambda t: torch.zeros((BATCH, 2), dtype=torch.int32)),
     ("ori", "INT8", lambda t: t.float()), ("ori", "every size", lambda t: t[:3]), ("cmp", "INT8", lambda t: None),
-    ("q", "every size", lambda t: t[:, :1].contiguous()), ("window", "every size", lambda w: 64),
+    ("q", "every size", lambda t: t[:, :1].contiguous()), ("ori", "16-byte", lambda t: off_by(t, 8)),
+    ("cmp", "16-byte", lambda t: off_by(t, 8)), ("window", "every size", lambda w: 64),
     ("window", "window", lambda w: 0), ("softmax_scale", "every size", lambda x: 0.05),
     ("ratio", "every size", lambda r: 1), ("ratio", "ratio 4", lambda r: 4)])
 def test_the_case_is_checked(bound, field, match, make):
