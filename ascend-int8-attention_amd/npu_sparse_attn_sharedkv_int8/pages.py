@@ -34,9 +34,24 @@ def _ints(tensor, shape, device, what):
         raise ValueError(f"Expected contiguous INT32 {what}[{sizes}] on the caches' GPU")
 
 
+def _extent(x):
+    """Bytes from a tensor's first to its last."""
+    if x.is_contiguous():
+        return x.nbytes
+    return (1 + sum((n - 1) * step for n, step in zip(x.shape, x.stride()))) * x.element_size() if x.numel() else 0
+
+
+def _overlaps(tensor, others):
+    first, end = tensor.data_ptr(), tensor.data_ptr() + _extent(tensor)
+    for x in others:
+        at = x.data_ptr()
+        if at < end and first < at + _extent(x):
+            return True
+    return False
+
+
 def _overlap(a, b):
-    first, second = a.data_ptr(), b.data_ptr()
-    return first < second + b.numel() * b.element_size() and second < first + a.numel() * a.element_size()
+    return _overlaps(a, (b,))
 
 
 def _inner(cache, first):
@@ -165,7 +180,7 @@ class PreparedPathCommit(_Prepared):
             raise ValueError("Expected one request, path entry and table entry or more")
         self.seq_lens = output if output is not None else torch.empty_like(seq_lens)
         _ints(self.seq_lens, (batch,), device, "output")
-        if any(_overlap(self.seq_lens, x) for x in (seq_lens, cu_q, block_table, paths, path_lens)):
+        if _overlaps(self.seq_lens, (seq_lens, cu_q, block_table, paths, path_lens, *caches)):
             raise ValueError("The new lengths need a buffer of their own")
         self.block_table, self.inputs = block_table, (cu_q, seq_lens, paths, path_lens)
         self.spans, sizes = _spans(caches, 2)
@@ -245,7 +260,8 @@ class PreparedPageFork(_Prepared):
         self.block_table, self.refs = _table_outputs(block_table, (children, width), refs, (new_table, new_refs), device)
         self.seq_lens = new_lens if new_lens is not None else torch.empty(children, dtype=torch.int32, device=device)
         _ints(self.seq_lens, (children,), device, "new seq_lens")
-        _check_aliases([(self.block_table, block_table), (self.seq_lens, seq_lens), (self.refs, refs)], [parents])
+        _check_aliases([(self.block_table, block_table), (self.seq_lens, seq_lens), (self.refs, refs)],
+                       [parents, *caches])
         self.missing = torch.zeros(1, dtype=torch.int32, device=device)
         self.inputs = block_table, seq_lens, refs, parents
         self.spans, sizes = _spans(caches, 1)
@@ -293,7 +309,7 @@ class PreparedPageCompact(_Prepared):
             raise ValueError("Expected one row and entry or more")
         self.block_table, self.refs = _table_outputs(block_table, tuple(block_table.shape), refs,
                                                      output if output is not None else (None, None), device)
-        _check_aliases([(self.block_table, block_table), (self.refs, refs)], [])
+        _check_aliases([(self.block_table, block_table), (self.refs, refs)], caches)
         self.moved = torch.empty_like(refs)
         self.live = torch.zeros(1, dtype=torch.int32, device=device)
         self.inputs = block_table, refs

@@ -27,7 +27,7 @@ import torch
 
 from .attention import _check_cache
 from .c8_attention import BLOCK, MAX_HEADS
-from .pages import _overlap
+from .pages import _overlaps
 from .runtime import TreeAttentionArgs, library, native_launcher
 
 RATIOS = (1, 128)
@@ -86,7 +86,7 @@ def _layout(case, parents):
                 case.q, case.ori, case.ori_block_table, case.cu_q, case.seq_lens, case.sink, parents, *cmp)])
 
 
-def _check_outputs(out, lse, case, parents):
+def _check_outputs(out, lse, case, parents, scales):
     q = case.q
     if (out is None or tuple(out.shape) != tuple(q.shape) or out.device != q.device or out.dtype != torch.bfloat16
             or not out.is_contiguous() or out.data_ptr() % 16):
@@ -94,9 +94,11 @@ def _check_outputs(out, lse, case, parents):
     if lse is not None and (tuple(lse.shape) != tuple(q.shape[:2]) or lse.dtype != torch.float32
                             or lse.device != q.device or not lse.is_contiguous()):
         raise ValueError("Invalid FP32 LSE[T,H] output buffer")
-    inputs = [q, parents, case.cu_q, case.seq_lens, case.sink]
-    if any(_overlap(out, x) for x in inputs + ([lse] if lse is not None else [])) \
-            or lse is not None and any(_overlap(lse, x) for x in inputs):
+    # A work-group may end, and write, before another reads.
+    inputs = [q, parents, case.cu_q, case.seq_lens, case.sink, case.ori, case.ori_block_table, scales[0]]
+    if case.ratio != 1:
+        inputs += [case.cmp, case.cmp_block_table, scales[1]]
+    if _overlaps(out, inputs) or lse is not None and _overlaps(lse, inputs + [out]):
         raise ValueError("Outputs must not overlap inputs or each other")
 
 
@@ -125,7 +127,7 @@ class PreparedTreeAttention:
         self.lse = lse_output
         if lse_output is None and return_lse:
             self.lse = torch.empty(q.shape[:2], dtype=torch.float32, device=device)
-        _check_outputs(self.out, self.lse, case, parents)
+        _check_outputs(self.out, self.lse, case, parents, self.scales)
         _, sizes = self.geometry
         self.args = TreeAttentionArgs(**sizes, oriScale=ori_scale.data_ptr(),
                                       cmpScale=cmp_scale.data_ptr() if case.ratio != 1 else 0)
@@ -170,7 +172,7 @@ class PreparedTreeAttention:
             if _check_inputs(case, parents, *self.scales) != self.geometry:
                 raise ValueError("Rebinding keeps the device and every size of the launch")
         out, lse = (output, lse_output) if output is not None else (self.out, self.lse)
-        _check_outputs(out, lse, case, parents)
+        _check_outputs(out, lse, case, parents, self.scales)
         self.case, self.parents, self.out, self.lse = case, parents, out, lse
         self._bind()
 

@@ -100,3 +100,36 @@ def test_outputs_are_checked(bound):
             lse_output=torch.empty((TOKENS, HEADS + 1)))
     bound.out = None                                                   # an operator whose caller took its output
     refused(bound, "output", case=case, parents=parents)
+
+
+@pytest.mark.parametrize("field", ["ori", "cmp", "ori_block_table", "cmp_block_table", "cu_q", "seq_lens", "sink", "q"])
+@pytest.mark.parametrize("which", ["output", "lse_output"])
+def test_outputs_over_any_input_are_refused(bound, field, which):
+    """Also an output that lies between the first and the last byte of pages with room between them."""
+    case, parents = inputs()
+    good = dict(output=aligned(torch.empty_like(case.q)), lse_output=torch.empty((TOKENS, HEADS)))
+    count = {name: x.nbytes for name, x in good.items()}[which]
+    held = getattr(case, field)
+    # The input at the end of a buffer whose start is the output, a few bytes of it shared.
+    room = aligned(torch.zeros(count + held.nbytes, dtype=torch.int8))
+    at = count - 16
+    moved = room[at:at + held.nbytes].view(held.dtype).view(held.shape).copy_(held)
+    setattr(case, field, moved)
+    refused(bound, "overlap", case=case, parents=parents,
+            **dict(good, **{which: room[:count].view(good[which].dtype).view(good[which].shape)}))
+
+
+@pytest.mark.parametrize("which", [0, 1])
+def test_outputs_over_a_scale_are_refused(bound, which):
+    case, parents = inputs()
+    lse = bound.scales[which][100:100 + TOKENS * HEADS].view(TOKENS, HEADS)
+    refused(bound, "overlap", case=case, parents=parents, output=aligned(torch.empty_like(case.q)), lse_output=lse)
+
+
+def test_bytes_between_pages_count_as_the_caches():
+    from npu_sparse_attn_sharedkv_int8 import pages
+    flat = torch.zeros(4 * 100, dtype=torch.int8)
+    strided = flat.as_strided((3, 32), (100, 1))
+    assert pages._extent(strided) == 232 and pages._extent(flat) == 400 and pages._extent(flat[:0]) == 0
+    assert pages._overlap(flat[40:50], strided) and pages._overlap(strided, flat[231:]) and not pages._overlap(strided, flat[232:])
+    assert not pages._overlap(flat[:10], flat[10:]) and pages._overlap(flat[:11].view(torch.int8), flat[10:])
