@@ -129,12 +129,13 @@ struct alignas(1024) Shared {
         _Float16 p[ROWS * P_STRIDE];   // weights [row][key]
         float scale[2][D];             // channel scales (compressed, original) while Q is encoded
     };
-    uint64_t mask[ROWS];               // the tile's original rows that each of the unit's tokens sees
+    uint64_t mask[ROWS];               // the tile's rows that each of the unit's tokens sees
     float factor[ROWS], top[ROWS], sum[PARTS][ROWS], peak[PARTS][ROWS];
     int32_t moved[RT];                 // whether a row tile moved its maximum in this tile
     int32_t scan[3][WAVES];
     int32_t found[7];
-    int32_t walk[ROWS], steps[ROWS], depth[ROWS];   // of the unit's tokens: node that the walk is at, steps to it, depth
+    // Of the unit's tokens: node that the walk is at, steps to it, depth, compressed rows it sees.
+    int32_t walk[ROWS], steps[ROWS], depth[ROWS], compressed[ROWS];
     uint8_t token[ROWS];               // of the unit's rows
     uint16_t parent[PARENTS];
 };
@@ -144,7 +145,7 @@ struct alignas(1024) Shared {
 struct Request {
     int32_t first, nodes, length, committed;   // first token, drafted tokens, all rows, committed rows
     bool live;
-    int32_t compressed;                // visible compressed rows
+    int32_t compressed, shared;        // compressed rows that some token may see, that all do
     int32_t low, end;                  // original rows [low, end), low a multiple of PAGE_ROWS
     int32_t cmp_tiles, ori_tiles;
 };
@@ -153,6 +154,7 @@ struct Request {
 struct Sizes {
     uint32_t tokens, ratio, window, oriTableWidth, cmpTableWidth;
 };
+template <bool CAUSAL>
 __device__ __forceinline__ Request request_of(const Sizes &p, int c0, int c1, int length)
 {
     Request r;
@@ -163,7 +165,8 @@ __device__ __forceinline__ Request request_of(const Sizes &p, int c0, int c1, in
     r.live = length > 0 && r.nodes > 0;
     r.committed = max(0, length - r.nodes);
     const int64_t ori_rows = (int64_t)p.oriTableWidth * PAGE_ROWS, cmp_rows = (int64_t)p.cmpTableWidth * PAGE_ROWS;
-    r.compressed = p.ratio > 1 ? (int)min((int64_t)(r.committed / (int)p.ratio), cmp_rows) : 0;
+    r.shared = p.ratio > 1 ? (int)min((int64_t)(r.committed / (int)p.ratio), cmp_rows) : 0;
+    r.compressed = CAUSAL ? (int)min((int64_t)((r.committed + r.nodes) / (int)p.ratio), cmp_rows) : r.shared;
     r.low = max(0, r.committed - (int)min(p.window, 0x7fffffffu) + 1) & ~(PAGE_ROWS - 1);
     r.end = (int)min((int64_t)r.committed + r.nodes, ori_rows);
     r.cmp_tiles = r.live ? (r.compressed + KEYS - 1) / KEYS : 0;
@@ -289,7 +292,9 @@ __device__ __forceinline__ int by_length(int group, int units)
     return group < shared ? CUS - shared + group : group < CUS ? group - shared : units - 1 - (group - CUS);
 }
 
-template <int TERMS, int RT>
+// CAUSAL: compressed rows go by a token's own position (a kernel of its own: the masks' scalars, kept over the tile loop,
+// cost whole contexts 2 %, which launches without them need not pay).
+template <int TERMS, int RT, bool CAUSAL>
 __global__ void __launch_bounds__(THREADS, TERMS == 2 || RT < 4 ? 2 : 1) tree_attention(const uint64_t cu_q, const uint64_t seq_lens, const uint32_t batch_arg, const uint32_t heads_arg,
                const uint32_t split, const uint32_t tokens_arg, const uint32_t ratio, const uint32_t window_rows,
                const uint32_t ori_width, const uint32_t cmp_width, const TreeAttentionArgs p)
@@ -308,7 +313,7 @@ __global__ void __launch_bounds__(THREADS, TERMS == 2 || RT < 4 ? 2 : 1) tree_at
     Request mine = {};
     int units = 0, kinds = 0, work = 0;                // units, times their kinds, times their tiles
     for (int b = tid; b < batch; b += THREADS) {
-        mine = request_of(size, cu[b], cu[b + 1], lens[b]);
+        mine = request_of<CAUSAL>(size, cu[b], cu[b + 1], lens[b]);
         const int u = units_of(mine);
         units += u;
         kinds += u * max(1, (mine.cmp_tiles > 0) + (mine.ori_tiles > 0));
@@ -352,7 +357,7 @@ __global__ void __launch_bounds__(THREADS, TERMS == 2 || RT < 4 ? 2 : 1) tree_at
             const bool one_step = batch <= THREADS;
             for (int at = 0; at < batch; at += THREADS) {
                 const int b0 = at + tid;
-                if (!one_step) mine = b0 < batch ? request_of(size, cu[b0], cu[b0 + 1], lens[b0]) : Request{};
+                if (!one_step) mine = b0 < batch ? request_of<CAUSAL>(size, cu[b0], cu[b0 + 1], lens[b0]) : Request{};
                 const bool there = b0 < batch;
                 const int u = there ? units_of(mine) : 0, n_items = there ? u * items_of(mine) : 0;
                 upto = wave_upto(n_items), at_units = wave_upto(u);
@@ -407,7 +412,7 @@ __global__ void __launch_bounds__(THREADS, TERMS == 2 || RT < 4 ? 2 : 1) tree_at
         return;
     }
     b = uni(b);
-    const Request r = request_of(size, uni(s.found[3]), uni(s.found[4]), uni(s.found[5]));
+    const Request r = request_of<CAUSAL>(size, uni(s.found[3]), uni(s.found[4]), uni(s.found[5]));
     const int splits = items_of(r), local = uni(s.found[1]);
     const int part_no = local % splits;                // which of the unit's items
     unit = local / splits;
@@ -478,6 +483,7 @@ __global__ void __launch_bounds__(THREADS, TERMS == 2 || RT < 4 ? 2 : 1) tree_at
     const int token0 = row0 / heads, tokens = (row0 + rows - 1) / heads - token0 + 1;
     const float softmax2 = p.softmaxScale * LOG2E;
     const bool has_cmp = k0 < r.cmp_tiles && k0 < k1, has_ori = k1 > r.cmp_tiles;
+    const bool walks = has_ori || (CAUSAL && r.shared != r.compressed);
     // The waves of a row tile encode a share of its channels each (64 j .. 64 j + 63, j from j0 on) and pass the codes
     // round in the tile buffer that is free.
     constexpr bool SHARE = PARTS > 1;
@@ -540,7 +546,7 @@ __global__ void __launch_bounds__(THREADS, TERMS == 2 || RT < 4 ? 2 : 1) tree_at
         read_entries(k0 >> 5);
         load_scales();
         if (tid < ROWS) s.token[tid] = (uint8_t)((row0 + min(tid, rows - 1)) / heads - token0);
-        if (has_ori)
+        if (walks)
             for (int i = tid; i < min(r.nodes, PARENTS); i += THREADS) {
                 const int up = gptr<int32_t>(p.parents)[r.first + i];
                 s.parent[i] = (uint16_t)(up >= 0 && up < i ? up : ROOT);
@@ -600,22 +606,31 @@ __global__ void __launch_bounds__(THREADS, TERMS == 2 || RT < 4 ? 2 : 1) tree_at
         return up >= 0 && up < node ? up : -1;
     };
     // Thread t < tokens walks token t's chain, and says which of an original tile's rows the token sees.
-    if (has_ori && tid < tokens) {
+    if ((CAUSAL || has_ori) && tid < tokens) {
         int depth = 0;
-        for (int a = parent_of(token0 + tid); a >= 0; a = parent_of(a)) ++depth;
+        if (walks)
+            for (int a = parent_of(token0 + tid); a >= 0; a = parent_of(a)) ++depth;
         s.walk[tid] = token0 + tid, s.steps[tid] = 0, s.depth[tid] = depth;
+        if (CAUSAL) s.compressed[tid] = min(r.compressed, (r.committed + depth + 1) / (int)p.ratio);
     }
-    // Original tiles of committed rows that the deepest token's window still holds need no masks.
+    // Original tiles of committed rows that the deepest token's window still holds need no masks, nor do compressed ones
+    // whose rows all tokens see.
     const int plain_from = max(0, r.committed + r.nodes - (int)min(p.window, 0x7fffffffu));
     auto is_plain = [&](int k) {
         const int base = base_of(k);
-        return k < r.cmp_tiles || (base >= plain_from && base + KEYS <= r.committed);
+        if (k < r.cmp_tiles) return !CAUSAL || base + KEYS <= r.shared;
+        return base >= plain_from && base + KEYS <= r.committed;
     };
     auto make_mask = [&](int k, uint64_t rows_there) {
         const int at = tid;
         if (is_plain(k) || at >= tokens) return;
-        // Committed rows (C + depth - window, C), then the ancestors.
         const int base = base_of(k);
+        if (CAUSAL && k < r.cmp_tiles) {
+            const int left = s.compressed[at] - base;
+            s.mask[at] = left > 0 ? (~0ull >> (KEYS - min(left, KEYS))) & rows_there : 0;
+            return;
+        }
+        // Committed rows (C + depth - window, C), then the ancestors.
         const int from = max(0, max(0, r.committed + s.depth[at] + 1 - (int)min(p.window, 0x7fffffffu)) - base);
         const int to = min(KEYS, r.committed - base);
         uint64_t bits = 0;
@@ -675,7 +690,7 @@ __global__ void __launch_bounds__(THREADS, TERMS == 2 || RT < 4 ? 2 : 1) tree_at
 
         // S = Q K^T: query row n, keys key0 + 16 kt + 4 g + i.
         const bool plain = is_plain(k);
-        if (!window) {
+        if (!CAUSAL && !window) {
             const int left = r.compressed - k * KEYS;
             if (left < KEYS) seen &= (1ull << left) - 1;
         }
@@ -980,6 +995,7 @@ bool rejected(const TreeAttentionArgs *a)
     if (!a || !a->heads || a->heads > MAX_HEADS || !a->batch || !a->window || !a->ratio) return true;
     if (!a->q || !a->ori || !a->oriScale || !a->oriTable || !a->cuQ || !a->seqLens || !a->sinks || !a->parents || !a->out)
         return true;
+    if (a->ratio > 0x7fffffffu || a->causalCompressed > 1) return true;
     if (!a->oriPages || !a->oriTableWidth || (a->oriStride & 15) || a->oriStride < (uint64_t)PAGE_ROWS * D) return true;
     if ((a->q | a->ori | a->oriScale | a->out) & 15) return true;
     if (a->ratio > 1 && (!a->cmp || !a->cmpScale || !a->cmpTable || !a->cmpPages || !a->cmpTableWidth ||
@@ -1030,9 +1046,15 @@ int launch_sharedkv_tree(void *stream, const TreeAttentionArgs *a)
     if (!a->tokens) return (int)hipSuccess;
     const Plan plan = plan_of(a);
     if (plan.split && (!a->workspace || !a->partial || ((a->workspace | a->partial) & 15))) return (int)hipErrorInvalidValue;
-    const auto kernel = plan.rt == 4   ? (a->lse ? &tree_attention<3, 4> : &tree_attention<2, 4>)
-                        : plan.rt == 2 ? (a->lse ? &tree_attention<3, 2> : &tree_attention<2, 2>)
-                                       : (a->lse ? &tree_attention<3, 1> : &tree_attention<2, 1>);
+    const auto of_rows = [&](auto terms, auto causal) {
+        return plan.rt == 4   ? &tree_attention<terms.value, 4, causal.value>
+               : plan.rt == 2 ? &tree_attention<terms.value, 2, causal.value>
+                              : &tree_attention<terms.value, 1, causal.value>;
+    };
+    const auto of_terms = [&](auto causal) {
+        return a->lse ? of_rows(std::integral_constant<int, 3>{}, causal) : of_rows(std::integral_constant<int, 2>{}, causal);
+    };
+    const auto kernel = a->ratio > 1 && a->causalCompressed ? of_terms(std::true_type{}) : of_terms(std::false_type{});
     const bool local = plan.split && sharedkv::xcd_local(static_cast<hipStream_t>(stream));
     hipLaunchKernelGGL(kernel, dim3(plan.grid), dim3(THREADS), 0, static_cast<hipStream_t>(stream), a->cuQ, a->seqLens,
                        a->batch, a->heads, (plan.split ? plan.units : 0u) | (local ? XCD_LOCAL : 0u), a->tokens, a->ratio,

@@ -61,7 +61,7 @@ class TreeAttentionArgs(ctypes.Structure):
     _fields_ = _block("q ori cmp oriScale cmpScale oriTable cmpTable cuQ seqLens sinks parents out lse workspace "
                       "partial oriStride cmpStride",
                       "tokens heads batch oriPages cmpPages oriTableWidth cmpTableWidth ratio window",
-                      [("softmaxScale", ctypes.c_float)])
+                      [("softmaxScale", ctypes.c_float), ("causalCompressed", ctypes.c_uint32)])
 
 
 class PathCommitArgs(ctypes.Structure):

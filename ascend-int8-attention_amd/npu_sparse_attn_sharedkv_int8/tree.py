@@ -13,9 +13,18 @@ token's own (-1, by convention) makes it a root, a child of the last committed
 token.  A token of depth d (0 for a root) stands at position C + d and sees
   * the original rows j < C with j > C + d - window,
   * its ancestors and itself, those fewer than `window` steps above it,
-  * with ratio 128, the compressed rows r < C // 128 (what the committed
-    tokens completed; a branch's own rows are not compressed yet).
-For a chain this is PreparedAttention over the same rows.  Top-k layers
+  * with ratio 128, the compressed rows r < C // 128, those that the committed
+    tokens completed, or with causal_compressed=True r < (C + d + 1) // 128,
+    those completed up to its own position.
+PreparedAttention sees the compressed rows up to a token's position.  A chain is
+PreparedAttention over the same rows with ratio 1 and, with ratio 128, with
+causal_compressed: its drafted tokens' compressed rows are then written before
+the launch, like their rows of the original cache.  Without it a token whose
+path passes a multiple of 128 rows misses the row that ends there, and the
+original rows of it that have left the window.  With it, row C // 128 + k is one
+row for the request: every token from the depth that completes it on sees it, so
+where several nodes of a tree stand at that depth (and their paths complete
+different rows) the branches have to be requests of their own.  Top-k layers
 (ratio 4) have a list of their own for every token, so nothing is shared:
 PreparedAttention takes them, with the ancestors' slots in ori_indices.
 
@@ -118,7 +127,7 @@ class PreparedTreeAttention:
     """
 
     def __init__(self, case, parents, ori_scale, cmp_scale=None, *, output=None, return_lse=False, lse_output=None,
-                 scratch_allocator=None):
+                 scratch_allocator=None, causal_compressed=False):
         self.geometry = _check_inputs(case, parents, ori_scale, cmp_scale)
         self.layout = _layout(case, parents)
         q, device = case.q, case.q.device
@@ -130,7 +139,8 @@ class PreparedTreeAttention:
         _check_outputs(self.out, self.lse, case, parents, self.scales)
         _, sizes = self.geometry
         self.args = TreeAttentionArgs(**sizes, oriScale=ori_scale.data_ptr(),
-                                      cmpScale=cmp_scale.data_ptr() if case.ratio != 1 else 0)
+                                      cmpScale=cmp_scale.data_ptr() if case.ratio != 1 else 0,
+                                      causalCompressed=int(bool(causal_compressed)))
         self._bind()
         self._take_scratch(scratch_allocator, device)
         self.native = native_launcher()

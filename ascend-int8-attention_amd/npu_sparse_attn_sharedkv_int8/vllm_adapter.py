@@ -258,7 +258,9 @@ class SharedKVLayer:
         """The sparse attention call (keyword contract above); returns
         (out BF16 [T, H, 512], lse FP32 [T, H, 1]) or (out, empty FP32).
         With tree_parents (INT32 [T], each token's parent by its index in the
-        request) the tokens are the drafted trees of PreparedTreeAttention."""
+        request) the tokens are the drafted trees of PreparedTreeAttention, with
+        the causal rule of every call for the compressed rows: a token sees
+        those completed up to its own position, which the call finds written."""
         case, return_lse = parse_attention_call(q, kw)
         parents = kw.get("tree_parents")
         out = torch.empty_like(q)
@@ -268,7 +270,7 @@ class SharedKVLayer:
         if op is None and parents is not None:
             op = PreparedTreeAttention(case, parents, self.scale("ori", q.device)[0],
                                        self.scale("cmp", q.device)[0] if case.ratio > 1 else None, output=out,
-                                       lse_output=lse, scratch_allocator=scratch_allocator)
+                                       lse_output=lse, scratch_allocator=scratch_allocator, causal_compressed=True)
             self.operators.put(key, op)
         elif op is None:
             op = PreparedAttention(case, self.scale("ori", q.device)[0],

@@ -71,7 +71,10 @@ typedef struct CacheWriteArgs {
  * (a root's is 0) sees
  *   original rows j < C with j > C + d - window,
  *   its ancestors and itself, those fewer than `window` steps above it,
- *   with a compressed cache (ratio > 1) its rows r < C / ratio.
+ *   with a compressed cache (ratio > 1) its rows r < C / ratio, or where
+ *   causalCompressed is 1 (instead of 0) r < (C + d + 1) / ratio, as
+ *   SharedKVArgs' queries do at position C + d.  The rows behind C / ratio are
+ *   the request's: one row for all of its nodes at the depth that completes it.
  * Rows on a page outside [0, oriPages) / [0, cmpPages), or past the block
  * table, are masked.  q, out BF16 [tokens][heads][512], heads 1..128; sinks
  * FP32 [heads]; lse FP32 [tokens][heads] or 0; ori / cmp INT8 pages of 32
@@ -86,6 +89,7 @@ typedef struct TreeAttentionArgs {
     uint64_t oriStride, cmpStride;
     uint32_t tokens, heads, batch, oriPages, cmpPages, oriTableWidth, cmpTableWidth, ratio, window;
     float softmaxScale;
+    uint32_t causalCompressed;
 } TreeAttentionArgs;
 
 /* One cache of a pool, for the entries below: page i at base + i * pageStride,
