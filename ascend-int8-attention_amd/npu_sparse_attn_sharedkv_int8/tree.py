@@ -159,8 +159,10 @@ class PreparedTreeAttention:
             # Merge tickets, which every launch leaves zero, and partition states.
             self.workspace = allocate("tree_workspace", (tickets,), torch.int32, device)
             self.partial = allocate("tree_partial", (states,), torch.float32, device)
-            # Under capture a clear only becomes part of that graph: run() then clears too, until it has done so eagerly.
-            self._unclear = torch.cuda.is_current_stream_capturing()
+            # A caller's scratch is cleared by the first run, in its stream's order, so that making an operator in a
+            # serving loop waits for nothing.  Under capture a clear only becomes part of that graph: run() clears too,
+            # until it has done so eagerly.
+            self._unclear = allocator is not None or torch.cuda.is_current_stream_capturing()
             if not self._unclear:
                 self.workspace.zero_()
                 torch.cuda.current_stream(device).synchronize()  # run() may come on another stream
@@ -189,8 +191,9 @@ class PreparedTreeAttention:
     def run(self):
         """Launch on the current stream of the case's device; returns .out."""
         if self._unclear:
-            self.workspace.zero_()
-            self._unclear = torch.cuda.is_current_stream_capturing()
+            with torch.cuda.device(self.device_index):
+                self.workspace.zero_()
+                self._unclear = torch.cuda.is_current_stream_capturing()
         if self.args.tokens:
             self.native.launch("tree_attention", self.argument_address, self.device_index)
         return self.out
