@@ -28,6 +28,9 @@ constexpr uint32_t FEW_CHUNKS = 8;              // up to which compact_plan coun
 constexpr uint64_t STREAMED_POOL = 256ull << 20;
 constexpr int COPY = 8;                          // 16-byte units of a thread that are under way at once
 constexpr int WANTED = -2;                      // a staged entry that gets a free page
+// Work-groups of a launch: their threads are counted in 32 bits.  Checked before the first of a call's launches, so
+// that a refused call leaves the workspace as it was.
+constexpr uint64_t MAX_GROUPS = 0xffffffffull / THREADS;
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
@@ -645,7 +648,7 @@ int launch_sharedkv_path_commit(void *stream, const PathCommitArgs *a)
     if (a->pages > 0x7fffffffu || a->tokens > 0x7fffffffu || a->depth > 0x3fffffffu) return (int)hipErrorInvalidValue;
     if (!a->batch) return (int)hipSuccess;
     const uint64_t groups = ((uint64_t)a->cacheCount * (a->rowBytes / 16) + THREADS - 1) / THREADS;
-    if (groups > 65535) return (int)hipErrorInvalidValue;
+    if (groups > 65535 || a->batch > MAX_GROUPS) return (int)hipErrorInvalidValue;
     hipLaunchKernelGGL(path_commit, dim3(a->batch, (uint32_t)groups), dim3(THREADS), 0, static_cast<hipStream_t>(stream), *a);
     return (int)hipGetLastError();
 }
@@ -659,9 +662,10 @@ int launch_sharedkv_page_fork(void *stream, const PageForkArgs *a)
         return (int)hipErrorInvalidValue;
     const uint64_t slices = (a->pageBytes + SLICE - 1) / SLICE;
     if (a->pages > MAX_PAGES || a->rows > 0xfffffu || a->children > 0xfffffu || a->width > 0xffffffu ||
-        a->pageRows > 0xffffffu || a->room > 0x3fffffffu || slices * a->children > 0x3fffffffu)
+        a->pageRows > 0xffffffu || a->room > 0x3fffffffu)
         return (int)hipErrorInvalidValue;
     const uint32_t chunks = chunks_of(a->pages);
+    if (slices > MAX_GROUPS || slices * a->children + chunks > MAX_GROUPS) return (int)hipErrorInvalidValue;
     hipStream_t s = static_cast<hipStream_t>(stream);
     hipLaunchKernelGGL(fork_plan, dim3(a->children + a->rows + chunks), dim3(THREADS), 0, s, *a);
     hipLaunchKernelGGL(fork_apply, dim3((uint32_t)slices * a->children + chunks), dim3(THREADS), 0, s, *a, (uint32_t)slices);
@@ -683,6 +687,7 @@ int launch_sharedkv_page_compact(void *stream, const PageCompactArgs *a)
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (a->pages <= (uint32_t)CHUNK && a->newTable != a->table && a->newRefs != a->refs) {
         const uint32_t groups = (uint32_t)((entries + THREADS - 1) / THREADS);
+        if (copies + (uint64_t)groups + 1 > MAX_GROUPS) return (int)hipErrorInvalidValue;
         hipLaunchKernelGGL((streamed ? &compact_small<true> : &compact_small<false>), dim3(copies + groups + 1), dim3(THREADS), 0, s, *a, groups, copies,
                            (uint32_t)slices);
         return (int)hipGetLastError();

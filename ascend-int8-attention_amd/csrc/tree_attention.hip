@@ -54,6 +54,7 @@ constexpr int ROOT = 0xffff;
 constexpr int WHOLE = 0x3fffffff;  // tiles of an item where units are not split
 constexpr uint32_t MAX_HEADS = 128;
 constexpr int CUS = 256;
+constexpr uint32_t MAX_GROUPS = 0xffffffffu / THREADS;   // the threads of a launch are counted in 32 bits
 // Items of a launch: two work-groups on each of 256 CUs; of small units, whose items differ most, half as many again (32
 // requests of 4-16 nodes: 24.8 us in at most 512 items, 22.7 in 768, 30.1 in 1024).
 __host__ __device__ constexpr uint32_t items_for(int rt) { return rt == 1 ? 768 : 512; }
@@ -1045,6 +1046,7 @@ int launch_sharedkv_tree(void *stream, const TreeAttentionArgs *a)
     if (rejected(a)) return (int)hipErrorInvalidValue;
     if (!a->tokens) return (int)hipSuccess;
     const Plan plan = plan_of(a);
+    if (plan.grid > MAX_GROUPS) return (int)hipErrorInvalidValue;
     if (plan.split && (!a->workspace || !a->partial || ((a->workspace | a->partial) & 15))) return (int)hipErrorInvalidValue;
     const auto of_rows = [&](auto terms, auto causal) {
         return plan.rt == 4   ? &tree_attention<terms.value, 4, causal.value>
@@ -1066,6 +1068,7 @@ int sharedkv_tree_scratch(const TreeAttentionArgs *a, uint64_t *workspace, uint6
 {
     if (!workspace || !partial || rejected(a)) return (int)hipErrorInvalidValue;
     const Plan plan = plan_of(a);
+    if (plan.grid > MAX_GROUPS) return (int)hipErrorInvalidValue;
     *workspace = plan.split ? plan.units * 4ull : 0;
     *partial = plan.split ? plan.grid * state_floats(plan.rt) * 4 : 0;
     return (int)hipSuccess;

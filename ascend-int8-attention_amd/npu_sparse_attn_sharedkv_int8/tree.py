@@ -150,7 +150,7 @@ class PreparedTreeAttention:
     def _take_scratch(self, allocator, device):
         sizes = ctypes.c_uint64(), ctypes.c_uint64()
         if self.args.tokens and library().sharedkv_tree_scratch(ctypes.addressof(self.args), *map(ctypes.byref, sizes)):
-            raise ValueError("This launch is outside the tree kernel's limits (2^31 query rows)")
+            raise ValueError("This launch is outside the tree kernel's limits (some 2^30 query rows, 2^24 requests)")
         allocate = allocator or (lambda name, shape, dtype, dev: torch.empty(shape, dtype=dtype, device=dev))
         tickets, states = (size.value // 4 for size in sizes)
         self.workspace = self.partial = None

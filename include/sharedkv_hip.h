@@ -238,7 +238,9 @@ int launch_sharedkv_tree(void *stream, const TreeAttentionArgs *args);
 int sharedkv_tree_scratch(const TreeAttentionArgs *args, uint64_t *workspace, uint64_t *partial);
 
 /* Accepted paths, and pages of a pool (argument blocks above).  pageBytes is
- * the sum of the caches' bytes and rowBytes the largest row's. */
+ * the sum of the caches' bytes and rowBytes the largest row's.  All take up to
+ * 2^24 - 1 work-groups of 256 threads (a fork one for every 64 KiB of every
+ * child's page) and refuse larger calls before their first launch. */
 int launch_sharedkv_path_commit(void *stream, const PathCommitArgs *args);
 int launch_sharedkv_page_fork(void *stream, const PageForkArgs *args);
 int launch_sharedkv_page_compact(void *stream, const PageCompactArgs *args);
