@@ -1021,12 +1021,21 @@ Plan plan_of(const TreeAttentionArgs *a)
     const uint64_t near = (uint64_t)a->window + 2 * (a->tokens / a->batch + 1) + PAGE_ROWS;
     const uint64_t ori_pages = near / PAGE_ROWS + 1 < a->oriTableWidth ? near / PAGE_ROWS + 1 : a->oriTableWidth;
     const uint64_t work = (rows + 63) / 64 * (cmp_tiles + (ori_pages + 1) / 2);
-    // Units of 16 rows spread few rows over more work-groups and join smaller states; units of 64 rows read and convert
-    // a key's row for more of them.  In tiles of 64 rows and 64 keys (microseconds of 16, 32 and 64 rows a unit): 1
-    // request of 8 nodes, 4 tiles 13.5, 18.2, 34.7; 32 requests of 4-16 nodes, 400 tiles 22.7, 28.8, 64; 48 of 25 nodes,
-    // 750 tiles 31.5, 24.6, 33.4; 16 of 24 nodes and 64 heads, 5400 tiles 140, 112, 79; 4 of 61 over 32 K rows, 31000
-    // tiles 626, 284, 236.
-    plan.rt = work <= 500 ? 1 : work <= 2000 ? 2 : 4;
+    // Units of 16 rows spread few rows over more work-groups and join smaller states, in more work-groups at once; units
+    // of 64 rows read and convert a key's row for more of them.  With R tiles of 64 rows and `work` tiles of 64 rows and 64
+    // keys, the better one goes by R * work (microseconds of 16, 32 and 64 rows a unit, whole contexts but for two):
+    //        1 K  64 rows, 65536 keys           97, 220,  906      16 K  256 rows, 65536 keys       122, 115, 352
+    //       16 K  1024 rows, 4096 keys        46.7, 46.5, 103      17 K  32 requests of 4-16 nodes  19.5, 26.1, 38.7
+    //       66 K  2048 rows, 4096 keys          69, 49.5,  85      90 K  48 of 25 nodes, window     29.8, 23.3, 30.5
+    //      263 K  2048 rows, 16384 keys        204, 112,  130       1 M  2048 rows, 65536 keys      749, 364, 296
+    //      1.8 M  4 of 57-61 nodes, 32 K keys  609, 313,  243       3 M  16 of 24 nodes, 64 heads   152, 115, 86
+    // Of 173 launches (8 to 98304 rows, windows of 128 to 262144 keys) its choice is 1 % behind the best of the three on
+    // average and 23 % at worst; `work` alone, which ignores how many units share it, was 21 % behind, and 7 times at worst.
+    // Measured without the log-sum-exp.  With it units of 64 rows hold one work-group a CU, and units of 32 are faster where
+    // they are chosen too (the last two: 326 against 429, and 122 against 155): still chosen, as for the output alone, since
+    // the scratch is the same for both.
+    const uint64_t score = (rows + 63) / 64 * work;
+    plan.rt = score < 28000 ? 1 : score < 400000 ? 2 : 4;
     // A request's last unit may be short, and so may the padding's.
     plan.units = (uint32_t)(rows / (16 * plan.rt)) + a->batch + 1;
     const uint64_t tiles = cmp_tiles + (a->oriTableWidth + 1) / 2;
