@@ -22,7 +22,10 @@ constexpr int MAX_CHUNKS = 2048;
 constexpr int64_t MAX_PAGES = (int64_t)CHUNK * MAX_CHUNKS;
 constexpr int PATH = 64;                        // path entries that are resident at once
 constexpr int64_t SLICE = 65536;                // bytes of a page that one work-group copies
-constexpr uint32_t FEW_CHUNKS = 8;              // up to which compact_plan counts the pool itself
+// Chunks up to which compact_plan counts the pool itself, in every work-group, where a launch before it would (16 KiB
+// pages, half of them in use, microseconds counted by itself and before: 3000 pages 15.5 and 16.9, 4096 17.0 and 18.2,
+// 6000 25.5 and 22.2, 16000 46.4 and 31.9).
+constexpr uint32_t FEW_CHUNKS = 2;
 // Pools above this size do not fit the memory-side cache: compaction copies past it (1536 pages of 608 KiB with 380
 // moves: 88.6 us, 96.4 with ordinary copies).  Forked tails are read again soon and stay (64 beams: 11.5 us, 13.1 past it).
 constexpr uint64_t STREAMED_POOL = 256ull << 20;
