@@ -4366,6 +4366,6 @@ int sharedkv_c8_xcd_local(void)
 
 uint32_t sharedkv_attention_args_size(void) { return (uint32_t)sizeof(SharedKVArgs); }
 uint32_t sharedkv_cache_args_size(void) { return (uint32_t)sizeof(CacheWriteArgs); }
-uint32_t sharedkv_abi_version(void) { return 3; }
+uint32_t sharedkv_abi_version(void) { return 4; }
 
 }  // extern "C"

@@ -27,8 +27,8 @@
 // What bounds it.  4 * 512 flops for every 512-byte key and query row: from some
 // hundred rows a request on, the matrix instructions and the vector ones beside
 // them (a key's codes to FP16, the softmax).  4 requests of 57-61 tokens and 16
-// heads over 20-32 K rows take 236 us, 860 TFLOP/s, three quarters of a large
-// library FP16 product's rate; a SIMD takes about 4960 cycles for a wave's tile,
+// heads over 20-32 K rows take 231-246 us by the card, 824-880 TFLOP/s, three quarters of
+// a large library FP16 product's rate; a SIMD takes about 4960 cycles for a wave's tile,
 // 2048 of them busy with matrix instructions, beside some 420 vector ones.  Small launches are a chain of
 // round trips (lengths, Q and tables, tiles, states): one request of 8 tokens and
 // 4096 rows takes 13.5 us, 32 of 4-16 tokens 22.6.
@@ -293,8 +293,9 @@ __device__ __forceinline__ int by_length(int group, int units)
     return group < shared ? CUS - shared + group : group < CUS ? group - shared : units - 1 - (group - CUS);
 }
 
-// CAUSAL: compressed rows go by a token's own position (a kernel of its own: the masks' scalars, kept over the tile loop,
-// cost whole contexts 2 %, which launches without them need not pay).
+// CAUSAL: compressed rows go by a token's own position.  A kernel of its own: the masks' scalars, kept over the tile loop,
+// cost whole contexts 2 % (243.3 to 248.1 us, 16 requests of 24 nodes and 64 heads 79.6 to 80.4), which launches without
+// them need not pay.
 template <int TERMS, int RT, bool CAUSAL>
 __global__ void __launch_bounds__(THREADS, TERMS == 2 || RT < 4 ? 2 : 1) tree_attention(const uint64_t cu_q, const uint64_t seq_lens, const uint32_t batch_arg, const uint32_t heads_arg,
                const uint32_t split, const uint32_t tokens_arg, const uint32_t ratio, const uint32_t window_rows,

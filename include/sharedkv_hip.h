@@ -318,7 +318,8 @@ uint32_t sharedkv_path_commit_args_size(void);
 uint32_t sharedkv_page_fork_args_size(void);
 uint32_t sharedkv_page_compact_args_size(void);
 
-/* sizeof(SharedKVArgs), sizeof(CacheWriteArgs), library ABI version. */
+/* sizeof(SharedKVArgs), sizeof(CacheWriteArgs), library ABI version (4 since
+ * TreeAttentionArgs.causalCompressed). */
 uint32_t sharedkv_attention_args_size(void);
 uint32_t sharedkv_cache_args_size(void);
 uint32_t sharedkv_abi_version(void);

@@ -110,6 +110,7 @@ SHAPES = [
     ([24] * 16, [8185 + 128 * b + b % 5 for b in range(16)], 64, 128, False),     # whole units of 64 rows
     ([14] * 10, [128 * 7 * b + 122 + b % 6 for b in range(10)], 64, 128, False),     # of 32
     ([30, 20], [20475, 124], 128, 1000, False),    # units split over items
+    ([1100, 3], [90, 126], 1, 128, False),         # more tokens than parents kept in LDS
     ([3] * 300, [121 + 5 * b for b in range(300)], 2, 128, True),        # more requests than threads
 ]
 
