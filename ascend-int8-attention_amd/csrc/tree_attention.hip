@@ -54,6 +54,7 @@ constexpr int ROOT = 0xffff;
 constexpr int WHOLE = 0x3fffffff;  // tiles of an item where units are not split
 constexpr uint32_t MAX_HEADS = 128;
 constexpr int CUS = 256;
+constexpr uint32_t MAX_WIDTH = (0x7fffffffu - KEYS) / PAGE_ROWS;
 constexpr uint32_t MAX_GROUPS = 0xffffffffu / THREADS;   // the threads of a launch are counted in 32 bits
 // Items of a launch: two work-groups on each of 256 CUs; of small units, whose items differ most, half as many again (32
 // requests of 4-16 nodes: 24.8 us in at most 512 items, 22.7 in 768, 30.1 in 1024).
@@ -1003,9 +1004,9 @@ bool rejected(const TreeAttentionArgs *a)
     if (a->ratio > 1 && (!a->cmp || !a->cmpScale || !a->cmpTable || !a->cmpPages || !a->cmpTableWidth ||
                          (a->cmpStride & 15) || a->cmpStride < (uint64_t)PAGE_ROWS * D || ((a->cmp | a->cmpScale) & 15)))
         return true;
-    // Rows and pages are counted in 32 bits.
-    return a->batch > 0xffffffu || (uint64_t)a->tokens * a->heads > 0x7fff0000ull || a->oriTableWidth > 0x3ffffffu ||
-           a->cmpTableWidth > 0x3ffffffu;
+    // Rows and pages are counted in 32 bits, signed: a table's rows and a tile more.
+    return a->batch > 0xffffffu || (uint64_t)a->tokens * a->heads > 0x7fff0000ull || a->oriTableWidth > MAX_WIDTH ||
+           a->cmpTableWidth > MAX_WIDTH;
 }
 
 struct Plan {

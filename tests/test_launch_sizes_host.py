@@ -50,6 +50,17 @@ def test_trees():
     assert runtime.library().sharedkv_tree_scratch(ctypes.addressof(a), *map(ctypes.byref, sizes)) == 0
 
 
+@pytest.mark.parametrize("field", ["oriTableWidth", "cmpTableWidth"])
+def test_tables_whose_rows_and_a_tile_pass_32_bits(field):
+    """Tiles of a context are its rows, rounded up to 64, in signed 32 bits."""
+    sizes = ctypes.c_uint64(), ctypes.c_uint64()
+    limit = (2 ** 31 - 1 - 64) // 32
+    for width, expected in ((limit, 0), (limit + 1, INVALID), (2 ** 26 - 1, INVALID)):
+        a = good_tree()
+        setattr(a, field, width)
+        assert runtime.library().sharedkv_tree_scratch(ctypes.addressof(a), *map(ctypes.byref, sizes)) == expected
+
+
 def test_ordinary_calls_are_not_refused():
     for launch, block in (("launch_sharedkv_page_fork", good_fork()), ("launch_sharedkv_path_commit", good_commit()),
                           ("launch_sharedkv_page_compact", good_compact())):
