@@ -1032,7 +1032,7 @@ Plan plan_of(const TreeAttentionArgs *a)
     //      263 K  2048 rows, 16384 keys        204, 112,  130       1 M  2048 rows, 65536 keys      749, 364, 296
     //      1.8 M  4 of 57-61 nodes, 32 K keys  609, 313,  243       3 M  16 of 24 nodes, 64 heads   152, 115, 86
     // Of 173 launches (8 to 98304 rows, windows of 128 to 262144 keys) its choice is 1 % behind the best of the three on
-    // average and 23 % at worst; `work` alone, which ignores how many units share it, was 21 % behind, and 7 times at worst.
+    // average and 23 % at worst; bounds on `work` alone, whatever units share it, are 21 % behind, and 7 times at worst.
     // Measured without the log-sum-exp.  With it units of 64 rows hold one work-group a CU, and units of 32 are faster where
     // they are chosen too (the last two: 326 against 429, and 122 against 155): still chosen, as for the output alone, since
     // the scratch is the same for both.

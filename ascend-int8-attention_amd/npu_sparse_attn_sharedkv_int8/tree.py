@@ -114,13 +114,15 @@ def _check_outputs(out, lse, case, parents, scales):
 class PreparedTreeAttention:
     """run() launches on the current stream of the inputs' device, allocates
     nothing and reads nothing back.  Its scratch comes from
-    scratch_allocator(name, shape, dtype, device), by default a new tensor;
-    launches that may overlap must not share it (an operator each, or an
-    allocator by stream).
+    scratch_allocator(name, shape, dtype, device), by default a new tensor, and
+    is cleared by the first run (a new tensor of its own before that); launches
+    that may overlap must not share it (an operator each, or an allocator by
+    stream).
 
     Protocol: BF16 q[T, H, 512], 1..128 heads; INT8 caches [P, 32, 1, 512] with
     any page stride that is a multiple of 16 bytes; frozen FP32[512] scales;
-    ratio 1 (window only) or 128 (and every compressed row); any window >= 1
+    ratio 1 (window only) or 128 (and every compressed row of the committed
+    tokens, or with causal_compressed of a token's own position); any window >= 1
     (2**30 attends the whole context); cu_q rises from 0.  Rows on pages outside the pool or past
     the block table are masked.  Tokens past cu_q[batch], and those of requests
     with seq_lens 0, are graph padding: their outputs are zero.

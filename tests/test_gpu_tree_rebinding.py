@@ -61,6 +61,24 @@ def test_new_tensors(ratio, lse):
     compare(op, first, lse)
 
 
+@pytest.mark.parametrize("nodes,committed,heads", [([7, 12], [500, 4000], 8), ([16] * 30, [0, 17, 128, 500, 9000, 700] * 5, 64)])
+def test_the_log_sum_exp_comes_and_goes(nodes, committed, heads):
+    """Outputs with and without it, bound in turn to one operator: its scratch serves both kernels."""
+    import torch
+    from npu_sparse_attn_sharedkv_int8 import PreparedTreeAttention
+    trees = Trees(42, nodes, committed, heads=heads)
+    case, parents, scale, cmp_scale = trees.device()
+    op = PreparedTreeAttention(case, parents, scale, cmp_scale)
+    for lse in (False, True, False):
+        out = torch.full_like(case.q, float("nan"))
+        op._rebind_same_geometry(case, parents, output=out, lse_output=torch.full(
+            case.q.shape[:2], float("nan"), device="cuda") if lse else None)
+        say(f"[rebinding] {len(nodes)} requests, lse={lse}")
+        op.run()
+        torch.cuda.synchronize()
+        compare(op, trees, lse)
+
+
 def adapter(scale, cmp_scale):
     from npu_sparse_attn_sharedkv_int8 import vllm_adapter
     impl = SimpleNamespace(swa_cache_layer=SimpleNamespace(prefix="unit.swa_cache"), head_dim=512)
