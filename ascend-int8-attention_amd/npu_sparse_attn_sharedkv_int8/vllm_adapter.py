@@ -260,17 +260,19 @@ class SharedKVLayer:
         With tree_parents (INT32 [T], each token's parent by its index in the
         request) the tokens are the drafted trees of PreparedTreeAttention, with
         the causal rule of every call for the compressed rows: a token sees
-        those completed up to its own position, which the call finds written."""
+        those completed up to its own position, which the call finds written.
+        Engines that write none for drafted tokens say
+        tree_causal_compressed=False: then all see the committed tokens' rows."""
         case, return_lse = parse_attention_call(q, kw)
-        parents = kw.get("tree_parents")
+        parents, causal = kw.get("tree_parents"), bool(kw.get("tree_causal_compressed", True))
         out = torch.empty_like(q)
         lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
-        key = (launch_shape(case, return_lse), parents is not None, q.device, stream_key(q.device))
+        key = (launch_shape(case, return_lse), parents is not None and (causal,), q.device, stream_key(q.device))
         op = self.operators.get(key)
         if op is None and parents is not None:
             op = PreparedTreeAttention(case, parents, self.scale("ori", q.device)[0],
                                        self.scale("cmp", q.device)[0] if case.ratio > 1 else None, output=out,
-                                       lse_output=lse, scratch_allocator=scratch_allocator, causal_compressed=True)
+                                       lse_output=lse, scratch_allocator=scratch_allocator, causal_compressed=causal)
             self.operators.put(key, op)
         elif op is None:
             op = PreparedAttention(case, self.scale("ori", q.device)[0],

@@ -5,6 +5,7 @@ for scales far apart, which are not drawn here), and a chain with
 PreparedAttention itself."""
 import sys
 import zlib
+from types import SimpleNamespace
 
 import numpy as np
 import pytest
@@ -187,6 +188,25 @@ def test_adapter_follows_its_causal_rule():
         layer.attention(case.q, **call(case))
         torch.cuda.synchronize()
         compare(trees, out, lse.squeeze(-1))
+
+
+def test_adapter_without_rows_for_drafted_tokens():
+    """tree_causal_compressed=False beside the causal call of the same shape: an operator each."""
+    import torch
+    from tests.test_gpu_tree import compare as committed_only
+    trees = Causal(76, [8, 16], [250, 8180])
+    case, parents, scale, cmp_scale = trees.device()
+    layer = adapter(scale, cmp_scale)
+    for _ in range(2):
+        out, lse = layer.attention(case.q, tree_parents=parents, **call(case))
+        less, less_lse = layer.attention(case.q, tree_parents=parents, tree_causal_compressed=False, **call(case))
+        torch.cuda.synchronize()
+        say("[causal] adapter, both rules")
+        compare(trees, out, lse.squeeze(-1))
+        want = Trees.expect(trees, 3)
+        committed_only(SimpleNamespace(out=less, lse=less_lse.squeeze(-1)),
+                       SimpleNamespace(expect=lambda terms: want), True)
+        assert len(layer.operators.values()) == 2
 
 
 def test_speculative_chains_over_both_caches():
