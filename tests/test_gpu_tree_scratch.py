@@ -70,3 +70,22 @@ def test_scratch_of_one_allocator_on_its_stream():
     for op, t in zip(ops, pair):
         compare(op, t, True)
     assert (held["tree_workspace"][:64] == 0).any() and not ops[0]._unclear
+
+
+@pytest.mark.parametrize("lse", [False, True], ids=["out", "lse"])
+def test_repeated_runs_agree_bit_for_bit(lse):
+    """Whichever of a unit's items ends last joins them, in the items' order."""
+    import torch
+    from npu_sparse_attn_sharedkv_int8 import PreparedTreeAttention
+    trees = Trees(85, [7, 12, 16], [500, 4000, 12000], ratio=1, window=1 << 30)
+    case, parents, scale, cmp_scale = trees.device()
+    op = PreparedTreeAttention(case, parents, scale, cmp_scale, return_lse=lse)
+    assert op.partial is not None
+    say(f"[scratch] twenty runs, lse={lse}")
+    op.run()
+    first = [x.clone() for x in (op.out, op.lse) if x is not None]
+    for _ in range(20):
+        op.out.fill_(float("nan"))
+        op.run()
+        assert all(torch.equal(a, b) for a, b in zip(first, (op.out, op.lse)))
+    compare(op, trees, lse)
