@@ -90,7 +90,7 @@ PyObject *cache_write(PyObject *, PyObject *const *args, Py_ssize_t nargs)
     Py_RETURN_NONE;
 }
 
-// A launch that takes (address, stream): the tree and page entries.
+// A launch that takes (address, stream): the entries of trees, block-scaled caches and pages.
 template <typename Args>
 PyObject *launch_block(PyObject *const *args, Py_ssize_t nargs, int (*launch)(void *, const Args *), const char *what)
 {
@@ -116,6 +116,14 @@ PyObject *tree_attention(PyObject *, PyObject *const *args, Py_ssize_t nargs)
 {
     return launch_block(args, nargs, launch_sharedkv_tree, "sharedkv tree attention");
 }
+PyObject *cache_append(PyObject *, PyObject *const *args, Py_ssize_t nargs)
+{
+    return launch_block(args, nargs, launch_sharedkv_append, "sharedkv cache append");
+}
+PyObject *block_attention(PyObject *, PyObject *const *args, Py_ssize_t nargs)
+{
+    return launch_block(args, nargs, launch_sharedkv_block, "sharedkv block attention");
+}
 PyObject *path_commit(PyObject *, PyObject *const *args, Py_ssize_t nargs)
 {
     return launch_block(args, nargs, launch_sharedkv_path_commit, "sharedkv path commit");
@@ -136,6 +144,10 @@ PyMethodDef methods[] = {
      "cache_write(address, blocks, stream): launch an INT8 cache-write argument block on a HIP stream"},
     {"tree_attention", (PyCFunction)(void (*)(void))tree_attention, METH_FASTCALL,
      "tree_attention(address, stream): launch a tree attention argument block on a HIP stream"},
+    {"cache_append", (PyCFunction)(void (*)(void))cache_append, METH_FASTCALL,
+     "cache_append(address, stream): launch a cache append argument block on a HIP stream"},
+    {"block_attention", (PyCFunction)(void (*)(void))block_attention, METH_FASTCALL,
+     "block_attention(address, stream): launch a block-scaled attention argument block on a HIP stream"},
     {"path_commit", (PyCFunction)(void (*)(void))path_commit, METH_FASTCALL,
      "path_commit(address, stream): launch a path commit argument block on a HIP stream"},
     {"page_fork", (PyCFunction)(void (*)(void))page_fork, METH_FASTCALL,

@@ -11,7 +11,7 @@ __version__ = "0.1.0+mi355x"
 __stage__ = "c8-gfx950"
 
 __all__ = ["CacheQuantization", "SharedKVCase", "PreparedAttention", "PreparedCacheWrite", "PreparedTreeAttention",
-           "PreparedPathCommit", "PreparedPageFork", "PreparedPageCompact"]
+           "PreparedCacheAppend", "PreparedBlockAttention", "PreparedPathCommit", "PreparedPageFork", "PreparedPageCompact"]
 
 _EXPORTS = {
     "CacheQuantization": ("contract", "CacheQuantization"),
@@ -19,6 +19,8 @@ _EXPORTS = {
     "PreparedAttention": ("attention", "PreparedAttention"),
     "PreparedCacheWrite": ("cache", "PreparedCacheWrite"),
     "PreparedTreeAttention": ("tree", "PreparedTreeAttention"),
+    "PreparedCacheAppend": ("block_cache", "PreparedCacheAppend"),
+    "PreparedBlockAttention": ("block_cache", "PreparedBlockAttention"),
     "PreparedPathCommit": ("pages", "PreparedPathCommit"),
     "PreparedPageFork": ("pages", "PreparedPageFork"),
     "PreparedPageCompact": ("pages", "PreparedPageCompact"),

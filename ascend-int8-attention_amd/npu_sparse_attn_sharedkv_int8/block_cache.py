@@ -1,0 +1,324 @@
+"""Caches with a scale for each page of 32 rows and KV head: rows appended with
+their position rotation applied on the way, and attention over them.
+
+No counterpart in the reference, whose caches hold INT8 codes with frozen
+channel scales from a calibration.  Here a page of a KV head has one FP32 scale,
+made from the rows themselves when they are appended:
+
+  cache  INT8 or float8_e4m3fn [pages, 32, KV heads, 512], any page stride that
+         is a multiple of 16 bytes
+  scale  FP32 [pages, KV heads], any page stride: a tensor of its own, or a view
+         of the bytes behind each page's codes in one backing, so that whatever
+         moves whole pages (PreparedPageFork, PreparedPageCompact) moves both
+  value  code * scale
+
+PreparedCacheAppend fills such caches, and with inverse_scale the framework's
+caches of frozen channel scales (PreparedCacheWrite's codes, of rotated rows);
+PreparedBlockAttention attends them.
+"""
+import ctypes
+
+import torch
+
+from .pages import _apart, _ints, _overlaps, _runs
+from .runtime import BlockAttentionArgs, CacheAppendArgs, library, native_launcher
+from .tree import _check_query, MAX_WINDOW, RATIOS
+
+BLOCK, DIM = 32, 512
+MAX_HEADS = 128
+CODES = {torch.int8: 0, torch.float8_e4m3fn: 1}
+MAX_THREADS = 2 ** 32 - 1
+APPEND_THREADS = 512
+
+
+def _check_block_cache(cache, scale, device, unit):
+    """A cache [pages, 32, heads, 512] with its block scales (None: checked by the caller)."""
+    if not isinstance(cache, torch.Tensor) or cache.dtype not in CODES or cache.ndim != 4 \
+            or cache.shape[1] != BLOCK or cache.shape[3] != DIM or cache.device != device:
+        raise ValueError("Expected INT8 or float8_e4m3fn cache[pages,32,heads,512] on the same GPU")
+    pages, _, heads, _ = cache.shape
+    if not 1 <= heads <= MAX_HEADS or not pages or pages * BLOCK >= 2 ** 31:
+        raise ValueError(f"Expected 1..{MAX_HEADS} KV heads and pages of fewer than 2**31 rows")
+    if (cache.stride(3) != 1 or (heads > 1 and cache.stride(2) != DIM) or cache.stride(1) != heads * DIM
+            or cache.stride(0) < BLOCK * heads * DIM or cache.stride(0) % unit or cache.data_ptr() % unit):
+        raise ValueError(f"Cache pages must be contiguous, {unit}-byte aligned and apart")
+    if scale is None:
+        return
+    if (not isinstance(scale, torch.Tensor) or scale.dtype != torch.float32 or tuple(scale.shape) != (pages, heads)
+            or scale.device != device or (heads > 1 and scale.stride(1) != 1) or (pages > 1 and scale.stride(0) < heads)):
+        raise ValueError("Expected FP32 scale[pages,heads] of the cache, a page's heads side by side")
+    if not _apart(_runs(cache, 1), _runs(scale, 1)):
+        raise ValueError("Scales must not overlap the cache's codes")
+
+
+def _step(tensor, dim):
+    """Stride of a dimension, 0 where it has one entry (whatever its stride says)."""
+    return tensor.stride(dim) if tensor.shape[dim] > 1 else 0
+
+
+class PreparedCacheAppend:
+    """Appends rows to a paged cache, rotated by their positions.
+
+    Request b has the new rows cu_q[b] .. cu_q[b + 1] - 1 of `updates` (BF16
+    [T, 512] or [T, heads, 512], any strides of whole 16 bytes), the last of its
+    seq_lens[b] rows; row r goes to row r % 32 of page block_table[b, r // 32].
+
+    rotation FP32 [N, R] (R a multiple of 16): the cosines of R / 2 angles, then
+    their sines, for each position.  The last R channels of a row turn by those
+    of its position, positions INT32 / INT64 [T] (by default the row's own index
+    r), in pairs 2k, 2k + 1 or, with interleaved=False, k and k + R / 2:
+    a' = a cos - b sin, b' = a sin + b cos.  Without rotation rows go as they are.
+
+    scale FP32 [pages, heads] (INT8 or float8_e4m3fn caches): a page's scale is
+    that of its first appended rows, max(m / D, 1e-8) with m their largest
+    absolute value and D = 127 or 448, where the page's row 0 is among them, and
+    otherwise doubled as often as the new rows need, the codes before them
+    rounded to the new scale.  Code = the value / scale to the nearest, ties to
+    even.  NaN is stored as 0 (INT8) or NaN (e4m3) and infinities as the largest
+    value; neither spoils the page's other rows.
+    inverse_scale FP32 [512] (INT8, one head): frozen channel scales, the codes
+    of PreparedCacheWrite.
+
+    Rows on no page of the pool, past the block table or with a position outside
+    the rotation are skipped; so are tokens past cu_q[batch] and requests with
+    seq_lens 0.  Bytes behind a request's last row are left as they are.  No two
+    requests append to one page in a call (PreparedPageFork sees to that).
+    run() launches on the current stream of the cache's device, allocates
+    nothing, reads nothing back and can be captured.  Codes of a page whose rows
+    were appended in several calls depend on how they were divided (by the
+    scale's growth), nothing else does.
+    """
+
+    def __init__(self, cache, updates, block_table, cu_q, seq_lens, *, scale=None, inverse_scale=None, rotation=None,
+                 positions=None, interleaved=True):
+        self.args = CacheAppendArgs()
+        self._bind(cache, updates, block_table, cu_q, seq_lens, scale, inverse_scale, rotation, positions, interleaved)
+        self.native = native_launcher()
+        self.argument_address = ctypes.addressof(self.args)
+
+    def _bind(self, cache, updates, block_table, cu_q, seq_lens, scale, inverse_scale, rotation, positions, interleaved):
+        if not isinstance(cache, torch.Tensor) or cache.device.type != "cuda":
+            raise ValueError("Expected a cache on a GPU")
+        device = cache.device
+        if (scale is None) == (inverse_scale is None):
+            raise ValueError("Expected block scales (scale) or frozen channel scales (inverse_scale)")
+        _check_block_cache(cache, scale, device, 8)
+        heads = cache.shape[2]
+        if inverse_scale is not None:
+            if cache.dtype != torch.int8 or heads != 1:
+                raise ValueError("Frozen channel scales go with INT8 caches of one head")
+            if (inverse_scale.dtype != torch.float32 or tuple(inverse_scale.shape) != (DIM,)
+                    or not inverse_scale.is_contiguous() or inverse_scale.device != device
+                    or inverse_scale.data_ptr() % 16):
+                raise ValueError("Expected frozen contiguous FP32 inverse_scale[512]")
+        if (not isinstance(updates, torch.Tensor) or updates.dtype != torch.bfloat16 or updates.ndim not in (2, 3)
+                or updates.shape[-1] != DIM or (updates.shape[1] if updates.ndim == 3 else 1) != heads
+                or updates.device != device or updates.stride(-1) != 1):
+            raise ValueError("Expected BF16 updates[T,heads,512] (or [T,512]) with contiguous rows")
+        steps = _step(updates, 0), _step(updates, 1) if updates.ndim == 3 else 0
+        if steps[0] % 8 or steps[1] % 8 or updates.data_ptr() % 16:
+            raise ValueError("Updates rows must be 16-byte aligned")
+        tokens = updates.shape[0]
+        if not isinstance(seq_lens, torch.Tensor) or not isinstance(block_table, torch.Tensor):
+            raise ValueError("Expected INT32 seq_lens[batch] and block_table[batch,pages]")
+        batch = seq_lens.numel()
+        _ints(seq_lens, (batch,), device, "seq_lens")
+        _ints(cu_q, (batch + 1,), device, "cu_q")
+        _ints(block_table, (batch, None), device, "block_table")
+        if not batch or not block_table.shape[1]:
+            raise ValueError("Expected one request and table entry or more")
+        if block_table.shape[1] > (2 ** 31 - 1) // BLOCK or tokens >= 2 ** 31 \
+                or (tokens // BLOCK + 2 * batch) * heads * APPEND_THREADS > MAX_THREADS:
+            raise ValueError("This launch is outside the kernel's limits (2**23 pages of new rows, 2**26 of a request)")
+        rotary = rows = 0
+        if rotation is not None:
+            if (not isinstance(rotation, torch.Tensor) or rotation.dtype != torch.float32 or rotation.ndim != 2
+                    or rotation.device != device or not rotation.shape[0]):
+                raise ValueError("Expected FP32 rotation[positions,R]")
+            rows, rotary = rotation.shape
+            if (not 16 <= rotary <= DIM or rotary % 16 or rotation.stride(1) != 1 or rotation.data_ptr() % 16
+                    or rows >= 2 ** 32 or _step(rotation, 0) % 4 or (rows > 1 and rotation.stride(0) < rotary)):
+                raise ValueError("Expected R a multiple of 16 up to 512 and 16-byte aligned rows of rotation[positions,R]")
+        if positions is not None and (
+                rotation is None or not isinstance(positions, torch.Tensor) or tuple(positions.shape) != (tokens,)
+                or positions.dtype not in (torch.int32, torch.int64) or positions.device != device
+                or not positions.is_contiguous()):
+            raise ValueError("Expected contiguous INT32/INT64 positions[T] beside a rotation")
+        inputs = [x for x in (updates, block_table, cu_q, seq_lens, inverse_scale, rotation, positions) if x is not None]
+        if _overlaps(cache, inputs) or scale is not None and _overlaps(scale, inputs):
+            raise ValueError("The cache and its scales must not overlap the other inputs")
+        self.cache, self.scale = cache, scale
+        self.inputs = inputs
+        ptr = lambda t: t.data_ptr() if t is not None else 0  # noqa: E731
+        args = self.args
+        for name, value in dict(
+                cache=ptr(cache), updates=ptr(updates), table=ptr(block_table), cuQ=ptr(cu_q), seqLens=ptr(seq_lens),
+                positions=ptr(positions), rotation=ptr(rotation), scale=ptr(scale), inverseScale=ptr(inverse_scale),
+                pageStride=cache.stride(0), updateStride=steps[0], updateHeadStride=steps[1],
+                scaleStride=_step(scale, 0) if scale is not None else 0,
+                rotationStride=rotation.stride(0) if rows > 1 else rotary, tokens=tokens, batch=batch, heads=heads,
+                pages=cache.shape[0], tableWidth=block_table.shape[1], rotary=rotary, rotationRows=rows,
+                interleaved=int(bool(interleaved)),
+                int64Positions=int(positions is not None and positions.dtype == torch.int64),
+                codes=CODES[cache.dtype]).items():
+            setattr(args, name, value)
+        self.interleaved = interleaved
+        self.device_index = device.index if device.index is not None else torch.cuda.current_device()
+
+    def _rebind(self, cache, updates, block_table, cu_q, seq_lens, *, scale=None, inverse_scale=None, rotation=None,
+                positions=None):
+        """Serving fast path: other tensors, of any sizes, under the constructor's checks."""
+        self._bind(cache, updates, block_table, cu_q, seq_lens, scale, inverse_scale, rotation, positions,
+                   self.interleaved)
+
+    def run(self):
+        """Launch on the current stream of the cache's device; returns the cache."""
+        if self.args.tokens:
+            self.native.launch("cache_append", self.argument_address, self.device_index)
+        return self.cache
+
+
+def _check_inputs(case, ori_scale, cmp_scale):
+    """Refuses what the kernel cannot take; returns the launch's geometry, (device, the argument block's sizes)."""
+    q = case.q
+    _check_query(q)
+    tokens, heads, _ = q.shape
+    if case.ratio not in RATIOS or case.cmp_indices is not None or case.ori_indices is not None:
+        raise ValueError("Block-scaled caches are attended as a window (ratio 1) or a window and every compressed row "
+                         "(ratio 128)")
+    if not 1 <= case.window <= MAX_WINDOW:
+        raise ValueError("Expected a positive window")
+    device = q.device
+    if not isinstance(case.seq_lens, torch.Tensor):
+        raise ValueError("Expected INT32 seq_lens[batch]")
+    batch = case.seq_lens.numel()
+    caches = [(case.ori, case.ori_block_table, ori_scale)]
+    if case.ratio != 1:
+        caches.append((case.cmp, case.cmp_block_table, cmp_scale))
+    for cache, table, scale in caches:
+        if scale is None:
+            raise ValueError("Expected the block scales of each cache")
+        _check_block_cache(cache, scale, device, 16)
+        _ints(table, (batch, None), device, "block_table")
+        if not table.shape[1]:
+            raise ValueError("Expected a block table of one page or more")
+    kv_heads = case.ori.shape[2]
+    if heads % kv_heads or any(c.shape[2] != kv_heads or c.dtype != case.ori.dtype for c, _, _ in caches):
+        raise ValueError("Expected query heads in equal groups over the KV heads, and caches of one kind")
+    if not batch:
+        raise ValueError("Expected one request or more")
+    _ints(case.seq_lens, (batch,), device, "seq_lens")
+    _ints(case.cu_q, (batch + 1,), device, "cu_q")
+    sink = case.sink
+    if not isinstance(sink, torch.Tensor) or tuple(sink.shape) != (heads,) or sink.dtype != torch.float32 \
+            or sink.device != device or not sink.is_contiguous():
+        raise ValueError("Expected FP32 sink[heads]")
+    sizes = dict(tokens=tokens, heads=heads, kvHeads=kv_heads, batch=batch, oriPages=case.ori.shape[0],
+                 oriStride=case.ori.stride(0), oriScaleStride=_step(ori_scale, 0),
+                 oriTableWidth=case.ori_block_table.shape[1], ratio=case.ratio, window=case.window,
+                 codes=CODES[case.ori.dtype], softmaxScale=case.softmax_scale)
+    if case.ratio != 1:
+        sizes.update(cmpPages=case.cmp.shape[0], cmpStride=case.cmp.stride(0), cmpScaleStride=_step(cmp_scale, 0),
+                     cmpTableWidth=case.cmp_block_table.shape[1])
+    return device, sizes
+
+
+class PreparedBlockAttention:
+    """Attention over caches with block scales.
+
+    `case` is a SharedKVCase whose caches are INT8 or float8_e4m3fn [pages, 32,
+    KV heads, 512] with ori_scale / cmp_scale FP32 [pages, KV heads]: BF16
+    q[T, H, 512], H up to 128 and a multiple of the KV heads (head h attends KV
+    head h // (H / KV heads)); ratio 1 (original rows only) or 128 (and
+    compressed ones); any window >= 1 (2**30 attends whole contexts); requests
+    of one token or many.  Token i of a request's T stands at position
+    P = seq_lens[b] - T + i and sees
+      original rows j <= P with j > P - window,
+      with ratio 128 the compressed rows r < (P + 1) // 128.
+    With v_j = code_j * scale[page of j],
+      out = sum_j e^{s_j} v_j / (e^{sink} + sum_j e^{s_j}),  s_j = softmax_scale q v_j
+    and lse = log of the denominator.
+
+    Rows on pages outside the pool, or past the block table, are masked; what
+    masked rows hold (codes, scales, NaN or infinities) reaches no output.  A
+    token that sees no row gets 0 (lse = sink).  Tokens past cu_q[batch], and
+    those of requests with seq_lens 0, are graph padding: zero.  cu_q rises from
+    0; scales are not negative.
+
+    run() launches on the current stream of the inputs' device (one kernel, or
+    two where contexts are split), allocates nothing and reads nothing back.
+    Its scratch comes from scratch_allocator(name, shape, dtype, device), by
+    default a new tensor, and may hold anything; launches that may overlap must
+    not share it (an operator each, or an allocator by stream).
+    """
+
+    def __init__(self, case, ori_scale, cmp_scale=None, *, output=None, return_lse=False, lse_output=None,
+                 scratch_allocator=None):
+        self.geometry = _check_inputs(case, ori_scale, cmp_scale)
+        device, sizes = self.geometry
+        out = output if output is not None else torch.empty_like(case.q)
+        lse = lse_output
+        if lse is None and return_lse:
+            lse = torch.empty(case.q.shape[:2], dtype=torch.float32, device=device)
+        self._check_outputs(out, lse, case, ori_scale, cmp_scale)
+        self.args = BlockAttentionArgs(**sizes)
+        self._bind(case, ori_scale, cmp_scale, out, lse)
+        self._take_scratch(scratch_allocator, device)
+        self.native = native_launcher()
+        self.argument_address = ctypes.addressof(self.args)
+        self.device_index = device.index if device.index is not None else torch.cuda.current_device()
+
+    @staticmethod
+    def _check_outputs(out, lse, case, ori_scale, cmp_scale):
+        q = case.q
+        if (not isinstance(out, torch.Tensor) or tuple(out.shape) != tuple(q.shape) or out.device != q.device
+                or out.dtype != torch.bfloat16 or not out.is_contiguous() or out.data_ptr() % 16):
+            raise ValueError("Invalid output buffer")
+        if lse is not None and (tuple(lse.shape) != tuple(q.shape[:2]) or lse.dtype != torch.float32
+                                or lse.device != q.device or not lse.is_contiguous()):
+            raise ValueError("Invalid FP32 LSE[T,H] output buffer")
+        inputs = [q, case.cu_q, case.seq_lens, case.sink, case.ori, case.ori_block_table, ori_scale]
+        if case.ratio != 1:
+            inputs += [case.cmp, case.cmp_block_table, cmp_scale]
+        # A work-group may end, and write, before another reads.
+        if _overlaps(out, inputs) or lse is not None and _overlaps(lse, inputs + [out]):
+            raise ValueError("Outputs must not overlap inputs or each other")
+
+    def _take_scratch(self, allocator, device):
+        sizes = ctypes.c_uint64(), ctypes.c_uint64()
+        if self.args.tokens and library().sharedkv_block_scratch(ctypes.addressof(self.args), *map(ctypes.byref, sizes)):
+            raise ValueError("This launch is outside the kernel's limits (some 2^30 query rows, 2^24 requests)")
+        allocate = allocator or (lambda name, shape, dtype, dev: torch.empty(shape, dtype=dtype, device=dev))
+        states, units = (size.value // 4 for size in sizes)
+        self.partial = self.units = None
+        if states:
+            self.partial = allocate("block_partial", (states,), torch.float32, device)
+            self.units = allocate("block_units", (units,), torch.int32, device)
+            self.args.partial, self.args.units = self.partial.data_ptr(), self.units.data_ptr()
+
+    def _bind(self, case, ori_scale, cmp_scale, out, lse):
+        cmp = case.ratio != 1
+        for name, tensor in (("q", case.q), ("ori", case.ori), ("oriTable", case.ori_block_table),
+                             ("oriScale", ori_scale), ("cmp", case.cmp if cmp else None),
+                             ("cmpTable", case.cmp_block_table if cmp else None), ("cmpScale", cmp_scale if cmp else None),
+                             ("cuQ", case.cu_q), ("seqLens", case.seq_lens), ("sinks", case.sink), ("out", out),
+                             ("lse", lse)):
+            setattr(self.args, name, tensor.data_ptr() if tensor is not None else 0)
+        self.case, self.scales, self.out, self.lse = case, (ori_scale, cmp_scale), out, lse
+
+    def _rebind_same_geometry(self, case, ori_scale=None, cmp_scale=None, *, output=None, lse_output=None):
+        """Serving fast path: same geometry, new tensors (scales and outputs as before where none are given), under the
+        constructor's checks."""
+        ori_scale = self.scales[0] if ori_scale is None else ori_scale
+        cmp_scale = self.scales[1] if cmp_scale is None else cmp_scale
+        if _check_inputs(case, ori_scale, cmp_scale) != self.geometry:
+            raise ValueError("Rebinding keeps the device and every size of the launch")
+        out, lse = (output, lse_output) if output is not None else (self.out, self.lse)
+        self._check_outputs(out, lse, case, ori_scale, cmp_scale)
+        self._bind(case, ori_scale, cmp_scale, out, lse)
+
+    def run(self):
+        """Launch on the current stream of the case's device; returns .out."""
+        if self.args.tokens:
+            self.native.launch("block_attention", self.argument_address, self.device_index)
+        return self.out

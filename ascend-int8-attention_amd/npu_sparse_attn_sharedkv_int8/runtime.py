@@ -64,6 +64,21 @@ class TreeAttentionArgs(ctypes.Structure):
                       [("softmaxScale", ctypes.c_float), ("causalCompressed", ctypes.c_uint32)])
 
 
+class CacheAppendArgs(ctypes.Structure):
+    """include/sharedkv_hip.h."""
+    _fields_ = _block("cache updates table cuQ seqLens positions rotation scale inverseScale pageStride updateStride "
+                      "updateHeadStride scaleStride rotationStride",
+                      "tokens batch heads pages tableWidth rotary rotationRows interleaved int64Positions codes")
+
+
+class BlockAttentionArgs(ctypes.Structure):
+    """include/sharedkv_hip.h."""
+    _fields_ = _block("q ori cmp oriScale cmpScale oriTable cmpTable cuQ seqLens sinks out lse partial units oriStride "
+                      "cmpStride oriScaleStride cmpScaleStride",
+                      "tokens heads kvHeads batch oriPages cmpPages oriTableWidth cmpTableWidth ratio window codes",
+                      [("softmaxScale", ctypes.c_float)])
+
+
 class PathCommitArgs(ctypes.Structure):
     """include/sharedkv_hip.h."""
     _fields_ = _block("caches table cuQ seqLens paths pathLens lengths",
@@ -85,6 +100,8 @@ class PageCompactArgs(ctypes.Structure):
 # Entries that take (stream, argument block): library function, block, its size query.
 BLOCK_LAUNCHES = {
     "tree_attention": ("launch_sharedkv_tree", TreeAttentionArgs, "sharedkv_tree_args_size"),
+    "cache_append": ("launch_sharedkv_append", CacheAppendArgs, "sharedkv_append_args_size"),
+    "block_attention": ("launch_sharedkv_block", BlockAttentionArgs, "sharedkv_block_args_size"),
     "path_commit": ("launch_sharedkv_path_commit", PathCommitArgs, "sharedkv_path_commit_args_size"),
     "page_fork": ("launch_sharedkv_page_fork", PageForkArgs, "sharedkv_page_fork_args_size"),
     "page_compact": ("launch_sharedkv_page_compact", PageCompactArgs, "sharedkv_page_compact_args_size"),
@@ -97,7 +114,8 @@ EXPORTS = ("launch_sharedkv_c8_sparse", "launch_sharedkv_c8_dense", "launch_shar
            "sharedkv_c8_workspace_bytes", "sharedkv_c8_partial_bytes", "sharedkv_c8_noalloc_scratch_bytes",
            "sharedkv_c8_noalloc_layout", "sharedkv_c8_set_merge_mode", "sharedkv_c8_set_xcd_local",
            "sharedkv_c8_xcd_local", "sharedkv_attention_args_size", "sharedkv_cache_args_size",
-           "sharedkv_abi_version", "sharedkv_tree_scratch", "sharedkv_page_fork_workspace", "sharedkv_page_compact_workspace",
+           "sharedkv_abi_version", "sharedkv_tree_scratch", "sharedkv_block_scratch",
+           "sharedkv_page_fork_workspace", "sharedkv_page_compact_workspace",
            *(name for launch, _, size in BLOCK_LAUNCHES.values() for name in (launch, size)))
 
 
@@ -148,9 +166,10 @@ def library():
         getattr(lib, size).restype = ctypes.c_uint32
         if getattr(lib, size)() != ctypes.sizeof(block):
             raise RuntimeError(f"Native {block.__name__} ABI changed; rebuild the library")
-    lib.sharedkv_tree_scratch.argtypes = [ctypes.c_void_p, ctypes.POINTER(ctypes.c_uint64),
-                                          ctypes.POINTER(ctypes.c_uint64)]
-    lib.sharedkv_tree_scratch.restype = ctypes.c_int
+    for name in ("sharedkv_tree_scratch", "sharedkv_block_scratch"):
+        getattr(lib, name).argtypes = [ctypes.c_void_p, ctypes.POINTER(ctypes.c_uint64),
+                                       ctypes.POINTER(ctypes.c_uint64)]
+        getattr(lib, name).restype = ctypes.c_int
     for name, count in (("sharedkv_page_fork_workspace", 3), ("sharedkv_page_compact_workspace", 1)):
         getattr(lib, name).argtypes = [ctypes.c_uint32] * count
         getattr(lib, name).restype = ctypes.c_uint64

@@ -147,6 +147,67 @@ typedef struct PageCompactArgs {
     uint64_t pageBytes;
 } PageCompactArgs;
 
+/* Rows appended to paged 8-bit caches, their position rotation applied on the
+ * way (no counterpart in the reference).  Request b has the new rows cuQ[b] ..
+ * cuQ[b + 1] - 1 of updates (BF16, token t and KV head h at updates +
+ * 2 (t updateStride + h updateHeadStride) bytes, 512 values), the last of its
+ * seqLens[b] rows; row r lies on page table[b][r / 32] of the cache (pages of
+ * 32 rows of `heads` * 512 bytes, pageStride bytes apart).
+ * rotary > 0: channels 512 - rotary on are rotated.  rotation (FP32
+ * [rotationRows], rotationStride floats apart) holds rotary / 2 cosines and as
+ * many sines for each position; positions (INT32, or INT64 where
+ * int64Positions is 1, [tokens]; 0: the row's own index) names a row's.
+ * Channels 2k and 2k + 1 of the rotated ones turn together where interleaved
+ * is 1, else k and k + rotary / 2: a' = a cos - b sin, b' = a sin + b cos.
+ * inverseScale (FP32 [512], one KV head, INT8): the codes of launch_cache_write,
+ * of the rotated value as FP32.  Otherwise scale FP32 [pages][heads]
+ * (scaleStride floats between pages) holds a scale for each page and KV head,
+ * and codes are INT8 (codes 0, largest D = 127) or OCP e4m3 (1, D = 448):
+ *   a page whose row 0 is appended gets scale = max(m / D, 1e-8), m the largest
+ *   absolute value of its new rows as FP32; one that has rows keeps its scale,
+ *   doubled as often as it takes to reach m / D, and where it is doubled its
+ *   codes become round(code / 2^k);
+ *   code = round(value / scale), to the nearest, ties to even.
+ * NaN values become 0 (INT8) or NaN of either sign (e4m3) and are none of m; infinities count
+ * as the largest FP32 number.  A scale that is no positive number counts as
+ * that of a new page.  Rows on no page of the pool, past the block table,
+ * below row 0 or with a position outside the table are skipped; padding as in
+ * TreeAttentionArgs.  No two rows of a launch may lie on the same place, and
+ * no two requests append to one page. */
+typedef struct CacheAppendArgs {
+    uint64_t cache, updates, table, cuQ, seqLens, positions, rotation, scale, inverseScale;
+    uint64_t pageStride, updateStride, updateHeadStride, scaleStride, rotationStride;
+    uint32_t tokens, batch, heads, pages, tableWidth, rotary, rotationRows, interleaved, int64Positions, codes;
+} CacheAppendArgs;
+
+/* Attention over caches with a scale for each page and KV head, as
+ * CacheAppendArgs fills them (no counterpart in the reference).  Request b has
+ * the query tokens cuQ[b] .. cuQ[b + 1] - 1 (T of them) and seqLens[b] rows; its
+ * token i stands at position P = seqLens[b] - T + i and sees
+ *   original rows j <= P with j > P - window,
+ *   with ratio > 1 compressed rows r < (P + 1) / ratio.
+ * Query head h attends KV head h / (heads / kvHeads).  With v_j = code_j *
+ * scale[page of j] and s_j = softmaxScale q v_j,
+ *   out = sum_j e^{s_j} v_j / (e^{sink} + sum_j e^{s_j}), lse = log of the denominator.
+ * q, out BF16 [tokens][heads][512], heads 1..128, a multiple of kvHeads; sinks
+ * FP32 [heads]; lse FP32 [tokens][heads] or 0; ori / cmp pages of 32 rows of
+ * kvHeads * 512 codes (INT8: codes 0, OCP e4m3: 1), page strides in bytes,
+ * multiples of 16; oriScale / cmpScale FP32 [pages][kvHeads],
+ * oriScaleStride / cmpScaleStride floats between pages, no scale negative
+ * (one below 2^-80 counts as 2^-80 where it weighs values).  Rows on no page
+ * of the pool or past the block table are masked, and nothing they hold, nor
+ * their page's scale, reaches an output; the same holds for rows that a token
+ * does not see.  Padding as in TreeAttentionArgs.  partial and units: the
+ * scratch that sharedkv_block_scratch names; any contents, and launches that
+ * may overlap need their own. */
+typedef struct BlockAttentionArgs {
+    uint64_t q, ori, cmp, oriScale, cmpScale, oriTable, cmpTable, cuQ;
+    uint64_t seqLens, sinks, out, lse, partial, units;
+    uint64_t oriStride, cmpStride, oriScaleStride, cmpScaleStride;
+    uint32_t tokens, heads, kvHeads, batch, oriPages, cmpPages, oriTableWidth, cmpTableWidth, ratio, window, codes;
+    float softmaxScale;
+} BlockAttentionArgs;
+
 /* Keys per tile of the attention kernels.  Together with SharedKVArgs.splits
  * it fixes the numerics: tile k of a query (kinds in order: original window,
  * then compressed rows) is folded into partition k % splits. */
@@ -237,6 +298,14 @@ int launch_cache_write(uint32_t blocks, void *stream, const CacheWriteArgs *args
 int launch_sharedkv_tree(void *stream, const TreeAttentionArgs *args);
 int sharedkv_tree_scratch(const TreeAttentionArgs *args, uint64_t *workspace, uint64_t *partial);
 
+/* Rows appended to 8-bit caches (CacheAppendArgs); attention over caches with
+ * block scales (BlockAttentionArgs), one launch or, where long contexts are
+ * split, two, and the bytes of its scratch (0: none needed), a host-only query
+ * that reads everything but the partial and units fields. */
+int launch_sharedkv_append(void *stream, const CacheAppendArgs *args);
+int launch_sharedkv_block(void *stream, const BlockAttentionArgs *args);
+int sharedkv_block_scratch(const BlockAttentionArgs *args, uint64_t *partial, uint64_t *units);
+
 /* Accepted paths, and pages of a pool (argument blocks above).  pageBytes is
  * the sum of the caches' bytes and rowBytes the largest row's.  All take up to
  * 2^24 - 1 work-groups of 256 threads (a fork one for every 64 KiB of every
@@ -312,14 +381,16 @@ int sharedkv_c8_set_xcd_local(int enable);
  * (probe failed), -1 not probed yet. */
 int sharedkv_c8_xcd_local(void);
 
-/* sizeof the argument blocks of trees and pages. */
+/* sizeof the argument blocks of trees, block-scaled caches and pages. */
+uint32_t sharedkv_append_args_size(void);
+uint32_t sharedkv_block_args_size(void);
 uint32_t sharedkv_tree_args_size(void);
 uint32_t sharedkv_path_commit_args_size(void);
 uint32_t sharedkv_page_fork_args_size(void);
 uint32_t sharedkv_page_compact_args_size(void);
 
-/* sizeof(SharedKVArgs), sizeof(CacheWriteArgs), library ABI version (4 since
- * TreeAttentionArgs.causalCompressed). */
+/* sizeof(SharedKVArgs), sizeof(CacheWriteArgs), library ABI version (5 since
+ * CacheAppendArgs and BlockAttentionArgs). */
 uint32_t sharedkv_attention_args_size(void);
 uint32_t sharedkv_cache_args_size(void);
 uint32_t sharedkv_abi_version(void);
