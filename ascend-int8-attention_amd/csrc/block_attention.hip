@@ -410,9 +410,9 @@ __global__ void __launch_bounds__(THREADS, 2) block_attention(const uint64_t cu_
     int entries = -1;                                  // page of half (lane & 1) of tile 32 block + lane / 2
     float scales = 1.0f;                               // and its scale
     auto read_entries = [&](int block) {
-        const int k = 32 * block + (lane >> 1);
+        const int lx = again(tid) & 63, k = 32 * block + (lx >> 1);
         const bool ori = k >= cmp_tiles;
-        const int e = base_of(k) / PAGE_ROWS + (lane & 1), width = (int)(ori ? p.oriTableWidth : p.cmpTableWidth);
+        const int e = base_of(k) / PAGE_ROWS + (lx & 1), width = (int)(ori ? p.oriTableWidth : p.cmpTableWidth);
         entries = k < k1 && e < width ? gptr<int32_t>(ori ? p.oriTable : p.cmpTable)[(int64_t)b * width + e] : -1;
         scales = 1.0f;
         if ((uint32_t)entries < (ori ? p.oriPages : p.cmpPages))
@@ -428,7 +428,7 @@ __global__ void __launch_bounds__(THREADS, 2) block_attention(const uint64_t cu_
         const bool ori = k >= cmp_tiles;
         const uint64_t pool = (ori ? p.ori : p.cmp) + (uint64_t)kv_head * D, stride = ori ? p.oriStride : p.cmpStride;
         const uint32_t pages = ori ? p.oriPages : p.cmpPages;
-        const int lx = again(lane);
+        const int lx = again(tid) & 63;
         const uint32_t lane_offset =
             (uint32_t)(4 * wave + (lx >> 5)) * row_bytes + (uint32_t)(((lx & 31) ^ (4 * wave + (lx >> 5))) << 4);
         const uint32_t to = (uint32_t)(uintptr_t)s.tile[k & 1] + 4 * wave * D;
@@ -544,56 +544,45 @@ __global__ void __launch_bounds__(THREADS, 2) block_attention(const uint64_t cu_
 #pragma nounroll
     for (int k = k0; k < k1; ++k) {
         seen = next_seen;
-        // The tile's two scales: of a score, of a weight, and its inverse (below LEAST a scale is 0 to any sum it is in).
-        float step[2], lift[2], drop[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const float its = __uint_as_float((uint32_t)__builtin_amdgcn_readlane(__float_as_int(scales), 2 * (k & 31) + h));
-            step[h] = its;
-            lift[h] = __builtin_amdgcn_logf(its < LEAST ? LEAST : its);
-            drop[h] = __builtin_amdgcn_exp2f(-lift[h]);
-        }
+        const int scale0 = __builtin_amdgcn_readlane(__float_as_int(scales), 2 * (k & 31));
+        const int scale1 = __builtin_amdgcn_readlane(__float_as_int(scales), 2 * (k & 31) + 1);
         vm_wait_all();
         lds_barrier();                                 // tile k is there; nobody uses tile k - 1 or its weights any more
         if (k + 1 < k1) {
             if (!((k + 1) & 31)) read_entries((k + 1) >> 5);
             next_seen = copy_tile(k + 1);
         }
-        const int lx = again(lane), its_row = 16 * (wave % RT) + (lx & 15);
+        const int lx = again(tid) & 63, its_row = 16 * (wave % RT) + (lx & 15);
         const uint32_t tile = (uint32_t)(uintptr_t)s.tile[k & 1];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) step[h] = __builtin_elementwise_maximum(q.step * step[h], 0x1p-126f);   // keeps a NaN
 
         // S = Q K^T: query row n, keys key0 + 16 kt + 4 g + i.
         float w[RT][4];
         {
             const uint32_t at = tile + (uint32_t)((key0 + (lx & 15)) * D + (((lx >> 4) ^ (lx & 15)) << 4));
             if constexpr (E4M3) {
-                // Step st: keys of tile st / 8, channels 64 (st % 8) on; reads run two steps ahead, conversions one.
+                // Step st: keys of tile st / 8, channels 64 (st % 8) on; reads run two steps ahead, conversions half a one.
                 constexpr int STEPS = 8 * RT, AHEAD = 3;
                 v4i key[AHEAD];
-                bf16x8 value[2][2];
+                bf16x8 value[2];
                 auto fetch = [&](int st) {
                     key[st % AHEAD] = *(const lds_v4i *)(uintptr_t)((at ^ (uint32_t)(64 * (st & 7))) + (uint32_t)(16 * (st >> 3) * D));
                 };
-                auto convert = [&](int st) {
-                    const v4i w = key[st % AHEAD];
-                    value[st & 1][0] = to_bf16(w[0], w[1]), value[st & 1][1] = to_bf16(w[2], w[3]);
-                };
                 fetch(0);
                 fetch(1);
-                convert(0);
+                value[0] = to_bf16(key[0][0], key[0][1]);
                 f32x4 dots[2];
                 __builtin_amdgcn_s_setprio(1);
 #pragma unroll
                 for (int st = 0; st < STEPS; ++st) {
                     if (st + 2 < STEPS) fetch(st + 2);
-                    if (st + 1 < STEPS) convert(st + 1);
                     const int j = st & 7;
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
-                        dots[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(value[st & 1][h], __builtin_bit_cast(bf16x8, q.term[h][j]),
+                    for (int h = 0; h < 2; ++h) {
+                        if (h == 0) value[1] = to_bf16(key[st % AHEAD][2], key[st % AHEAD][3]);
+                        if (h == 1 && st + 1 < STEPS) value[0] = to_bf16(key[(st + 1) % AHEAD][0], key[(st + 1) % AHEAD][1]);
+                        dots[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(value[h], __builtin_bit_cast(bf16x8, q.term[h][j]),
                                                                           j ? dots[h] : f32x4{0, 0, 0, 0}, 0, 0, 0);
+                    }
                     if (j == 7)
 #pragma unroll
                         for (int i = 0; i < 4; ++i) w[st >> 3][i] = dots[0][i] + dots[1][i];
@@ -650,19 +639,22 @@ __global__ void __launch_bounds__(THREADS, 2) block_attention(const uint64_t cu_
                 for (int i = 0; i < 4; ++i) w[kt][i] = its >> i & 1 ? w[kt][i] : -INFINITY;
             }
         }
-        // Those of the wave's key tiles: page halves are 32 keys.
-        float its_step[RT], its_lift[RT], its_drop[RT];
+        // Of the pages that the wave's keys are on (one, or for units of 64 rows both): a unit's score, log2 of the scale that
+        // weighs values, and its inverse.
+        constexpr int PAGES = RT == 4 ? 2 : 1;
+        float step[PAGES], lift[PAGES], drop[PAGES];
 #pragma unroll
-        for (int kt = 0; kt < RT; ++kt) {
-            its_step[kt] = RT == 4 ? step[kt >> 1] : wave >> 1 ? step[1] : step[0];
-            its_lift[kt] = RT == 4 ? lift[kt >> 1] : wave >> 1 ? lift[1] : lift[0];
-            its_drop[kt] = RT == 4 ? drop[kt >> 1] : wave >> 1 ? drop[1] : drop[0];
+        for (int h = 0; h < PAGES; ++h) {
+            const float its = __int_as_float((PAGES == 2 ? h : wave >> 1) ? scale1 : scale0);
+            step[h] = __builtin_elementwise_maximum(q.step * its, 0x1p-126f);   // never 0: masked keys score -infinity; keeps a NaN
+            lift[h] = __builtin_amdgcn_logf(its < LEAST ? LEAST : its);
+            drop[h] = __builtin_amdgcn_exp2f(-lift[h]);
         }
         float peak = -INFINITY;                        // of score + lift
 #pragma unroll
         for (int kt = 0; kt < RT; ++kt) {
             float most = fmaxf(fmaxf(w[kt][0], w[kt][1]), fmaxf(w[kt][2], w[kt][3]));
-            peak = fmaxf(peak, __builtin_fmaf(most, its_step[kt], its_lift[kt]));
+            peak = fmaxf(peak, __builtin_fmaf(most, step[PAGES == 2 ? kt >> 1 : 0], lift[PAGES == 2 ? kt >> 1 : 0]));
         }
         peak = row_max(peak);
         if (PARTS > 1) {                               // the row's keys are spread over waves
@@ -689,16 +681,17 @@ __global__ void __launch_bounds__(THREADS, 2) block_attention(const uint64_t cu_
 #pragma unroll
             for (int kt = 0; kt < RT; ++kt) {
                 f16x4 half;
-                const float less = its_lift[kt] - from;
+                const int h = PAGES == 2 ? kt >> 1 : 0;
+                const float less = lift[h] - from;
                 float together = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    float x = __builtin_amdgcn_exp2f(__builtin_fmaf(w[kt][i], its_step[kt], less));
+                    float x = __builtin_amdgcn_exp2f(__builtin_fmaf(w[kt][i], step[h], less));
                     if (edge) x = w[kt][i] == -INFINITY ? 0.0f : x;   // whatever the page's scale is
                     together += x;
                     half[i] = (_Float16)x;
                 }
-                if (!edge || together != 0.0f) sum = __builtin_fmaf(together, its_drop[kt], sum);
+                if (!edge || together != 0.0f) sum = __builtin_fmaf(together, drop[h], sum);
                 *reinterpret_cast<f16x4 *>(s.p + its_row * P_STRIDE + key0 + 16 * kt + 4 * (lx >> 4)) = half;
             }
         }
@@ -706,7 +699,7 @@ __global__ void __launch_bounds__(THREADS, 2) block_attention(const uint64_t cu_
             // A code that is no number may lie in a row that some token does not see, and 0 times it is none either.
             // Rows that see it have weights that are no numbers already.
             lds_barrier();                             // all scores are made
-            for (int i = tid; i < KEYS * D / 16; i += THREADS) {
+            for (int i = again(tid); i < KEYS * D / 16; i += THREADS) {
                 u32x4 v = reinterpret_cast<u32x4 *>(s.tile[k & 1])[i];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) v[e] &= ~((((v[e] & 0x7f7f7f7fu) + 0x01010101u) >> 7 & 0x01010101u) * 255u);
@@ -717,7 +710,7 @@ __global__ void __launch_bounds__(THREADS, 2) block_attention(const uint64_t cu_
 
         // acc[ct][rt]: channels 128 wave + 16 ct + 4 g + i, row 16 rt + n.
         {
-            const int lx = again(lane);
+            const int lx = again(tid) & 63;
             const int slot = 8 * (lx >> 4) + ((lx & 15) >> 1);
             const uint32_t from = tile + (uint32_t)(slot * D + 8 * (lx & 1) + (((8 * wave) ^ (slot & 15)) << 4));
             const _Float16 *its = s.p + (lx & 15) * P_STRIDE + 8 * (lx >> 4);
@@ -771,9 +764,10 @@ __global__ void __launch_bounds__(THREADS, 2) block_attention(const uint64_t cu_
     }
     sum += __shfl_xor(sum, 16);
     sum += __shfl_xor(sum, 32);
-    if (g == 0) {
-        s.sum[wave / RT][row] = sum;
-        if (wave < RT) s.top[row] = m;
+    const int last = again(tid), lx = last & 63, gx = lx >> 4, nx = lx & 15;
+    if (gx == 0) {
+        s.sum[wave / RT][16 * (wave % RT) + nx] = sum;
+        if (wave < RT) s.top[16 * (wave % RT) + nx] = m;
     }
     lds_barrier();
     auto row_sum = [&](int at) {
@@ -788,27 +782,27 @@ __global__ void __launch_bounds__(THREADS, 2) block_attention(const uint64_t cu_
         for (int ct = 0; ct < 8; ++ct)
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt)
-                if (16 * rt + n < rows)
-                    *gout<f32x4>(state + ((16 * rt + n) * D + 128 * wave + 16 * ct + 4 * g) * 4) = acc[ct][rt];
-        if (tid < rows) {
-            gout<float>(state)[ROWS * D + tid] = s.top[tid];
-            gout<float>(state)[ROWS * (D + 1) + tid] = row_sum(tid);
+                if (16 * rt + nx < rows)
+                    *gout<f32x4>(state + ((16 * rt + nx) * D + 128 * wave + 16 * ct + 4 * gx) * 4) = acc[ct][rt];
+        if (last < rows) {
+            gout<float>(state)[ROWS * D + last] = s.top[last];
+            gout<float>(state)[ROWS * (D + 1) + last] = row_sum(last);
         }
         return;
     }
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-        const int at = 16 * rt + n;
+        const int at = 16 * rt + nx;
         if (at >= rows) continue;
         const uint32_t place = (uint32_t)s.place[at];
         const Final f(s.top[at], row_sum(at), gptr<float>(p.sinks)[place % (uint32_t)heads] * LOG2E);
 #pragma unroll
         for (int ct = 0; ct < 8; ++ct) {
             const f32x4 v = acc[ct][rt] * f.give;
-            *gout<u32x2>(p.out + (uint64_t)place * (D * 2) + (128 * wave + 16 * ct + 4 * g) * 2) =
+            *gout<u32x2>(p.out + (uint64_t)place * (D * 2) + (128 * wave + 16 * ct + 4 * gx) * 2) =
                 u32x2{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
         }
-        if (p.lse && wave == 0 && g == 0) gout<float>(p.lse)[place] = f.lse2 * LN2;
+        if (p.lse && wave == 0 && gx == 0) gout<float>(p.lse)[place] = f.lse2 * LN2;
     }
 }
 
