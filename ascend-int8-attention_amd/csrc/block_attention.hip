@@ -50,7 +50,8 @@ constexpr int WHOLE = 0x3fffffff;  // tiles of an item where units are not split
 constexpr uint32_t MAX_HEADS = 128;
 constexpr uint32_t MAX_WIDTH = (0x7fffffffu - KEYS) / PAGE_ROWS;
 constexpr uint32_t MAX_GROUPS = 0xffffffffu / THREADS;   // the threads of a launch are counted in 32 bits
-constexpr uint32_t ITEMS = 512;    // of a split launch: two work-groups on each of 256 CUs
+constexpr uint32_t SLOTS = 512;    // work-groups that run at once: two on each of 256 CUs
+constexpr uint32_t MAX_SPLIT_UNITS = SLOTS * 3 / 4;       // launches of more units fill the slots as they are
 // Tiles of a launch's units together, up to which a launch is split: they are summed over 64 lanes in 32 bits.
 constexpr uint64_t MAX_SPLIT_WORK = 0x1ffffff;
 constexpr float LOG2E = 1.44269504088896341f, LN2 = 0.69314718055994531f;
@@ -108,8 +109,21 @@ __device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w 
 
 // The launch's sizes.
 struct Sizes {
-    uint32_t tokens, ratio, window, oriTableWidth, cmpTableWidth, group, kvHeads;
+    uint32_t tokens, ratioBits, window, oriTableWidth, cmpTableWidth, group, kvHeads;
+    uint32_t groupInverse, groupBits;  // n / group is n * groupInverse >> groupBits for n below 2^31
 };
+__device__ __forceinline__ int by_group(const Sizes &p, int n) { return (int)((uint64_t)(uint32_t)n * p.groupInverse >> p.groupBits); }
+
+// a / b, rounded down, for a from 0 and b from 1 on, with `inverse` about 1 / b: a step by the remainder for what FP32
+// cannot hold, and one for its rounding.  (Divisions are most of the plan's instructions, and this one is half of a
+// 32-bit division's.)
+__device__ __forceinline__ int quotient(int a, int b, float inverse)
+{
+    int q = (int)((float)a * inverse), r = a - q * b;
+    const int more = (int)((float)r * inverse);
+    q += more, r -= more * b;
+    return q + (r >= b) - (r < 0);
+}
 
 // A split unit as the join finds it: its parts' states are those of items first, first + stride, ...
 struct Unit {
@@ -122,12 +136,13 @@ struct Unit {
 struct Request {
     int32_t first, count, length;      // first token, tokens, all rows
     int32_t per_head, units, tiles;    // units of a KV head, of all; tiles of a unit, at most
+    int32_t work;                      // tiles of all units, about
 };
 
 __device__ __forceinline__ int compressed_at(const Sizes &p, int position)
 {
     const int64_t rows = (int64_t)p.cmpTableWidth * PAGE_ROWS;
-    return p.ratio > 1 ? (int)min((int64_t)((uint32_t)max(position + 1, 0) / p.ratio), rows) : 0;
+    return p.ratioBits ? (int)min((int64_t)((uint32_t)max(position + 1, 0) >> p.ratioBits), rows) : 0;
 }
 
 template <int ROWS>
@@ -140,11 +155,15 @@ __device__ __forceinline__ Request request_of(const Sizes &p, int c0, int c1, in
     r.length = length;
     r.per_head = (int)((r.count * (int64_t)p.group + ROWS - 1) / ROWS);
     r.units = r.per_head * (int)p.kvHeads;
-    r.tiles = 0;
+    r.tiles = r.work = 0;
     if (length > 0 && r.count > 0) {
-        const int64_t near = (int64_t)p.window + (ROWS - 1) / p.group + 1 + PAGE_ROWS;
+        const int64_t near = (int64_t)p.window + by_group(p, ROWS - 1) + 1 + PAGE_ROWS;
         const int64_t rows = min(min((int64_t)length, (int64_t)p.oriTableWidth * PAGE_ROWS), near);
-        r.tiles = (compressed_at(p, length - 1) + KEYS - 1) / KEYS + (int)((rows + KEYS - 1) / KEYS);
+        const int compressed = compressed_at(p, length - 1);
+        r.tiles = (compressed + KEYS - 1) / KEYS + (int)((rows + KEYS - 1) / KEYS);
+        // The first unit lacks the rows behind its tokens: half of that on average.
+        const int less = (int)min(rows, max((int64_t)0, (int64_t)r.count - (length - rows))) + (compressed - compressed_at(p, length - r.count));
+        r.work = (int)min((int64_t)r.units * max(1, r.tiles - less / (2 * KEYS)), (int64_t)MAX_SPLIT_WORK);
     }
     return r;
 }
@@ -274,10 +293,11 @@ struct alignas(1024) Shared {
 
 template <bool E4M3, int RT>
 __global__ void __launch_bounds__(THREADS, 2) block_attention(const uint64_t cu_q, const uint64_t seq_lens, const uint32_t batch_arg, const uint32_t split,
-                const uint32_t tokens_arg, const uint32_t ratio, const uint32_t window_rows, const uint32_t ori_width,
-                const uint32_t cmp_width, const uint32_t group_arg, const uint32_t kv_heads, const BlockAttentionArgs p)
+                const uint32_t tokens_arg, const uint32_t ratio_bits, const uint32_t window_rows, const uint32_t ori_width,
+                const uint32_t cmp_width, const uint32_t group_arg, const uint32_t kv_heads, const uint32_t group_inverse,
+                const uint32_t group_bits, const BlockAttentionArgs p)
 {
-    const Sizes size = {tokens_arg, ratio, window_rows, ori_width, cmp_width, group_arg, kv_heads};
+    const Sizes size = {tokens_arg, ratio_bits, window_rows, ori_width, cmp_width, group_arg, kv_heads, group_inverse, group_bits};
     using S = Shared<RT>;
     constexpr int ROWS = S::ROWS, PARTS = S::PARTS;
     __shared__ S s;
@@ -287,44 +307,76 @@ __global__ void __launch_bounds__(THREADS, 2) block_attention(const uint64_t cu_
     const auto *cu = gptr<int32_t>(cu_q), *lens = gptr<int32_t>(seq_lens);
 
     // ---- plan: units and tiles of the live requests, tiles of an item, this work-group's item ----
+    const bool one_step = batch <= THREADS, one_wave = batch <= 64;
     Request mine = {};
     int units = 0, work = 0;                           // units, times their tiles
-    for (int b = tid; b < batch; b += THREADS) {
+    for (int b = one_wave ? lane : tid; b < batch; b += THREADS) {
         mine = request_of<ROWS>(size, cu[b], cu[b + 1], lens[b]);
         units += mine.units;
-        work = (int)min((int64_t)mine.units * mine.tiles + work, (int64_t)MAX_SPLIT_WORK);
+        work = min(mine.work + work, (int)MAX_SPLIT_WORK);
     }
     const int end = min(max(cu[batch], 0), (int)size.tokens) * heads;
     const int all_rows = (int)size.tokens * heads, pad_units = (all_rows - end + ROWS - 1) / ROWS;
-    units = wave_sum(units), work = wave_sum(work);
-    if (lane == 0) s.scan[0][wave] = units, s.scan[1][wave] = work;
-    if (tid == 0) s.found[0] = -1;
-    __syncthreads();
-    units = 0;
-    int64_t all_work = 0;
+    units = wave_sum(units);
+    uint32_t all_work = (uint32_t)wave_sum(work);      // of launches that may be split at most MAX_SPLIT_WORK
+    if (!one_wave) {
+        if (lane == 0) s.scan[0][wave] = units, s.scan[1][wave] = (int)all_work;
+        if (tid == 0) s.found[0] = -1;
+        __syncthreads();
+        units = 0, all_work = 0;
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) units += s.scan[0][w], all_work += s.scan[1][w];
-    // Tiles of an item: as many as leave no more than ITEMS items (a unit's last may be short).  `split` is the number of
-    // units that the launch has scratch for: requests that lie one behind the other are never more, and others are not
-    // split.
+        for (int w = 0; w < WAVES; ++w) units += s.scan[0][w], all_work += (uint32_t)s.scan[1][w];
+    }
+    // Tiles of an item: the fewest of four that leave no more than SLOTS items, the last of which always does (a unit's
+    // last item may be short).  `split` is the number of units that the launch has scratch for: requests that lie one
+    // behind the other are never more, and others are not split.
     int per_item = WHOLE;
     if (units + pad_units <= (int)split) {
-        const int64_t room = (int64_t)ITEMS - units - pad_units;
-        per_item = (int)min((int64_t)WHOLE - 1, max((int64_t)1, (all_work + room - 1) / room));
+        const int whole = units + pad_units;
+        int tries[4], items[3] = {};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int room = (int)SLOTS - whole * i / 3;
+            tries[i] = max(1, quotient((int)all_work + room - 1, room, __builtin_amdgcn_rcpf((float)room)));
+        }
+        per_item = tries[3];
+        if (one_wave) {
+#pragma unroll
+            for (int i = 0; i < 3; ++i)
+                items[i] = wave_sum(mine.units * max(1, quotient(mine.tiles + tries[i] - 1, tries[i], __builtin_amdgcn_rcpf((float)tries[i]))));
+#pragma unroll
+            for (int i = 2; i >= 0; --i) per_item = items[i] + pad_units <= (int)SLOTS ? tries[i] : per_item;
+        }
     }
     per_item = uni(per_item), units = uni(units);
     const bool may_split = per_item != WHOLE;
     if (split && blockIdx.x == 0 && tid == 0) *gout<int32_t>(p.units) = may_split ? units : 0;
-    auto parts_of = [&](int tiles) { return max(1, (tiles + per_item - 1) / per_item); };
+    const float item_inverse = __builtin_amdgcn_rcpf((float)per_item);
+    auto parts_of = [&](int tiles) { return max(1, quotient(tiles + per_item - 1, per_item, item_inverse)); };
     // Where units are split, the work-groups of one XCD (blockIdx modulo 8) take neighbouring items, which read the same
     // rows.
-    int item, items = 0, unit0 = 0, b = -1;
-    {
+    int item = 0, items = 0, unit0 = 0, b = -1, local = 0, first = 0, past = 0, length = 0;
+    auto take = [&](int number) {                      // the work-group's item of `number`; false: none
+        items = number;
+        const int share = (items + 7) / 8;
+        item = may_split ? (int)(blockIdx.x & 7) * share + (int)(blockIdx.x >> 3) : (int)blockIdx.x;
+        return item < items && !(may_split && (int)(blockIdx.x >> 3) >= share);
+    };
+    if (one_wave) {                                    // every wave for itself
+        const int n_items = mine.units * parts_of(mine.tiles), upto = wave_upto(n_items), at_units = wave_upto(mine.units);
+        if (!take(__builtin_amdgcn_readlane(upto, 63) + pad_units)) return;
+        const uint64_t its = __ballot(item < upto && item >= upto - n_items);
+        if (its) {
+            b = __builtin_ctzll(its);
+            local = item - __builtin_amdgcn_readlane(upto - n_items, b), unit0 = __builtin_amdgcn_readlane(at_units - mine.units, b);
+            first = __builtin_amdgcn_readlane(mine.first, b), past = first + __builtin_amdgcn_readlane(mine.count, b);
+            length = __builtin_amdgcn_readlane(mine.length, b);
+        }
+    } else {
         int upto = 0, at_units = 0;
         for (int pass = 0; pass < 2 && b < 0; ++pass) {
             // First the number of items (pass 0 ends there where one step holds all requests), then whose this one is.
             int before = 0, units_before = 0;
-            const bool one_step = batch <= THREADS;
             for (int at = 0; at < batch; at += THREADS) {
                 const int b0 = at + tid;
                 if (!one_step) mine = b0 < batch ? request_of<ROWS>(size, cu[b0], cu[b0 + 1], lens[b0]) : Request{};
@@ -343,11 +395,7 @@ __global__ void __launch_bounds__(THREADS, 2) block_attention(const uint64_t cu_
                 upto += before, at_units += units_before;
                 before += total, units_before += total_units;
                 if (one_step || pass) {
-                    if (one_step) items = before + pad_units;
-                    const int share = (items + 7) / 8;
-                    item = uni(may_split ? (int)(blockIdx.x & 7) * share + (int)(blockIdx.x >> 3) : (int)blockIdx.x);
-                    if (may_split && (int)(blockIdx.x >> 3) >= share) return;
-                    if (item >= items) return;
+                    if (!take(one_step ? before + pad_units : items)) return;
                     if (item < upto && item >= upto - n_items) {
                         s.found[0] = b0, s.found[1] = item - (upto - n_items), s.found[2] = at_units - u;
                         s.found[3] = mine.first, s.found[4] = mine.first + mine.count, s.found[5] = mine.length;
@@ -359,7 +407,9 @@ __global__ void __launch_bounds__(THREADS, 2) block_attention(const uint64_t cu_
         }
         __syncthreads();
         b = s.found[0];
+        if (b >= 0) local = s.found[1], unit0 = s.found[2], first = s.found[3], past = s.found[4], length = s.found[5];
     }
+    item = uni(item), items = uni(items);
     auto zero_row = [&](int64_t place) {               // by one wave
         *gout<u32x4>(p.out + (uint64_t)place * (D * 2) + lane * 16) = u32x4{0, 0, 0, 0};
         if (p.lse && lane == 0) gout<float>(p.lse)[place] = 0.0f;
@@ -370,16 +420,16 @@ __global__ void __launch_bounds__(THREADS, 2) block_attention(const uint64_t cu_
             if (first + i < all_rows) zero_row(first + i);
         return;
     }
-    b = uni(b);
-    const Request r = request_of<ROWS>(size, uni(s.found[3]), uni(s.found[4]), uni(s.found[5]));
-    const int slots = uni(parts_of(r.tiles)), local = uni(s.found[1]);
+    b = uni(b), local = uni(local), unit0 = uni(unit0);
+    const Request r = request_of<ROWS>(size, uni(first), uni(past), uni(length));
+    const int slots = uni(parts_of(r.tiles));
     // Items of a request: by KV head, part, unit.  Whole units go from the last, which see most.
-    const int kv_head = uni(local / (slots * r.per_head)), part = uni(local / r.per_head % slots);
-    const int in_head = uni(slots == 1 ? r.per_head - 1 - local % r.per_head : local % r.per_head);
-    unit0 = uni(s.found[2]);
+    const int of_parts = uni(quotient(local, r.per_head, __builtin_amdgcn_rcpf((float)r.per_head)));
+    const int kv_head = uni(quotient(of_parts, slots, __builtin_amdgcn_rcpf((float)slots))), part = of_parts - kv_head * slots;
+    const int from_first = local - of_parts * r.per_head, in_head = slots == 1 ? r.per_head - 1 - from_first : from_first;
     const int row0 = in_head * ROWS;                   // of the request and KV head
     const int rows = min((int64_t)ROWS, r.count * (int64_t)group - row0);
-    const int t0 = uni(row0 / group), t1 = uni((row0 + rows - 1) / group);
+    const int t0 = by_group(size, row0), t1 = by_group(size, row0 + rows - 1);
     // ---- the unit's tiles: compressed rows, then original ones, upwards ----
     const int start = r.length - r.count, at0 = start + t0, at1 = start + t1;     // positions
     const int window = (int)min(size.window, 0x7fffffffu);
@@ -394,9 +444,11 @@ __global__ void __launch_bounds__(THREADS, 2) block_attention(const uint64_t cu_
         to[0] = u.first, to[1] = u.stride, to[2] = u.parts, to[3] = u.rows, to[4] = u.token, to[5] = u.row0, to[6] = u.head0;
     }
     if (part >= parts) return;
-    const int k0 = uni((int)((int64_t)tiles * part / parts)), k1 = uni((int)((int64_t)tiles * (part + 1) / parts));
+    const int share = parts == 1 ? tiles : uni(quotient(tiles, parts, __builtin_amdgcn_rcpf((float)parts)));
+    const int more = tiles - share * parts;            // equal shares, the first ones a tile more
+    const int k0 = part * share + min(part, more), k1 = k0 + share + (part < more);
     if (tid < ROWS) {
-        const int at = row0 + min(tid, rows - 1), token = at / group;
+        const int at = row0 + min(tid, rows - 1), token = by_group(size, at);
         s.token[tid] = token;
         s.place[tid] = (r.first + token) * heads + kv_head * group + (at - token * group);
     }
@@ -471,7 +523,6 @@ __global__ void __launch_bounds__(THREADS, 2) block_attention(const uint64_t cu_
         // The copies come last: a wait for an earlier load does not wait for them.
 #pragma unroll
         for (int j = 0; j < JN; ++j) asm volatile("" : "+v"(raw[j][0]), "+v"(raw[j][1]));
-        asm volatile("" : "+v"(scales));
         next_seen = copy_tile(k0);
         if constexpr (E4M3) {
             const uint32_t flip = softmax2 < 0.0f ? 0x80008000u : 0u;
@@ -806,66 +857,84 @@ __global__ void __launch_bounds__(THREADS, 2) block_attention(const uint64_t cu_
     }
 }
 
-// Joins the states of a split unit's items, in the parts' order: a row and 128 of its channels.
-constexpr int JOINERS = THREADS / 32;                  // parts read at once
+// Joins the states of a split unit's items, in the parts' order: a row, all channels of it where there are few parts and
+// 128 where there are many.  What bounds it is the chain of its reads (the unit; all maxima, sums and the first
+// numerators), so each is started as soon as it can be.
+constexpr int AT_ONCE = 4;                             // parts that a thread reads at once
 
+template <int CHANNELS>
 __global__ void __launch_bounds__(THREADS) block_join(const uint64_t partial, const uint64_t units, const uint32_t rt, const uint32_t group,
                                                       const uint32_t heads, const BlockAttentionArgs p)
 {
-    __shared__ float factor[ITEMS];
+    constexpr int LANES = CHANNELS / 4, JOINERS = THREADS / LANES;        // of a part; parts read side by side
+    __shared__ float factor[SLOTS];
     __shared__ float most_of[THREADS / 64], sum_of[THREADS / 64];
-    __shared__ f32x4 sums[JOINERS][32];
+    __shared__ f32x4 sums[JOINERS][LANES];
     const uint32_t rows = 16 * rt;
     const int unit = (int)(blockIdx.x / rows), row = (int)(blockIdx.x % rows), tid = threadIdx.x;
-    if (unit >= *gptr<int32_t>(units)) return;
     const auto *u = gptr<int32_t>(units + sizeof(Unit) * (uint64_t)(1 + unit));
-    const int first = u[0], stride = u[1], parts = u[2];
-    if (parts < 2 || row >= u[3]) return;
+    const int number = *gptr<int32_t>(units), first = u[0], stride = u[1], parts = min(u[2], (int)SLOTS), its_rows = u[3];
+    const int token0 = u[4], row0 = u[5], head0 = u[6];
+    if (unit >= number || parts < 2 || row >= its_rows) return;
     const uint64_t size = 16ull * rt * (D + 2);
     auto state = [&](int part) { return gptr<float>(partial) + (uint64_t)(first + part * stride) * size; };
-    // The parts' factors.
-    float m[ITEMS / THREADS], l[ITEMS / THREADS], most = -INFINITY, total = 0.0f;
+    const int channel = CHANNELS * (int)blockIdx.y + 4 * (tid % LANES), joiner = tid / LANES;
+    auto numerators = [&](int part) {
+        return *reinterpret_cast<const __attribute__((address_space(1))) f32x4 *>(state(part) + row * D + channel);
+    };
+    constexpr int EACH = SLOTS / THREADS;
+    float m[EACH], l[EACH], most = -INFINITY, total = 0.0f;
 #pragma unroll
-    for (int i = 0; i < (int)(ITEMS / THREADS); ++i) {
+    for (int i = 0; i < EACH; ++i) {
         const int part = tid + i * THREADS;
         m[i] = -INFINITY, l[i] = 0.0f;
         if (part < parts) m[i] = state(part)[rows * D + row], l[i] = state(part)[rows * (D + 1) + row];
-        most = fmaxf(most, m[i]);
     }
+    f32x4 v[AT_ONCE];
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i) v[i] = numerators(min(joiner + i * JOINERS, parts - 1));
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) most = fmaxf(most, m[i]);
 #pragma unroll
     for (int step = 1; step < 64; step *= 2) most = fmaxf(most, __shfl_xor(most, step));
     if ((tid & 63) == 0) most_of[tid >> 6] = most;
-    __syncthreads();
+    lds_barrier();
 #pragma unroll
     for (int w = 0; w < THREADS / 64; ++w) most = fmaxf(most, most_of[w]);
     const float from = most == -INFINITY ? 0.0f : most;
 #pragma unroll
-    for (int i = 0; i < (int)(ITEMS / THREADS); ++i) {
+    for (int i = 0; i < EACH; ++i) {
         const int part = tid + i * THREADS;
-        if (part >= parts) continue;
         const float f = __builtin_amdgcn_exp2f(m[i] - from);
-        factor[part] = f;
+        factor[part] = f;                              // 0 past the parts
         total += l[i] * f;
     }
 #pragma unroll
     for (int step = 1; step < 64; step *= 2) total += __shfl_xor(total, step);
     if ((tid & 63) == 0) sum_of[tid >> 6] = total;
-    __syncthreads();
+    lds_barrier();
     total = 0.0f;
 #pragma unroll
     for (int w = 0; w < THREADS / 64; ++w) total += sum_of[w];
-    const int channel = 128 * (int)blockIdx.y + 4 * (tid & 31), joiner = tid >> 5;
     f32x4 sum = {};
-#pragma unroll 4
-    for (int part = joiner; part < parts; part += JOINERS)
-        sum += *reinterpret_cast<const __attribute__((address_space(1))) f32x4 *>(state(part) + row * D + channel) * factor[part];
-    sums[joiner][tid & 31] = sum;
-    __syncthreads();
+#pragma nounroll
+    for (int part = joiner; part < parts; part += AT_ONCE * JOINERS) {
+        f32x4 next[AT_ONCE];
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) next[i] = numerators(min(part + (AT_ONCE + i) * JOINERS, parts - 1));
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i)
+            if (part + i * JOINERS < parts) sum += v[i] * factor[part + i * JOINERS];
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) v[i] = next[i];
+    }
+    sums[joiner][tid % LANES] = sum;
+    lds_barrier();
     if (joiner) return;
 #pragma unroll
     for (int i = 1; i < JOINERS; ++i) sum += sums[i][tid];
-    const int at = u[5] + row, token = at / (int)group;
-    const uint32_t place = (uint32_t)((u[4] + token) * (int)heads + u[6] + at - token * (int)group);
+    const int at = row0 + row, token = at / (int)group;
+    const uint32_t place = (uint32_t)((token0 + token) * (int)heads + head0 + at - token * (int)group);
     const Final f(most, total, gptr<float>(p.sinks)[place % heads] * LOG2E);
     sum *= f.give;
     *gout<u32x2>(p.out + (uint64_t)place * (D * 2) + channel * 2) = u32x2{pack_bf16(sum[0], sum[1]), pack_bf16(sum[2], sum[3])};
@@ -877,7 +946,7 @@ bool rejected(const BlockAttentionArgs *a)
     if (!a || !a->heads || a->heads > MAX_HEADS || !a->kvHeads || a->heads % a->kvHeads || !a->batch || !a->window || !a->ratio)
         return true;
     if (!a->q || !a->ori || !a->oriScale || !a->oriTable || !a->cuQ || !a->seqLens || !a->sinks || !a->out) return true;
-    if (a->ratio > 0x7fffffffu || a->codes > 1) return true;
+    if (a->ratio > 0x40000000u || (a->ratio & (a->ratio - 1)) || a->codes > 1) return true;
     const uint64_t page = (uint64_t)PAGE_ROWS * D * a->kvHeads;
     if (!a->oriPages || !a->oriTableWidth || (a->oriStride & 15) || a->oriStride < page) return true;
     if ((a->q | a->ori | a->out) & 15 || a->oriScale & 3) return true;
@@ -900,15 +969,18 @@ Plan plan_of(const BlockAttentionArgs *a)
     const uint64_t rows = (uint64_t)a->tokens * a->heads;
     const uint64_t each = rows / a->kvHeads / a->batch;         // rows of a request and KV head
     plan.rt = each <= 16 ? 1 : each <= 32 ? 2 : 4;
-    // The last unit of a request and KV head may be short, and so may the padding's.
-    const uint64_t units = rows / (16 * plan.rt) + (uint64_t)a->batch * a->kvHeads + 1;
+    // The last unit of a request and KV head may be short, and so may the padding's; a token's rows are in few units.
+    const uint64_t group = a->heads / a->kvHeads, unit = 16 * plan.rt;
+    const uint64_t short_last = rows / unit + (uint64_t)a->batch * a->kvHeads;
+    const uint64_t by_token = (uint64_t)a->tokens * a->kvHeads * ((group + unit - 1) / unit);
+    const uint64_t units = (short_last < by_token ? short_last : by_token) + 1;
     plan.units = units > MAX_GROUPS ? MAX_GROUPS + 1 : (uint32_t)units;
     const uint64_t near = (uint64_t)a->window + 2 * PAGE_ROWS + 64;
     const uint64_t tiles = (a->ratio > 1 ? (a->cmpTableWidth + 1) / 2 : 0) +
                            ((near / PAGE_ROWS < a->oriTableWidth ? near / PAGE_ROWS : a->oriTableWidth) + 1) / 2;
-    plan.split = plan.units <= ITEMS * 3 / 8 && tiles > 1;
+    plan.split = plan.units <= MAX_SPLIT_UNITS && tiles > 1 && plan.units * tiles <= MAX_SPLIT_WORK;
     const uint64_t items = plan.split ? plan.units * tiles : plan.units;
-    plan.grid = (uint32_t)((plan.split && items > ITEMS ? ITEMS : items) + 7) & ~7u;
+    plan.grid = (uint32_t)((plan.split && items > SLOTS ? SLOTS : items) + 7) & ~7u;
     return plan;
 }
 
@@ -930,12 +1002,18 @@ int launch_sharedkv_block(void *stream, const BlockAttentionArgs *a)
     };
     const auto kernel = a->codes ? of_rows(std::true_type{}) : of_rows(std::false_type{});
     const uint32_t group = a->heads / a->kvHeads;
+    uint32_t bits = 0;                                 // 2^31 * 2^bits / group, rounded up, is exact for 31 bits
+    while ((1u << bits) < group) ++bits;
+    const uint32_t inverse = (uint32_t)(((0x80000000ull << bits) + group - 1) / group);
     hipLaunchKernelGGL(kernel, dim3(plan.grid), dim3(THREADS), 0, static_cast<hipStream_t>(stream), a->cuQ, a->seqLens,
-                       a->batch, plan.split ? plan.units : 0u, a->tokens, a->ratio, a->window, a->oriTableWidth,
-                       a->ratio > 1 ? a->cmpTableWidth : 0u, group, a->kvHeads, *a);
-    if (plan.split)
-        hipLaunchKernelGGL(block_join, dim3(plan.units * 16 * plan.rt, D / 128), dim3(THREADS), 0,
-                           static_cast<hipStream_t>(stream), a->partial, a->units, (uint32_t)plan.rt, group, a->heads, *a);
+                       a->batch, plan.split ? plan.units : 0u, a->tokens, (uint32_t)__builtin_ctz(a->ratio), a->window,
+                       a->oriTableWidth, a->ratio > 1 ? a->cmpTableWidth : 0u, group, a->kvHeads, inverse, 31 + bits, *a);
+    if (plan.split) {
+        // Parts of a unit, at most, where all are alike.
+        const bool few = plan.grid / plan.units <= 16;
+        hipLaunchKernelGGL(few ? &block_join<512> : &block_join<128>, dim3(plan.units * 16 * plan.rt, few ? 1 : 4), dim3(THREADS),
+                           0, static_cast<hipStream_t>(stream), a->partial, a->units, (uint32_t)plan.rt, group, a->heads, *a);
+    }
     return (int)hipGetLastError();
 }
 

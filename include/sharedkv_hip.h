@@ -185,7 +185,7 @@ typedef struct CacheAppendArgs {
  * the query tokens cuQ[b] .. cuQ[b + 1] - 1 (T of them) and seqLens[b] rows; its
  * token i stands at position P = seqLens[b] - T + i and sees
  *   original rows j <= P with j > P - window,
- *   with ratio > 1 compressed rows r < (P + 1) / ratio.
+ *   with ratio > 1 (a power of two) compressed rows r < (P + 1) / ratio.
  * Query head h attends KV head h / (heads / kvHeads).  With v_j = code_j *
  * scale[page of j] and s_j = softmaxScale q v_j,
  *   out = sum_j e^{s_j} v_j / (e^{sink} + sum_j e^{s_j}), lse = log of the denominator.
