@@ -299,7 +299,7 @@ __global__ void __launch_bounds__(THREADS, 2) block_attention(const uint64_t cu_
 {
     const Sizes size = {tokens_arg, ratio_bits, window_rows, ori_width, cmp_width, group_arg, kv_heads, group_inverse, group_bits};
     using S = Shared<RT>;
-    constexpr int ROWS = S::ROWS, PARTS = S::PARTS;
+    constexpr int ROWS = S::ROWS, PARTS = S::PARTS, MIN_TILES = RT == 4 ? 8 : RT;
     __shared__ S s;
     const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6), g = lane >> 4, n = lane & 15;
     // The leading arguments are the ones that the first loads need: the build preloads them into SGPRs.
@@ -337,7 +337,7 @@ __global__ void __launch_bounds__(THREADS, 2) block_attention(const uint64_t cu_
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int room = (int)SLOTS - whole * i / 3;
-            tries[i] = max(1, quotient((int)all_work + room - 1, room, __builtin_amdgcn_rcpf((float)room)));
+            tries[i] = max(MIN_TILES, quotient((int)all_work + room - 1, room, __builtin_amdgcn_rcpf((float)room)));
         }
         per_item = tries[3];
         if (one_wave) {
@@ -967,17 +967,18 @@ Plan plan_of(const BlockAttentionArgs *a)
 {
     Plan plan;
     const uint64_t rows = (uint64_t)a->tokens * a->heads;
-    const uint64_t each = rows / a->kvHeads / a->batch;         // rows of a request and KV head
-    plan.rt = each <= 16 ? 1 : each <= 32 ? 2 : 4;
+    const uint64_t near = (uint64_t)a->window + 2 * PAGE_ROWS + 64;
+    const uint64_t tiles = (a->ratio > 1 ? (a->cmpTableWidth + 1) / 2 : 0) +
+                           ((near / PAGE_ROWS < a->oriTableWidth ? near / PAGE_ROWS : a->oriTableWidth) + 1) / 2;
+    const uint64_t each = (rows / a->kvHeads + a->batch - 1) / a->batch;        // rows of a request and KV head, on average
+    const uint64_t score = (rows + 63) / 64 * ((rows + 63) / 64) * tiles;
+    plan.rt = each <= 16 || score < 8000 ? 1 : each <= 32 || score < 400000 ? 2 : 4;
     // The last unit of a request and KV head may be short, and so may the padding's; a token's rows are in few units.
     const uint64_t group = a->heads / a->kvHeads, unit = 16 * plan.rt;
     const uint64_t short_last = rows / unit + (uint64_t)a->batch * a->kvHeads;
     const uint64_t by_token = (uint64_t)a->tokens * a->kvHeads * ((group + unit - 1) / unit);
     const uint64_t units = (short_last < by_token ? short_last : by_token) + 1;
     plan.units = units > MAX_GROUPS ? MAX_GROUPS + 1 : (uint32_t)units;
-    const uint64_t near = (uint64_t)a->window + 2 * PAGE_ROWS + 64;
-    const uint64_t tiles = (a->ratio > 1 ? (a->cmpTableWidth + 1) / 2 : 0) +
-                           ((near / PAGE_ROWS < a->oriTableWidth ? near / PAGE_ROWS : a->oriTableWidth) + 1) / 2;
     plan.split = plan.units <= MAX_SPLIT_UNITS && tiles > 1 && plan.units * tiles <= MAX_SPLIT_WORK;
     const uint64_t items = plan.split ? plan.units * tiles : plan.units;
     plan.grid = (uint32_t)((plan.split && items > SLOTS ? SLOTS : items) + 7) & ~7u;
@@ -1009,10 +1010,11 @@ int launch_sharedkv_block(void *stream, const BlockAttentionArgs *a)
                        a->batch, plan.split ? plan.units : 0u, a->tokens, (uint32_t)__builtin_ctz(a->ratio), a->window,
                        a->oriTableWidth, a->ratio > 1 ? a->cmpTableWidth : 0u, group, a->kvHeads, inverse, 31 + bits, *a);
     if (plan.split) {
-        // Parts of a unit, at most, where all are alike.
-        const bool few = plan.grid / plan.units <= 16;
-        hipLaunchKernelGGL(few ? &block_join<512> : &block_join<128>, dim3(plan.units * 16 * plan.rt, few ? 1 : 4), dim3(THREADS),
-                           0, static_cast<hipStream_t>(stream), a->partial, a->units, (uint32_t)plan.rt, group, a->heads, *a);
+        // By the parts of a unit where all are alike: few rows of many parts take more work-groups.
+        const uint32_t parts = plan.grid / plan.units, channels = parts <= 16 ? 512 : parts <= 64 ? 128 : 32;
+        hipLaunchKernelGGL(channels == 512 ? &block_join<512> : channels == 128 ? &block_join<128> : &block_join<32>,
+                           dim3(plan.units * 16 * plan.rt, D / channels), dim3(THREADS), 0, static_cast<hipStream_t>(stream),
+                           a->partial, a->units, (uint32_t)plan.rt, group, a->heads, *a);
     }
     return (int)hipGetLastError();
 }
