@@ -131,8 +131,8 @@ struct Unit {
     int32_t token, row0, head0, unused;   // first token of the request, the unit's first row in it, its first head
 };
 
-// A request's rows of the launch, made safe: nothing below reads past the
-// arrays whatever cuQ and seqLens hold.
+// A request's rows of the launch, made safe: nothing below reads or writes past
+// the arrays whatever cuQ and seqLens hold.
 struct Request {
     int32_t first, count, length;      // first token, tokens, all rows
     int32_t per_head, units, tiles;    // units of a KV head, of all; tiles of a unit, at most
@@ -292,7 +292,7 @@ struct alignas(1024) Shared {
 };
 
 template <bool E4M3, int RT>
-__global__ void __launch_bounds__(THREADS, 2) block_attention(const uint64_t cu_q, const uint64_t seq_lens, const uint32_t batch_arg, const uint32_t split,
+__global__ void __launch_bounds__(THREADS, 2) block_attention(const uint64_t cu_q, const uint64_t seq_lens, const uint32_t batch_arg, const uint32_t split_arg,
                 const uint32_t tokens_arg, const uint32_t ratio_bits, const uint32_t window_rows, const uint32_t ori_width,
                 const uint32_t cmp_width, const uint32_t group_arg, const uint32_t kv_heads, const uint32_t group_inverse,
                 const uint32_t group_bits, const BlockAttentionArgs p)
@@ -302,7 +302,9 @@ __global__ void __launch_bounds__(THREADS, 2) block_attention(const uint64_t cu_
     constexpr int ROWS = S::ROWS, PARTS = S::PARTS, MIN_TILES = RT == 4 ? 8 : RT;
     __shared__ S s;
     const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6), g = lane >> 4, n = lane & 15;
-    // The leading arguments are the ones that the first loads need: the build preloads them into SGPRs.
+    // The leading arguments are the ones that the first loads need: the build preloads them into SGPRs.  split_arg: the units
+    // and, from bit 16 on, the work-groups that the launch has scratch for; 0 where it is not split.
+    const uint32_t split = split_arg & 0xffff;
     const int group = (int)group_arg, heads = group * (int)kv_heads, batch = (int)batch_arg;
     const auto *cu = gptr<int32_t>(cu_q), *lens = gptr<int32_t>(seq_lens);
 
@@ -360,7 +362,7 @@ __global__ void __launch_bounds__(THREADS, 2) block_attention(const uint64_t cu_
         items = number;
         const int share = (items + 7) / 8;
         item = may_split ? (int)(blockIdx.x & 7) * share + (int)(blockIdx.x >> 3) : (int)blockIdx.x;
-        return item < items && !(may_split && (int)(blockIdx.x >> 3) >= share);
+        return item < (may_split ? min(items, (int)(split_arg >> 16)) : items) && !(may_split && (int)(blockIdx.x >> 3) >= share);
     };
     if (one_wave) {                                    // every wave for itself
         const int n_items = mine.units * parts_of(mine.tiles), upto = wave_upto(n_items), at_units = wave_upto(mine.units);
@@ -417,7 +419,7 @@ __global__ void __launch_bounds__(THREADS, 2) block_attention(const uint64_t cu_
     if (b < 0) {                                       // rows behind the last request
         const int64_t first = (int64_t)end + (int64_t)(item - (items - pad_units)) * ROWS;
         for (int i = wave; i < ROWS; i += WAVES)
-            if (first + i < all_rows) zero_row(first + i);
+            if (first + i >= end && first + i < all_rows) zero_row(first + i);
         return;
     }
     b = uni(b), local = uni(local), unit0 = uni(unit0);
@@ -434,12 +436,13 @@ __global__ void __launch_bounds__(THREADS, 2) block_attention(const uint64_t cu_
     const int start = r.length - r.count, at0 = start + t0, at1 = start + t1;     // positions
     const int window = (int)min(size.window, 0x7fffffffu);
     const int cmp_rows = uni(compressed_at(size, at1)), cmp_tiles = (cmp_rows + KEYS - 1) / KEYS;
-    const int low = max(0, at0 - window + 1) & ~(PAGE_ROWS - 1);
+    const int low = (at0 >= window ? at0 - window + 1 : 0) & ~(PAGE_ROWS - 1);
     const int high = (int)min((int64_t)at1 + 1, (int64_t)size.oriTableWidth * PAGE_ROWS);
     const int tiles = r.length > 0 ? cmp_tiles + max(0, high - low + KEYS - 1) / KEYS : 0;
     const int parts = uni(min(slots, parts_of(tiles)));
-    if (may_split && part == 0 && tid == 0) {
-        auto *to = gout<int32_t>(p.units + sizeof(Unit) * (uint64_t)(1 + unit0 + kv_head * r.per_head + in_head));
+    const int its_unit = unit0 + kv_head * r.per_head + in_head;
+    if (may_split && part == 0 && tid == 0 && (uint32_t)its_unit < split) {
+        auto *to = gout<int32_t>(p.units + sizeof(Unit) * (uint64_t)(1 + its_unit));
         const Unit u = {item, r.per_head, parts, rows, r.first, row0, kv_head * group, 0};
         to[0] = u.first, to[1] = u.stride, to[2] = u.parts, to[3] = u.rows, to[4] = u.token, to[5] = u.row0, to[6] = u.head0;
     }
@@ -679,7 +682,7 @@ __global__ void __launch_bounds__(THREADS, 2) block_attention(const uint64_t cu_
         if (edge) {
             const int position = start + s.token[its_row], base = base_of(k);
             const int to = k < cmp_tiles ? compressed_at(size, position) - base : position + 1 - base;
-            const int from = k < cmp_tiles ? 0 : max(0, position - window + 1 - base);
+            const int from = k < cmp_tiles || position < window ? 0 : max(0, position - window + 1 - base);
             uint64_t bits = seen;
             bits &= to >= KEYS ? ~0ull : to <= 0 ? 0ull : ~0ull >> (KEYS - to);
             bits &= from >= KEYS ? 0ull : ~0ull << from;
@@ -1007,7 +1010,7 @@ int launch_sharedkv_block(void *stream, const BlockAttentionArgs *a)
     while ((1u << bits) < group) ++bits;
     const uint32_t inverse = (uint32_t)(((0x80000000ull << bits) + group - 1) / group);
     hipLaunchKernelGGL(kernel, dim3(plan.grid), dim3(THREADS), 0, static_cast<hipStream_t>(stream), a->cuQ, a->seqLens,
-                       a->batch, plan.split ? plan.units : 0u, a->tokens, (uint32_t)__builtin_ctz(a->ratio), a->window,
+                       a->batch, plan.split ? plan.grid << 16 | plan.units : 0u, a->tokens, (uint32_t)__builtin_ctz(a->ratio), a->window,
                        a->oriTableWidth, a->ratio > 1 ? a->cmpTableWidth : 0u, group, a->kvHeads, inverse, 31 + bits, *a);
     if (plan.split) {
         // By the parts of a unit where all are alike: few rows of many parts take more work-groups.
