@@ -704,11 +704,17 @@ __global__ void __launch_bounds__(THREADS, 2) block_attention(const uint64_t cu_
             lift[h] = __builtin_amdgcn_logf(its < LEAST ? LEAST : its);
             drop[h] = __builtin_amdgcn_exp2f(-lift[h]);
         }
-        float peak = -INFINITY;                        // of score + lift
+        float peak = -INFINITY, most = -INFINITY;      // of score + lift
 #pragma unroll
         for (int kt = 0; kt < RT; ++kt) {
-            float most = fmaxf(fmaxf(w[kt][0], w[kt][1]), fmaxf(w[kt][2], w[kt][3]));
-            peak = fmaxf(peak, __builtin_fmaf(most, step[PAGES == 2 ? kt >> 1 : 0], lift[PAGES == 2 ? kt >> 1 : 0]));
+            // (These maxima pass over a NaN and take two values an instruction.)
+            if (PAGES == 1 || !(kt & 1)) most = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 4; i += 2) most = __builtin_elementwise_maxnum(__builtin_elementwise_maxnum(most, w[kt][i]), w[kt][i + 1]);
+            if (PAGES == 1 || kt & 1) {
+                const int h = PAGES == 2 ? kt >> 1 : 0;
+                peak = __builtin_elementwise_maxnum(peak, __builtin_fmaf(most, step[h], lift[h]));
+            }
         }
         peak = row_max(peak);
         if (PARTS > 1) {                               // the row's keys are spread over waves
@@ -729,8 +735,8 @@ __global__ void __launch_bounds__(THREADS, 2) block_attention(const uint64_t cu_
             if (lx == 0) s.moved[wave] = any;
             if (any && lx < 16) s.factor[its_row] = factor;
         }
-        {
-            // Weights 2^(score + lift - m): 0 for masked keys, also where all have been masked so far.
+        // Weights 2^(score + lift - m): 0 for masked keys, also where all have been masked so far.
+        auto weigh = [&](auto masked) {
             const float from = m == -INFINITY ? 0.0f : m;
 #pragma unroll
             for (int kt = 0; kt < RT; ++kt) {
@@ -741,14 +747,18 @@ __global__ void __launch_bounds__(THREADS, 2) block_attention(const uint64_t cu_
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     float x = __builtin_amdgcn_exp2f(__builtin_fmaf(w[kt][i], step[h], less));
-                    if (edge) x = w[kt][i] == -INFINITY ? 0.0f : x;   // whatever the page's scale is
+                    if (masked.value) x = w[kt][i] == -INFINITY ? 0.0f : x;   // whatever the page's scale is
                     together += x;
                     half[i] = (_Float16)x;
                 }
-                if (!edge || together != 0.0f) sum = __builtin_fmaf(together, drop[h], sum);
+                if (!masked.value || together != 0.0f) sum = __builtin_fmaf(together, drop[h], sum);
                 *reinterpret_cast<f16x4 *>(s.p + its_row * P_STRIDE + key0 + 16 * kt + 4 * (lx >> 4)) = half;
             }
-        }
+        };
+        if (edge)
+            weigh(std::true_type{});
+        else
+            weigh(std::false_type{});
         if (E4M3 && edge) {
             // A code that is no number may lie in a row that some token does not see, and 0 times it is none either.
             // Rows that see it have weights that are no numbers already.
