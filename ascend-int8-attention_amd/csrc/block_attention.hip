@@ -172,9 +172,9 @@ __device__ __forceinline__ Request request_of(const Sizes &p, int c0, int c1, in
 __device__ __forceinline__ float row_max(float v)
 {
     auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    v = __builtin_elementwise_maxnum(__uint_as_float(a[0]), __uint_as_float(a[1]));
     a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    return __builtin_elementwise_maxnum(__uint_as_float(a[0]), __uint_as_float(a[1]));
 }
 
 // Sum over the lanes up to and with this one.
@@ -723,17 +723,14 @@ __global__ void __launch_bounds__(THREADS, 2) block_attention(const uint64_t cu_
 #pragma unroll
             for (int part = 0; part < PARTS; ++part) peak = fmaxf(peak, s.peak[part][its_row]);
         }
-        float factor = 1.0f;
         const bool move = peak > m + LIMIT;            // and where m is still -infinity
-        if (move) {
-            factor = __builtin_amdgcn_exp2f(m - (peak - HEAD));
-            m = peak - HEAD;
-            sum *= factor;
-        }
         const bool any = __ballot(move) != 0;
-        if (wave < RT) {
-            if (lx == 0) s.moved[wave] = any;
-            if (any && lx < 16) s.factor[its_row] = factor;
+        if (wave < RT && lx == 0) s.moved[wave] = any;
+        if (any) {                                     // seldom
+            const float factor = move ? __builtin_amdgcn_exp2f(m - (peak - HEAD)) : 1.0f;
+            if (move) m = peak - HEAD;
+            sum *= factor;
+            if (wave < RT && lx < 16) s.factor[its_row] = factor;
         }
         // Weights 2^(score + lift - m): 0 for masked keys, also where all have been masked so far.
         auto weigh = [&](auto masked) {
