@@ -13,7 +13,7 @@
 // e^{s_j} takes a page's weights times 1 / scale_j.
 //
 // Q K.  INT8 codes run on v_mfma_i32_16x16x64_i8: Q times a power of two of its
-// row becomes whole numbers of 16 bits (exactly, but for values below 2^-7 of
+// row becomes whole numbers of 16 bits (exactly, but for values below 2^-6 of
 // the row's largest), split into two signed bytes, and the sums are exact.  e4m3
 // codes, exact in BF16, run on v_mfma_f32_16x16x32_bf16 against Q as it is.  (Q in
 // two e4m3 terms would spare the conversion, at the same rate, but that matrix
@@ -29,7 +29,19 @@
 // channels, the weights passing between them in LDS.  Tiles come by LDS DMA into
 // a ring of two, one in flight while the other is used.  Every work-group makes
 // the same plan from the live lengths.  Where units are split, a second launch
-// joins their items' states, a row and 128 channels a work-group.
+// joins their items' states.
+//
+// What bounds it.  Few query rows: the cache's bytes, 5.1 TB/s for 16 requests
+// of one token and 8 heads over 32-128 K rows (131 us).  64 rows a unit: the
+// vector instructions beside the matrix ones: of INT8, 178 (most of them codes to
+// FP16) within the products of a wave and tile beside 128 matrix ones, and the
+// softmax's.  512 tokens of one request over 64 K rows reach 1183 TFLOP/s, a large
+// library FP16 product 1200-1240, and two prompts' chunks of 1900-2048 tokens over
+// 8-16 K rows 1035 (715 us).  Between them, split contexts:
+// the states of all items, written and read (up to 67 MB of 64-row units: 32
+// requests of 64 heads over 6-16 K rows 85 us, 15.5 of them the join), and the launch's chain
+// of round trips (lengths, pages and Q, scales, a tile; the join): one request of
+// 4096 rows takes 12.1 us; in a trace the two kernels take 8.5-9.2 and 3.9.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -299,7 +311,8 @@ __global__ void __launch_bounds__(THREADS, 2) block_attention(const uint64_t cu_
 {
     const Sizes size = {tokens_arg, ratio_bits, window_rows, ori_width, cmp_width, group_arg, kv_heads, group_inverse, group_bits};
     using S = Shared<RT>;
-    constexpr int ROWS = S::ROWS, PARTS = S::PARTS, MIN_TILES = RT == 4 ? 8 : RT;
+    constexpr int ROWS = S::ROWS, PARTS = S::PARTS;
+    constexpr int MIN_TILES = RT == 4 ? 8 : RT; // of an item; 1 to 12 differ little
     __shared__ S s;
     const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6), g = lane >> 4, n = lane & 15;
     // The leading arguments are the ones that the first loads need: the build preloads them into SGPRs.  split_arg: the units
@@ -980,9 +993,20 @@ Plan plan_of(const BlockAttentionArgs *a)
     const uint64_t near = (uint64_t)a->window + 2 * PAGE_ROWS + 64;
     const uint64_t tiles = (a->ratio > 1 ? (a->cmpTableWidth + 1) / 2 : 0) +
                            ((near / PAGE_ROWS < a->oriTableWidth ? near / PAGE_ROWS : a->oriTableWidth) + 1) / 2;
+    // Units of 16 rows spread few rows over more work-groups and have the smallest states; units of 64 rows convert a key
+    // for more of them, so that the matrix instructions bound them, but split contexts move four times the states.  With R
+    // tiles of 64 rows in a launch and `tiles` of 64 keys in a unit, the better one goes by R * R * tiles, and for units of
+    // 64 rows by the tiles too (microseconds of 16, 32 and 64 rows a unit):
+    //        64  1 request, 64 heads, 4 K      16.6, 18.5, 33.7     131 K  16 of 16 tokens, 8 K         82.3, 64.3, 63.7
+    //       4 K  8, 64 heads, 4 K              25.5, 28.9, 38.2     131 K  1 of 128 tokens, 32 K         144,  101, 89.3
+    //      16 K  8 of 8 tokens, 16 K           50.0, 42.7, 42.4     131 K  64 of 8 tokens, 2 K          53.0, 44.5, 45.2
+    //      32 K  8, 64 heads, 32 K             83.3, 69.6, 69.5     262 K  32, 64 heads, 6-16 K          120, 89.9, 85.0
+    //      65 K  4 of 32 tokens, 16 K          81.3, 61.1, 62.6     262 K  8 of 256 tokens, window      33.4, 24.4, 32.9
+    //     1.0 M  2 of 2048 tokens, window      65.3, 47.1, 38.3     4.2 M  4 of 512 tokens, 4 K          256,  160,  158
     const uint64_t each = (rows / a->kvHeads + a->batch - 1) / a->batch;        // rows of a request and KV head, on average
     const uint64_t score = (rows + 63) / 64 * ((rows + 63) / 64) * tiles;
-    plan.rt = each <= 16 || score < 8000 ? 1 : each <= 32 || score < 400000 ? 2 : 4;
+    const bool wide = score >= 400000 || (score >= 130000 && tiles >= 128);
+    plan.rt = each <= 16 || score < 8000 ? 1 : each <= 32 || !wide ? 2 : 4;
     // The last unit of a request and KV head may be short, and so may the padding's; a token's rows are in few units.
     const uint64_t group = a->heads / a->kvHeads, unit = 16 * plan.rt;
     const uint64_t short_last = rows / unit + (uint64_t)a->batch * a->kvHeads;
