@@ -17,12 +17,15 @@
 // within them, that row or page is done again in FP64.  (FP64 throughout takes
 // 26.5 us where this takes 18.8: 48 requests of 1-200 rows of four heads.)
 //
-// What bounds it.  1024 bytes read and 512 written for a row and head: bytes,
-// from some thousand rows on, and below that one chain of round trips (the
-// requests' ends; the rows, their positions and page; the angles and the old
-// scale; the codes).  A work-group takes a page: the rows that share a scale
-// are in its registers from the first read on, so they are read once and a
-// launch needs no second pass.
+// What bounds it.  1024 bytes read and 512 written for a row and head, beside
+// 185 vector instructions for the codes of a lane's eight values (e4m3 143); with
+// few rows one chain of round trips (the requests' ends; the rows, their positions and
+// page; the angles and the old scale; the codes).  One row takes 4.1 us, 256
+// requests' 6.4, five prompts of 700-2600 rows 8.1, 65536 rows 31 (3.8 TB/s).  A
+// work-group takes a page: the rows that share a scale are in its registers from
+// the first read on, so they are read once and a launch needs no second pass.
+// Eight waves with four rows each: with two rows each 9.9 and 39 us for the last
+// two, with eight 10.3 and 30.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
