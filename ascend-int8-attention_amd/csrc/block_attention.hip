@@ -32,14 +32,14 @@
 // joins their items' states.
 //
 // What bounds it.  Few query rows: the cache's bytes, 5.1 TB/s for 16 requests
-// of one token and 8 heads over 32-128 K rows (131 us).  64 rows a unit: the
-// vector instructions beside the matrix ones: of INT8, 178 (most of them codes to
-// FP16) within the products of a wave and tile beside 128 matrix ones, and the
-// softmax's.  512 tokens of one request over 64 K rows reach 1183 TFLOP/s, a large
-// library FP16 product 1200-1240, and two prompts' chunks of 1900-2048 tokens over
-// 8-16 K rows 1035 (715 us).  Between them, split contexts:
+// of one token and 8 heads over 32-128 K rows (131-135 us).  64 rows a unit: the
+// vector instructions beside the matrix ones (codes to FP16 and the softmax): a wave
+// and INT8 tile counts 513 SQ_INSTS_VALU and 128 SQ_INSTS_MFMA, and the matrix
+// cores are busy for 43 % of the time.  512 tokens of one request over 64 K rows
+// reach 1133-1183 TFLOP/s by the card, a large library FP16 product 1200-1240, and
+// two prompts' chunks of 1900-2048 tokens over 8-16 K rows 1015-1035 (715-730 us).  Between them, split contexts:
 // the states of all items, written and read (up to 67 MB of 64-row units: 32
-// requests of 64 heads over 6-16 K rows 85 us, 15.5 of them the join), and the launch's chain
+// requests of 64 heads over 6-16 K rows 80-85 us, 12-15.5 of them the join), and the launch's chain
 // of round trips (lengths, pages and Q, scales, a tile; the join): one request of
 // 4096 rows takes 12.1 us; in a trace the two kernels take 8.5-9.2 and 3.9.
 #include <hip/hip_runtime.h>
