@@ -94,6 +94,7 @@ __device__ __forceinline__ float sum_of(float a, float b, float c, float d)
 }
 
 // Rounded to FP32 such that another rounding to fewer bits is that of the value itself: inexact ones end in a set bit.
+// `larger`: the nearest number's size is larger than the value's, so it is none of the zeros.
 __device__ __forceinline__ float to_odd(float nearest, bool larger, bool inexact)
 {
     return __uint_as_float((__float_as_uint(nearest) - (larger ? 1u : 0u)) | (inexact ? 1u : 0u));
@@ -379,7 +380,7 @@ __global__ void __launch_bounds__(THREADS, 4) cache_append(const uint64_t cu_q, 
             for (int e = 0; e < 8; ++e) {
                 v[e] = __builtin_fmaf(__builtin_fmaf(-v[e], scale, y[i][e]), reciprocal, v[e]);
                 const float rest = __builtin_fmaf(-v[e], scale, y[i][e]);
-                v[e] = to_odd(v[e], rest != 0.0f && (rest < 0.0f) != (v[e] < 0.0f), rest != 0.0f);
+                v[e] = to_odd(v[e], rest < 0.0f ? v[e] > 0.0f : rest > 0.0f && v[e] < 0.0f, rest != 0.0f);
             }
             u32x2 other;
             const bool some = encode(v, true, other);

@@ -1,0 +1,59 @@
+"""PreparedCacheAppend where FP32 ends: values that vanish beside a page's scale.
+Byte for byte against the definition in 64 bits, as test_gpu_append.py."""
+import numpy as np
+import pytest
+
+from tests import block_cases as cases
+from tests.test_gpu_append import Appended, DIM
+
+pytestmark = pytest.mark.gpu
+KINDS = ["int8", "e4m3"]
+
+
+def one_row(case, x, length):
+    """Appends the row x [1, 1, 512] behind the first request's, on the device and in the definition; what both then hold."""
+    import torch
+    from npu_sparse_attn_sharedkv_int8 import PreparedCacheAppend
+    codes, scale = case.expect()
+    put = lambda a: torch.from_numpy(np.ascontiguousarray(a)).cuda()  # noqa: E731
+    cu, lens = np.array([0, 1], np.int32), np.array([length], np.int32)
+    PreparedCacheAppend(case.cache, put(x).to(torch.bfloat16), put(case.table[:1]), put(cu), put(lens), scale=case.scale,
+                        rotation=put(case.rotation)).run()
+    turned = cases.rotated(x.astype(np.float64), case.rotation, np.array([length - 1]), case.pairs)
+    cases.append(codes, scale, case.kind, turned, case.table[:1], cu, lens)
+    return codes, scale
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("peak,tiny", [(1e10, 1e-38), (1e8, 1e-40), (1e30, 1e-12), (3e38, 1.0), (1.0, 1e-39)])
+@pytest.mark.parametrize("rotary", [0, 64])
+def test_values_that_vanish_beside_the_largest(kind, peak, tiny, rotary):
+    case = Appended(40, [20, 3], [50, 3], kind=kind, rotary=rotary)
+    case.x *= tiny                                          # both signs, down to denormal ones
+    case.x[:, 0, 7] = -tiny
+    case.x[::2, 0, 100] = peak                              # 7 channels of a lane's eight beside it
+    case.x[3, 0, 470] = -peak
+    case.x = cases.bf16(case.x)
+    case.operator().run()
+    case.check(*case.expect())
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_small_rows_on_a_page_that_had_an_infinity(kind):
+    case = Appended(41, [3, 2], [3, 60], kind=kind)        # the second for its rotation's length
+    case.x[1, 0, 5] = np.inf
+    case.operator().run()
+    case.check(*case.expect())
+    x = cases.bf16(case.rng.standard_normal((1, 1, DIM)) * 1e-10)
+    case.check(*one_row(case, x, 4))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("lengths", [[70, 12], [40, 9]], ids=str)
+def test_rows_of_zeros(kind, lengths):
+    """Fresh pages get the smallest scale, pages that have rows keep theirs."""
+    case = Appended(42, [40, 3], lengths, kind=kind)
+    case.x[:] = 0
+    case.x[1::2] = -0.0
+    case.operator().run()
+    case.check(*case.expect())
