@@ -85,7 +85,8 @@ __device__ __forceinline__ float wave_max(float v)
 }
 
 // a b + c d.  FP32: the second product's rounding is taken back, so that the sum is off by 2^-23 of itself and 2^-47 of the
-// products at most, also where they nearly cancel.
+// products at most, also where they nearly cancel.  Where a product is infinite it is no number, though the sum may be one:
+// rows that have such a value are done in FP64.
 __device__ __forceinline__ double sum_of(double a, double b, double c, double d) { return fma(a, b, c * d); }
 __device__ __forceinline__ float sum_of(float a, float b, float c, float d)
 {
@@ -117,6 +118,7 @@ __device__ __forceinline__ uint32_t pack_bytes(const int (&x)[4])
 
 struct Shared {
     int32_t found[4];                            // request, its first and end token, its rows
+    uint32_t odd[WAVES];                         // whether a rotated value is no number in FP32
     float peak[2][WAVES];                        // of channels as they are, of rotated ones
 };
 
@@ -282,22 +284,32 @@ __global__ void __launch_bounds__(THREADS, 4) cache_append(const uint64_t cu_q, 
     constexpr float LARGEST = CODES == E4M3 ? 448.0f : 127.0f;
     // NaN values do not count, infinities as the largest number.
     float its = 0.0f, most[EACH];
+    uint32_t odd = 0;                            // rows of the wave with a rotated value that is no number in FP32
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
-        most[i] = 0.0f;
+        most[i] = 0.0f;                          // keeps a NaN
 #pragma unroll
-        for (int e = 0; e < 8; ++e) most[i] = fmaxf(most[i], mine[i] ? fabsf(y[i][e]) : 0.0f);
+        for (int e = 0; e < 8; ++e) most[i] = __builtin_elementwise_maximum(most[i], mine[i] ? fabsf(y[i][e]) : 0.0f);
+        const bool none = !(most[i] < INFINITY);
+        if (__ballot(none)) {                    // seldom
+            odd |= __ballot(none && turned) ? 1u << i : 0u;
+            float others = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) others = fmaxf(others, turned ? 0.0f : fabsf(y[i][e]));
+            most[i] = none ? others : most[i];
+        }
         its = fmaxf(its, most[i]);
     }
     const float still = wave_max(turned ? 0.0f : its), rotated = wave_max(turned ? its : 0.0f);
-    if (lane == 0) s.peak[0][wave] = still, s.peak[1][wave] = rotated;
+    if (lane == 0) s.peak[0][wave] = still, s.peak[1][wave] = rotated, s.odd[wave] = odd;
     asm volatile("" : "+v"(old));                // read before any wave may store the new one
     __syncthreads();
     float peak = 0.0f, other = 0.0f;
+    uint32_t any_odd = 0;
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) peak = fmaxf(peak, s.peak[0][w]), other = fmaxf(other, s.peak[1][w]);
-    if (!(peak >= other * (1.0f + 0x1p-20f))) {  // the page's largest value may be a rotated one: exactly
-        uint32_t rest = 0;
+    for (int w = 0; w < WAVES; ++w) peak = fmaxf(peak, s.peak[0][w]), other = fmaxf(other, s.peak[1][w]), any_odd |= s.odd[w];
+    if (any_odd || !(peak >= other * (1.0f + 0x1p-20f))) {  // the page's largest value may be a rotated one: exactly
+        uint32_t rest = odd;
 #pragma unroll
         for (int i = 0; i < EACH; ++i) rest |= __ballot(turned && most[i] * (1.0f + 0x1p-20f) >= other) && mine[i] ? 1u << i : 0u;
         its = 0.0f;
@@ -365,7 +377,7 @@ __global__ void __launch_bounds__(THREADS, 4) cache_append(const uint64_t cu_q, 
         }
         return most < 0.5f;
     };
-    uint32_t rest = 0;                           // rows that have a code to be made in FP64
+    uint32_t rest = odd;                         // rows that have a code to be made in FP64
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
         if (!mine[i]) continue;

@@ -1,5 +1,6 @@
-"""PreparedCacheAppend where FP32 ends: values that vanish beside a page's scale.
-Byte for byte against the definition in 64 bits, as test_gpu_append.py."""
+"""PreparedCacheAppend where FP32 ends: values that vanish beside a page's scale, and
+infinities in rotated channels.  Byte for byte against the definition in 64 bits,
+as test_gpu_append.py."""
 import numpy as np
 import pytest
 
@@ -55,5 +56,46 @@ def test_rows_of_zeros(kind, lengths):
     case = Appended(42, [40, 3], lengths, kind=kind)
     case.x[:] = 0
     case.x[1::2] = -0.0
+    case.operator().run()
+    case.check(*case.expect())
+
+
+def angled(case, size):
+    """The case with its rotation `size` times as long (position 0 too turns by some angle)."""
+    angle = np.arange(len(case.rotation))[:, None] * 0.7 + 0.3 + np.arange(case.rotation.shape[1] // 2)
+    case.rotation = (np.concatenate([np.cos(angle), np.sin(angle)], 1) * size).astype(np.float32)
+    return case
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("pairs", [True, False])
+@pytest.mark.parametrize("channels", [[448], [449], [511], [480, 481], [479, 450], [460, 12]], ids=str)
+def test_infinities_in_rotated_channels(kind, pairs, channels):
+    case = angled(Appended(43, [40, 3, 1], [70, 9, 33], kind=kind, pairs=pairs), 1.0)
+    for i, channel in enumerate(channels):
+        case.x[7 + 30 * (i % 2), 0, channel] = np.inf if i % 2 else -np.inf
+    case.x[41, 0, channels[0]] = np.inf                     # of a page that has rows
+    case.x[42, 0, 449] = np.nan                             # beside numbers: none of the page's scale
+    case.operator().run()
+    case.check(*case.expect())
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("channel", [448, 449, 479, 480, 510, 511])
+def test_an_infinity_on_its_own(kind, channel):
+    case = angled(Appended(44, [2, 1], [2, 20], kind=kind), 1.0)
+    case.x[0, 0, channel] = case.x[2, 0, channel] = np.inf
+    case.operator().run()
+    case.check(*case.expect())
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("pairs", [True, False])
+def test_products_past_the_largest_number(kind, pairs):
+    """A rotation longer than 1: finite values whose products pass FP32, and some that come back below it."""
+    case = angled(Appended(45, [40, 3], [70, 9], kind=kind, pairs=pairs), 4.0)
+    case.x[2, 0, 448:] *= 1e38
+    case.x[41, 0, 449::2] *= 1e38
+    case.x = cases.bf16(case.x)
     case.operator().run()
     case.check(*case.expect())
