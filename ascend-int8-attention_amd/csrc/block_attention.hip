@@ -13,8 +13,13 @@
 // e^{s_j} takes a page's weights times 1 / scale_j.
 //
 // Q K.  INT8 codes run on v_mfma_i32_16x16x64_i8: Q times a power of two of its
-// row becomes whole numbers of 16 bits (exactly, but for values below 2^-6 of
-// the row's largest), split into two signed bytes, and the sums are exact.  e4m3
+// row becomes whole numbers, off by half of one at most, and the sums are exact.
+// Two signed bytes hold the row's values up to the smaller of its largest and 8
+// times its mean |q| (normal values' largest of 512 is some 4-5 times), so a unit is
+// at most 2^-14 of that.  What is larger, in rows of which a few channels are, has a
+// third byte: those blocks of 64 channels take one more matrix instruction for each
+// sixteen keys, with that byte made from Q again for each tile.  (With 16 bits for
+// the row's largest a channel of 300 beside normal ones moves scores by 0.03.)  e4m3
 // codes, exact in BF16, run on v_mfma_f32_16x16x32_bf16 against Q as it is.  (Q in
 // two e4m3 terms would spare the conversion, at the same rate, but that matrix
 // instruction sums eight products with 13 bits below their largest: scores up to
@@ -190,6 +195,15 @@ __device__ __forceinline__ float row_max(float v)
     return __builtin_elementwise_maxnum(__uint_as_float(a[0]), __uint_as_float(a[1]));
 }
 
+// Sum over them.
+__device__ __forceinline__ float row_total(float v)
+{
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+
 // Sum over the lanes up to and with this one.
 __device__ __forceinline__ int wave_upto(int v)
 {
@@ -204,13 +218,14 @@ __device__ __forceinline__ int wave_upto(int v)
 __device__ __forceinline__ int wave_sum(int v) { return __builtin_amdgcn_readlane(wave_upto(v), 63); }
 
 // Q of a lane's row as the matrix instructions take it: INT8, in two terms of whole numbers relative to a power of two
-// of its own, most significant first; e4m3, the first and the last eight of sixteen channels as they are.
+// of its own, most significant first (and, made where they are used, third terms above them); e4m3, the first and the last eight of sixteen channels as they are.
 template <bool E4M3>
 struct Query {
     static constexpr float LARGEST = 127.0f * 256.0f;
     v4i term[2][8];                    // of channels 64 j + 16 g on
     float inverse, step;               // units of one; score (base 2) of one unit and scale 1
 
+    // `peak`: of the values that two terms hold.
     __device__ __forceinline__ void set(float peak, float softmax2)
     {
         // Rows below 2^-90 score zero to FP32 against any code; their inverse would overflow.  The units' sign is the
@@ -221,15 +236,18 @@ struct Query {
         inverse = some && !odd ? (softmax2 < 0.0f ? -1.0f : 1.0f) * ldexpf(1.0f, power) : 0.0f;
         step = odd ? __builtin_nanf("") : some ? ldexpf(fabsf(softmax2), -power) : 1.0f;
     }
+    // With 1.5 * 2^23 more, the nearest whole number sits in the low bits; with half of a byte's range more too,
+    // the second byte is rounded as the first, signed, byte wants it, and that one has its sign bit flipped.
+    static __device__ __forceinline__ uint32_t whole(const u32x4 &w, int e, float inverse)
+    {
+        return __float_as_uint(__builtin_fmaf(e & 1 ? bf16_hi(w[e / 2]) : bf16_lo(w[e / 2]), inverse, 12582912.0f + 128.0f));
+    }
     // Eight channels' whole numbers: words [term][0 and 1].
     __device__ __forceinline__ void make(uint32_t (&out)[2][2], const u32x4 &w) const
     {
         uint32_t v[8];
-        // With 1.5 * 2^23 more, the nearest whole number sits in the low bits; with half of a byte's range more too,
-        // the second byte is rounded as the first, signed, byte wants it, and that one has its sign bit flipped.
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-            v[e] = __float_as_uint(__builtin_fmaf(e & 1 ? bf16_hi(w[e / 2]) : bf16_lo(w[e / 2]), inverse, 12582912.0f + 128.0f));
+        for (int e = 0; e < 8; ++e) v[e] = whole(w, e, inverse);
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
             const uint32_t *u = v + 4 * q;
@@ -237,6 +255,21 @@ struct Query {
             out[0][q] = __builtin_amdgcn_perm(cd, ab, 0x07050301u);
             out[1][q] = __builtin_amdgcn_perm(cd, ab, 0x06040200u) ^ 0x80808080u;
         }
+    }
+    // What sixteen channels have beyond the two terms, in 65536 units: at most 32, as no value is more than 512 times the
+    // row's mean and the two terms hold 8 times that or all.
+    static __device__ __forceinline__ v4i beyond(const u32x4 &a, const u32x4 &b, float inverse)
+    {
+        v4i out;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            uint32_t word = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                word |= (((whole(q < 2 ? a : b, 4 * (q & 1) + e, inverse) - 0x4b400000u + 0x8000u) >> 16) & 255u) << (8 * e);
+            out[q] = (int)word;
+        }
+        return out;
     }
 };
 
@@ -297,11 +330,14 @@ struct alignas(1024) Shared {
     int8_t tile[2][KEYS * D];          // key rows, their 16-byte chunks XOR-swizzled with the row
     _Float16 p[ROWS * P_STRIDE];       // weights [row][key]
     float factor[ROWS], top[ROWS], sum[PARTS][ROWS], peak[PARTS][ROWS];
+    float mean[PARTS][ROWS], inverse[ROWS];   // INT8: sums of |q|, units of one
+    uint32_t far[WAVES];               // INT8: blocks of 64 channels where a row of the wave's has values beyond two terms
     int32_t moved[RT];                 // whether a row tile moved its maximum in this tile
     int32_t scan[3][WAVES];
     int32_t found[6];
     int32_t token[ROWS];               // of the unit's rows, counted in the request
     int32_t place[ROWS];               // their rows of q and out
+    uint64_t query[ROWS];              // INT8: their addresses in q
 };
 
 template <bool E4M3, int RT>
@@ -535,6 +571,7 @@ __global__ void __launch_bounds__(THREADS, 2) block_attention(const uint64_t cu_
     Query<E4M3> q = {};
     auto stage_at = [&](int8_t *stage, int t, int j) { return stage + ((((wave % RT) * AT_ONCE + t) * 8 + j) * 64 + lane) * 16; };
     uint64_t seen = 0, next_seen = 0;
+    uint32_t far = 0;                                  // INT8: blocks of 64 channels where a row has values beyond two terms
     if (k0 < k1) {
         const float softmax2 = p.softmaxScale * LOG2E;
         const auto *q_row = gptr<u32x4>(p.q + (uint64_t)(uint32_t)s.place[row] * (D * 2)) + 2 * g + 8 * j0;
@@ -554,25 +591,45 @@ __global__ void __launch_bounds__(THREADS, 2) block_attention(const uint64_t cu_
 #pragma unroll
                 for (int h = 0; h < 2; ++h) q.term[h][j] = __builtin_bit_cast(v4i, raw[j][h] ^ flip);
         } else {
-            float peak = 0.0f;                         // keeps a NaN
+            float peak = 0.0f, sums[2] = {0.0f, 0.0f}; // keeps a NaN; sums of |q|
 #pragma unroll
             for (int j = 0; j < JN; ++j)
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        peak = __builtin_elementwise_maximum(peak, fabsf(bf16_lo(raw[j][h][e])));
-                        peak = __builtin_elementwise_maximum(peak, fabsf(bf16_hi(raw[j][h][e])));
+                        const float lo = fabsf(bf16_lo(raw[j][h][e])), hi = fabsf(bf16_hi(raw[j][h][e]));
+                        peak = __builtin_elementwise_maximum(__builtin_elementwise_maximum(peak, lo), hi);
+                        sums[0] += lo, sums[1] += hi;
                     }
             peak = row_max(peak == peak ? peak : INFINITY);   // from here on infinity stands for both
+            float mean = row_total(sums[0] + sums[1]);
             if (SHARE) {
-                if (g == 0) s.peak[wave / RT][row] = peak;
+                if (g == 0) s.peak[wave / RT][row] = peak, s.mean[wave / RT][row] = mean;
                 lds_barrier();
+                mean = 0.0f;
 #pragma unroll
-                for (int part = 0; part < PARTS; ++part) peak = fmaxf(peak, s.peak[part][row]);
+                for (int part = 0; part < PARTS; ++part) peak = fmaxf(peak, s.peak[part][row]), mean += s.mean[part][row];
                 lds_barrier();
             }
-            q.set(peak, softmax2);
+            // Two terms hold 8 times the mean, whatever a few channels have: those go into a third.
+            const float most = peak < INFINITY ? fminf(peak, mean * (8.0f / D)) : peak;
+            q.set(most, softmax2);
+            if (__ballot(peak > most)) {               // in all waves of these rows
+                if (wave < RT && g == 0)
+                    s.inverse[row] = q.inverse, s.query[row] = p.q + (uint64_t)(uint32_t)s.place[row] * (D * 2);
+#pragma unroll
+                for (int j = 0; j < JN; ++j) {
+                    float its = 0.0f;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            its = fmaxf(its, fmaxf(fabsf(bf16_lo(raw[j][h][e])), fabsf(bf16_hi(raw[j][h][e]))));
+                    far |= __ballot(its * fabsf(q.inverse) > Query<false>::LARGEST) ? 1u << (j0 + j) : 0u;
+                }
+            }
+            if (SHARE && lane == 0) s.far[wave] = far;
             int8_t *stage = s.tile[(k0 + 1) & 1];
             v4i own[SHARE ? 2 : 1][SHARE ? JN : 1];
 #pragma unroll
@@ -603,6 +660,9 @@ __global__ void __launch_bounds__(THREADS, 2) block_attention(const uint64_t cu_
 #pragma unroll
                         for (int j = 0; j < 8; ++j) q.term[t][j] = *reinterpret_cast<const v4i *>(stage_at(stage, t - t0, j));
                 }
+#pragma unroll
+                for (int part = 0; part < PARTS; ++part) far |= s.far[wave % RT + part * RT];
+                far = (uint32_t)uni((int)far);
             }
         }
     }
@@ -690,9 +750,23 @@ __global__ void __launch_bounds__(THREADS, 2) block_attention(const uint64_t cu_
                         for (int kt = 0; kt < PAIR; ++kt)
 #pragma unroll
                             for (int i = 0; i < 4; ++i)
-                                // At most 512 * 32512 * 128 + 512 * 128 * 128: within 32 bits.
+                                // At most 512 * 32512 * 128 + 512 * 128 * 128, and far less where there is a third
+                                // term (fewer than 64 channels pass 8 times the mean): within 32 bits.
                                 w[PAIR * (st >> 3) + kt][i] = (float)(dots[0][kt][i] * 256 + dots[1][kt][i]);
                     __builtin_amdgcn_sched_barrier(0);
+                }
+                for (uint32_t rest = far; rest; rest &= rest - 1) {         // seldom
+                    const int j = __builtin_ctz(rest);
+                    const auto *from = gptr<u32x4>(s.query[its_row]) + 2 * (lx >> 4) + 8 * j;
+                    const u32x4 low = from[0], high = from[1];
+                    const v4i third = Query<E4M3>::beyond(low, high, s.inverse[its_row]);
+#pragma unroll
+                    for (int kt = 0; kt < RT; ++kt) {
+                        const v4i code = *(const lds_v4i *)(uintptr_t)((at ^ (uint32_t)(64 * j)) + (uint32_t)(16 * kt * D));
+                        const v4i dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(code, third, v4i{0, 0, 0, 0}, 0, 0, 0);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) w[kt][i] = __builtin_fmaf((float)dot[i], 65536.0f, w[kt][i]);
+                    }
                 }
             }
         }

@@ -51,9 +51,9 @@ def compare(a, op, rows=None):
         for i in range(n):
             t, place = a.cu[b] + i, length - n + i
             code, scale = a.rows(a.ori, a.ori_table, b, np.arange(place + 1), 0)
-            s = q[t] @ code.T * scale * a.softmax_scale
             sink = a.sink.astype(np.float64)
             with np.errstate(invalid="ignore"):
+                s = q[t] @ code.T * scale * a.softmax_scale
                 top = np.maximum(s.max(1), sink)
                 e = np.exp(s - top[:, None])
                 total = e.sum(1) + np.exp(sink - top)
