@@ -118,7 +118,8 @@ __device__ __forceinline__ uint32_t pack_bytes(const int (&x)[4])
 
 struct Shared {
     int32_t found[4];                            // request, its first and end token, its rows
-    uint32_t odd[WAVES];                         // whether a rotated value is no number in FP32
+    uint32_t odd[WAVES];                         // rows with a rotated value that is no number in FP32
+    int32_t begin[WAVES];                        // first row that is written
     float peak[2][WAVES];                        // of channels as they are, of rotated ones
 };
 
@@ -284,9 +285,11 @@ __global__ void __launch_bounds__(THREADS, 4) cache_append(const uint64_t cu_q, 
     constexpr float LARGEST = CODES == E4M3 ? 448.0f : 127.0f;
     // NaN values do not count, infinities as the largest number.
     float its = 0.0f, most[EACH];
+    int begin_row = PAGE_ROWS;                   // first row that is written
     uint32_t odd = 0;                            // rows of the wave with a rotated value that is no number in FP32
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
+        begin_row = min(begin_row, mine[i] ? wave + WAVES * i : PAGE_ROWS);
         most[i] = 0.0f;                          // keeps a NaN
 #pragma unroll
         for (int e = 0; e < 8; ++e) most[i] = __builtin_elementwise_maximum(most[i], mine[i] ? fabsf(y[i][e]) : 0.0f);
@@ -301,13 +304,16 @@ __global__ void __launch_bounds__(THREADS, 4) cache_append(const uint64_t cu_q, 
         its = fmaxf(its, most[i]);
     }
     const float still = wave_max(turned ? 0.0f : its), rotated = wave_max(turned ? its : 0.0f);
-    if (lane == 0) s.peak[0][wave] = still, s.peak[1][wave] = rotated, s.odd[wave] = odd;
+    if (lane == 0) s.peak[0][wave] = still, s.peak[1][wave] = rotated, s.odd[wave] = odd, s.begin[wave] = begin_row;
     asm volatile("" : "+v"(old));                // read before any wave may store the new one
     __syncthreads();
     float peak = 0.0f, other = 0.0f;
     uint32_t any_odd = 0;
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) peak = fmaxf(peak, s.peak[0][w]), other = fmaxf(other, s.peak[1][w]), any_odd |= s.odd[w];
+    for (int w = 0; w < WAVES; ++w) peak = fmaxf(peak, s.peak[0][w]), other = fmaxf(other, s.peak[1][w]);
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) any_odd |= s.odd[w], begin_row = min(begin_row, s.begin[w]);
+    if (begin_row == PAGE_ROWS) return;          // all are skipped: the page stays as it is, its scale too
     if (any_odd || !(peak >= other * (1.0f + 0x1p-20f))) {  // the page's largest value may be a rotated one: exactly
         uint32_t rest = odd;
 #pragma unroll
@@ -328,7 +334,7 @@ __global__ void __launch_bounds__(THREADS, 4) cache_append(const uint64_t cu_q, 
     }
     const bool infinite = !(peak < INFINITY);
     const float needed = fmaxf(fminf(peak, 0x1.fffffep127f) / LARGEST, FLOOR);
-    const bool begun = low > 0 && old > 0.0f && old < INFINITY;
+    const bool begun = begin_row > 0 && old > 0.0f && old < INFINITY;
     int power = 0;
     float scale = needed;
     if (begun) {
@@ -426,9 +432,12 @@ __global__ void __launch_bounds__(THREADS, 4) cache_append(const uint64_t cu_q, 
         }
         *gout<u32x2>(to + (uint64_t)row * row_bytes) = w;
     }
-    if (power) {                                 // the rows before, in the new scale; rows behind the last stay
+    if (power) {                                 // the rows that were there, in the new scale; rows behind the last stay
         const float f = ldexpf(1.0f, -power);
-        for (int row = wave; row < low; row += WAVES) {
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            const int row = wave + WAVES * i;
+            if (mine[i] || row >= high) continue;
             const u32x2 was = *gptr<u32x2>(to + (uint64_t)row * row_bytes);
             u32x2 w;
 #pragma unroll

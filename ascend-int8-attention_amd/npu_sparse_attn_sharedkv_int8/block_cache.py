@@ -80,7 +80,8 @@ class PreparedCacheAppend:
     of PreparedCacheWrite.
 
     Rows on no page of the pool, past the block table or with a position outside
-    the rotation are skipped; so are tokens past cu_q[batch] and requests with
+    the rotation are skipped, and what lies there counts as rows that the page has
+    (one whose new rows are all skipped stays as it is, its scale too); so are tokens past cu_q[batch] and requests with
     seq_lens 0.  Bytes behind a request's last row are left as they are.  No two
     requests append to one page in a call (PreparedPageFork sees to that).
     run() launches on the current stream of the cache's device, allocates

@@ -171,8 +171,10 @@ typedef struct PageCompactArgs {
  * NaN values become 0 (INT8) or NaN of either sign (e4m3) and are none of m; infinities count
  * as the largest FP32 number.  A scale that is no positive number counts as
  * that of a new page.  Rows on no page of the pool, past the block table,
- * below row 0 or with a position outside the table are skipped; padding as in
- * TreeAttentionArgs.  No two rows of a launch may lie on the same place, and
+ * below row 0 or with a position outside the table are skipped: what lies there
+ * counts as rows that the page has, so a page of which every new row is skipped
+ * stays as it is, and one whose row 0 is skipped keeps its scale, doubled or not;
+ * padding as in TreeAttentionArgs.  No two rows of a launch may lie on the same place, and
  * no two requests append to one page. */
 typedef struct CacheAppendArgs {
     uint64_t cache, updates, table, cuQ, seqLens, positions, rotation, scale, inverseScale;

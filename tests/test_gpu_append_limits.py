@@ -1,11 +1,11 @@
-"""PreparedCacheAppend where FP32 ends: values that vanish beside a page's scale, and
-infinities in rotated channels.  Byte for byte against the definition in 64 bits,
-as test_gpu_append.py."""
+"""PreparedCacheAppend where FP32 ends: values that vanish beside a page's scale,
+infinities in rotated channels; and rows that are skipped.  Byte for byte against
+the definition in 64 bits, as test_gpu_append.py."""
 import numpy as np
 import pytest
 
 from tests import block_cases as cases
-from tests.test_gpu_append import Appended, DIM
+from tests.test_gpu_append import Appended, BLOCK, DIM
 
 pytestmark = pytest.mark.gpu
 KINDS = ["int8", "e4m3"]
@@ -99,3 +99,59 @@ def test_products_past_the_largest_number(kind, pairs):
     case.x = cases.bf16(case.x)
     case.operator().run()
     case.check(*case.expect())
+
+
+def again(case, new, length, written, size):
+    """The first request's last `new` rows given again, all but `written` with positions outside the rotation; the rows."""
+    import torch
+    from npu_sparse_attn_sharedkv_int8 import PreparedCacheAppend
+    put = lambda a: torch.from_numpy(np.ascontiguousarray(a)).cuda()  # noqa: E731
+    x = cases.bf16(case.rng.standard_normal((new, 1, DIM)) * size)
+    places = np.where(np.arange(new) % 2, -1, len(case.rotation)).astype(np.int32)
+    for row in written:
+        places[row - (length - new)] = row
+    PreparedCacheAppend(case.cache, put(x).to(torch.bfloat16), put(case.table[:1]), put(np.array([0, new], np.int32)),
+                        put(np.array([length], np.int32)), scale=case.scale, rotation=put(case.rotation),
+                        positions=put(places)).run()
+    return x
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("length", [33, 40])
+def test_pages_of_skipped_rows_keep_their_scales(kind, length):
+    """Rows that are in the cache already, given again with positions outside the rotation: nothing changes."""
+    case = Appended(46, [length, 5], [length, 5], kind=kind)
+    case.operator().run()
+    codes, scale = case.expect()
+    case.check(codes, scale)
+    again(case, length - BLOCK, length, [], 50.0)           # the second page's rows, all of them
+    case.check(codes, scale)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("size", [0.1, 40.0])
+def test_rows_behind_skipped_ones(kind, size):
+    """A prompt of which 40 rows are in the cache, given whole: the rest goes behind them, as if given alone."""
+    case = Appended(48, [40, 1], [40, 60], kind=kind)
+    case.operator().run()
+    codes, scale = case.expect()
+    x = again(case, 45, 45, range(40, 45), size)
+    turned = cases.rotated(x[40:].astype(np.float64), case.rotation, np.arange(40, 45), True)
+    cases.append(codes, scale, kind, turned, case.table[:1], [0, 5], [45])
+    case.check(codes, scale)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_a_row_between_skipped_ones(kind):
+    """It is replaced, and all others of the page go over to the scale that it takes."""
+    case = Appended(49, [45, 1], [45, 60], kind=kind)
+    case.operator().run()
+    codes, scale = case.expect()
+    x = again(case, 13, 45, [38], 40.0)
+    page, old = case.table[0, 1], scale.copy()
+    turned = cases.rotated(x[6:7].astype(np.float64), case.rotation, np.array([38]), True)
+    cases.append(codes, scale, kind, turned, case.table[:1], [0, 1], [39])
+    grown = scale[page, 0] / old[page, 0]
+    assert grown > 1
+    codes[page, 7:13] = cases.encode(cases.decode(codes[page, 7:13], kind) / grown, kind)
+    case.check(codes, scale)
