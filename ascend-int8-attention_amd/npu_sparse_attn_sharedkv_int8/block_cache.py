@@ -308,13 +308,13 @@ class PreparedBlockAttention:
         self.case, self.scales, self.out, self.lse = case, (ori_scale, cmp_scale), out, lse
 
     def _rebind_same_geometry(self, case, ori_scale=None, cmp_scale=None, *, output=None, lse_output=None):
-        """Serving fast path: same geometry, new tensors (scales and outputs as before where none are given), under the
+        """Serving fast path: same geometry, new tensors (each scale and output as before where none is given), under the
         constructor's checks."""
         ori_scale = self.scales[0] if ori_scale is None else ori_scale
         cmp_scale = self.scales[1] if cmp_scale is None else cmp_scale
         if _check_inputs(case, ori_scale, cmp_scale) != self.geometry:
             raise ValueError("Rebinding keeps the device and every size of the launch")
-        out, lse = (output, lse_output) if output is not None else (self.out, self.lse)
+        out, lse = self.out if output is None else output, self.lse if lse_output is None else lse_output
         self._check_outputs(out, lse, case, ori_scale, cmp_scale)
         self._bind(case, ori_scale, cmp_scale, out, lse)
 
