@@ -284,25 +284,30 @@ __global__ void __launch_bounds__(THREADS, 4) cache_append(const uint64_t cu_q, 
     // ---- the page's scale ----
     constexpr float LARGEST = CODES == E4M3 ? 448.0f : 127.0f;
     // NaN values do not count, infinities as the largest number.
-    float its = 0.0f, most[EACH];
+    float its = 0.0f, most[EACH], all = 0.0f;    // `most` and `all` keep a NaN
     int begin_row = PAGE_ROWS;                   // first row that is written
     uint32_t odd = 0;                            // rows of the wave with a rotated value that is no number in FP32
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
-        begin_row = min(begin_row, mine[i] ? wave + WAVES * i : PAGE_ROWS);
-        most[i] = 0.0f;                          // keeps a NaN
+        most[i] = 0.0f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) most[i] = __builtin_elementwise_maximum(most[i], mine[i] ? fabsf(y[i][e]) : 0.0f);
-        const bool none = !(most[i] < INFINITY);
-        if (__ballot(none)) {                    // seldom
+        all = __builtin_elementwise_maximum(all, most[i]);
+        begin_row = min(begin_row, mine[i] ? wave + WAVES * i : PAGE_ROWS);
+    }
+    if (__ballot(!(all < INFINITY))) {           // seldom
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            const bool none = !(most[i] < INFINITY);
             odd |= __ballot(none && turned) ? 1u << i : 0u;
             float others = 0.0f;
 #pragma unroll
             for (int e = 0; e < 8; ++e) others = fmaxf(others, turned ? 0.0f : fabsf(y[i][e]));
             most[i] = none ? others : most[i];
         }
-        its = fmaxf(its, most[i]);
     }
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) its = fmaxf(its, most[i]);
     const float still = wave_max(turned ? 0.0f : its), rotated = wave_max(turned ? its : 0.0f);
     if (lane == 0) s.peak[0][wave] = still, s.peak[1][wave] = rotated, s.odd[wave] = odd, s.begin[wave] = begin_row;
     asm volatile("" : "+v"(old));                // read before any wave may store the new one
@@ -398,7 +403,8 @@ __global__ void __launch_bounds__(THREADS, 4) cache_append(const uint64_t cu_q, 
             for (int e = 0; e < 8; ++e) {
                 v[e] = __builtin_fmaf(__builtin_fmaf(-v[e], scale, y[i][e]), reciprocal, v[e]);
                 const float rest = __builtin_fmaf(-v[e], scale, y[i][e]);
-                v[e] = to_odd(v[e], rest < 0.0f ? v[e] > 0.0f : rest > 0.0f && v[e] < 0.0f, rest != 0.0f);
+                const bool apart = (int)(__float_as_uint(rest) ^ __float_as_uint(v[e])) < 0;
+                v[e] = to_odd(v[e], apart & (rest != 0.0f) & (v[e] != 0.0f), rest != 0.0f);
             }
             u32x2 other;
             const bool some = encode(v, true, other);
