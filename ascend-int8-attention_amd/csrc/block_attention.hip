@@ -18,7 +18,8 @@
 // times its mean |q| (normal values' largest of 512 is some 4-5 times), so a unit is
 // at most 2^-14 of that.  What is larger, in rows of which a few channels are, has a
 // third byte: those blocks of 64 channels take one more matrix instruction for each
-// sixteen keys, with that byte made from Q again for each tile.  (With 16 bits for
+// sixteen keys; where LDS has no room for that byte (units of 64 rows have it for one
+// block, of 32 for four) it is made from Q again for each tile.  (With 16 bits for
 // the row's largest a channel of 300 beside normal ones moves scores by 0.03.)  e4m3
 // codes, exact in BF16, run on v_mfma_f32_16x16x32_bf16 against Q as it is.  (Q in
 // two e4m3 terms would spare the conversion, at the same rate, but that matrix
@@ -330,14 +331,20 @@ struct alignas(1024) Shared {
     int8_t tile[2][KEYS * D];          // key rows, their 16-byte chunks XOR-swizzled with the row
     _Float16 p[ROWS * P_STRIDE];       // weights [row][key]
     float factor[ROWS], top[ROWS], sum[PARTS][ROWS], peak[PARTS][ROWS];
-    float mean[PARTS][ROWS], inverse[ROWS];   // INT8: sums of |q|, units of one
     uint32_t far[WAVES];               // INT8: blocks of 64 channels where a row of the wave's has values beyond two terms
     int32_t moved[RT];                 // whether a row tile moved its maximum in this tile
     int32_t scan[3][WAVES];
     int32_t found[6];
     int32_t token[ROWS];               // of the unit's rows, counted in the request
     int32_t place[ROWS];               // their rows of q and out
-    uint64_t query[ROWS];              // INT8: their addresses in q
+};
+// INT8: for rows of Q with values beyond two terms.
+template <int RT>
+struct Beyond {
+    static constexpr int BLOCKS = RT == 1 ? 8 : RT == 2 ? 4 : 1;   // as many as leave two work-groups a CU
+    v4i third[RT][BLOCKS][64];         // third terms of a row tile's first blocks that have some
+    uint64_t query[16 * RT];           // the rows' addresses in q
+    float inverse[16 * RT];            // units of one
 };
 
 template <bool E4M3, int RT>
@@ -351,6 +358,7 @@ __global__ void __launch_bounds__(THREADS, 2) block_attention(const uint64_t cu_
     constexpr int ROWS = S::ROWS, PARTS = S::PARTS;
     constexpr int MIN_TILES = RT == 4 ? 8 : RT; // of an item; 1 to 12 differ little
     __shared__ S s;
+    __shared__ Beyond<RT> beyond;
     const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6), g = lane >> 4, n = lane & 15;
     // The leading arguments are the ones that the first loads need: the build preloads them into SGPRs.  split_arg: the units
     // and, from bit 16 on, the work-groups that the launch has scratch for; 0 where it is not split.
@@ -605,11 +613,11 @@ __global__ void __launch_bounds__(THREADS, 2) block_attention(const uint64_t cu_
             peak = row_max(peak == peak ? peak : INFINITY);   // from here on infinity stands for both
             float mean = row_total(sums[0] + sums[1]);
             if (SHARE) {
-                if (g == 0) s.peak[wave / RT][row] = peak, s.mean[wave / RT][row] = mean;
+                if (g == 0) s.peak[wave / RT][row] = peak, s.sum[wave / RT][row] = mean;
                 lds_barrier();
                 mean = 0.0f;
 #pragma unroll
-                for (int part = 0; part < PARTS; ++part) peak = fmaxf(peak, s.peak[part][row]), mean += s.mean[part][row];
+                for (int part = 0; part < PARTS; ++part) peak = fmaxf(peak, s.peak[part][row]), mean += s.sum[part][row];
                 lds_barrier();
             }
             // Two terms hold 8 times the mean, whatever a few channels have: those go into a third.
@@ -617,7 +625,7 @@ __global__ void __launch_bounds__(THREADS, 2) block_attention(const uint64_t cu_
             q.set(most, softmax2);
             if (__ballot(peak > most)) {               // in all waves of these rows
                 if (wave < RT && g == 0)
-                    s.inverse[row] = q.inverse, s.query[row] = p.q + (uint64_t)(uint32_t)s.place[row] * (D * 2);
+                    beyond.inverse[row] = q.inverse, beyond.query[row] = p.q + (uint64_t)(uint32_t)s.place[row] * (D * 2);
 #pragma unroll
                 for (int j = 0; j < JN; ++j) {
                     float its = 0.0f;
@@ -664,6 +672,15 @@ __global__ void __launch_bounds__(THREADS, 2) block_attention(const uint64_t cu_
                 for (int part = 0; part < PARTS; ++part) far |= s.far[wave % RT + part * RT];
                 far = (uint32_t)uni((int)far);
             }
+        }
+    }
+    if constexpr (!E4M3) {
+        int n = 0;
+        for (uint32_t rest = far; rest && n < Beyond<RT>::BLOCKS; rest &= rest - 1, ++n) {   // seldom
+            if (wave / RT != n % PARTS) continue;
+            const auto *from = gptr<u32x4>(p.q + (uint64_t)(uint32_t)s.place[row] * (D * 2)) + 2 * g + 8 * __builtin_ctz(rest);
+            const u32x4 low = from[0], high = from[1];
+            beyond.third[wave % RT][n][lane] = Query<E4M3>::beyond(low, high, q.inverse);
         }
     }
     // Tiles whose rows all of the unit's tokens see need no masks.
@@ -755,11 +772,17 @@ __global__ void __launch_bounds__(THREADS, 2) block_attention(const uint64_t cu_
                                 w[PAIR * (st >> 3) + kt][i] = (float)(dots[0][kt][i] * 256 + dots[1][kt][i]);
                     __builtin_amdgcn_sched_barrier(0);
                 }
-                for (uint32_t rest = far; rest; rest &= rest - 1) {         // seldom
+                int n = 0;
+                for (uint32_t rest = far; rest; rest &= rest - 1, ++n) {         // seldom
                     const int j = __builtin_ctz(rest);
-                    const auto *from = gptr<u32x4>(s.query[its_row]) + 2 * (lx >> 4) + 8 * j;
-                    const u32x4 low = from[0], high = from[1];
-                    const v4i third = Query<E4M3>::beyond(low, high, s.inverse[its_row]);
+                    v4i third;
+                    if (Beyond<RT>::BLOCKS == 8 || n < Beyond<RT>::BLOCKS) {
+                        third = beyond.third[wave % RT][n][lx];
+                    } else {
+                        const auto *from = gptr<u32x4>(beyond.query[its_row]) + 2 * (lx >> 4) + 8 * j;
+                        const u32x4 low = from[0], high = from[1];
+                        third = Query<E4M3>::beyond(low, high, beyond.inverse[its_row]);
+                    }
 #pragma unroll
                     for (int kt = 0; kt < RT; ++kt) {
                         const v4i code = *(const lds_v4i *)(uintptr_t)((at ^ (uint32_t)(64 * j)) + (uint32_t)(16 * kt * D));
