@@ -772,8 +772,8 @@ __global__ void __launch_bounds__(THREADS, 2) block_attention(const uint64_t cu_
                                 w[PAIR * (st >> 3) + kt][i] = (float)(dots[0][kt][i] * 256 + dots[1][kt][i]);
                     __builtin_amdgcn_sched_barrier(0);
                 }
-                int n = 0;
-                for (uint32_t rest = far; rest; rest &= rest - 1, ++n) {         // seldom
+                for (uint32_t rest = far; rest; rest &= rest - 1) {         // seldom
+                    const int n = __builtin_popcount(far) - __builtin_popcount(rest);
                     const int j = __builtin_ctz(rest);
                     v4i third;
                     if (Beyond<RT>::BLOCKS == 8 || n < Beyond<RT>::BLOCKS) {
