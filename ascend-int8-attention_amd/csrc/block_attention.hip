@@ -8,25 +8,28 @@
 //   out_c = sum_j e^{s_j} scale_j code[j][c] / (e^{sink} + sum_j e^{s_j})
 // in one pass over the keys with a running maximum and sum.  A page's scale goes
 // into the exponent: weights are 2^(s_j + log2 scale_j - m), so that P V runs on
-// the codes as they lie in the cache, no weight is lost beside a page of far
-// larger values, and neither scale costs an instruction for a key.  The sum of
-// e^{s_j} takes a page's weights times 1 / scale_j.
+// the codes as they lie in the cache, a weight beside a page of far larger values
+// loses 2^-33 of the largest e^{s_j} scale_j at most, and neither scale costs an
+// instruction for a key.  The sum of e^{s_j} takes a page's weights times
+// 1 / scale_j.
 //
 // Q K.  INT8 codes run on v_mfma_i32_16x16x64_i8: Q times a power of two of its
 // row becomes whole numbers, off by half of one at most, and the sums are exact.
 // Two signed bytes hold the row's values up to the smaller of its largest and 8
 // times its mean |q| (normal values' largest of 512 is some 4-5 times), so a unit is
-// at most 2^-14 of that.  What is larger, in rows of which a few channels are, has a
-// third byte: those blocks of 64 channels take one more matrix instruction for each
-// sixteen keys; where LDS has no room for that byte (units of 64 rows have it for one
-// block, of 32 for four) it is made from Q again for each tile.  (With 16 bits for
-// the row's largest a channel of 300 beside normal ones moves scores by 0.03.)  e4m3
-// codes, exact in BF16, run on v_mfma_f32_16x16x32_bf16 against Q as it is.  (Q in
-// two e4m3 terms would spare the conversion, at the same rate, but that matrix
-// instruction sums eight products with 13 bits below their largest: scores up to
-// 1e-4 off.)  P V runs on v_mfma_f32_16x16x32_f16: codes are exact in FP16, weights
-// are rounded to its 11 bits (the output has 8); sums are of the weights before
-// rounding.
+// at most 1 / 16256 of that.  What is larger, in rows of which a few channels are,
+// has a third byte: those blocks of 64 channels take one more matrix instruction for
+// each sixteen keys; where LDS has no room for that byte (units of 64 rows have it
+// for one block, of 32 for four) it is made from Q again for each tile.  (With 16
+// bits for the row's largest a channel of 300 beside normal ones moves scores by
+// 0.03.  Two chunks of 1900-2048 tokens take 730 us without such channels, 772 with
+// one block of them, 920 with two and 1907 with eight; launches of few rows 0.35 us
+// for the mean and 0.5 for a block.)  e4m3 codes, exact in BF16, run on v_mfma_f32_16x16x32_bf16
+// against Q as it is.  (Q in two e4m3 terms would spare the conversion, at the same
+// rate, but that matrix instruction sums eight products with 13 bits below their
+// largest: scores up to 1e-4 off.)  P V runs on v_mfma_f32_16x16x32_f16: codes are
+// exact in FP16, weights are rounded to its 11 bits (the output has 8); sums are of
+// the weights before rounding.
 //
 // A unit is 16 RT query rows of one request and KV head (a row is a token and a
 // head, heads innermost), which share every key tile of 64 rows (two pages).  A
@@ -38,16 +41,16 @@
 // joins their items' states.
 //
 // What bounds it.  Few query rows: the cache's bytes, 5.1 TB/s for 16 requests
-// of one token and 8 heads over 32-128 K rows (131-135 us).  64 rows a unit: the
+// of one token and 8 heads over 32-128 K rows (130-138 us).  64 rows a unit: the
 // vector instructions beside the matrix ones (codes to FP16 and the softmax): a wave
-// and INT8 tile counts 513 SQ_INSTS_VALU and 128 SQ_INSTS_MFMA, and the matrix
-// cores are busy for 43 % of the time.  512 tokens of one request over 64 K rows
-// reach 1133-1183 TFLOP/s by the card, a large library FP16 product 1200-1240, and
-// two prompts' chunks of 1900-2048 tokens over 8-16 K rows 1015-1035 (715-730 us).  Between them, split contexts:
-// the states of all items, written and read (up to 67 MB of 64-row units: 32
-// requests of 64 heads over 6-16 K rows 80-85 us, 12-15.5 of them the join), and the launch's chain
-// of round trips (lengths, pages and Q, scales, a tile; the join): one request of
-// 4096 rows takes 12.1 us; in a trace the two kernels take 8.5-9.2 and 3.9.
+// and INT8 tile counts 512 SQ_INSTS_VALU and 128 SQ_INSTS_MFMA, and the matrix
+// cores are busy for 44 % of the time.  512 tokens of one request over 64 K rows
+// reach 1120-1183 TFLOP/s by the card, a large library FP16 product 1200-1240, and
+// two prompts' chunks of 1900-2048 tokens over 8-16 K rows 1010-1035 (715-735 us).
+// Between them, split contexts: the states of all items, written and read (up to
+// 67 MB of 64-row units: 32 requests of 64 heads over 6-16 K rows 79-86 us, 12-15.5
+// of them the join), and the launch's chain of round trips (lengths, pages and Q,
+// scales, a tile; the join): one request of 4096 rows takes 12.5 us; in a trace the two kernels take 9.2 and 4.1.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -219,7 +222,8 @@ __device__ __forceinline__ int wave_upto(int v)
 __device__ __forceinline__ int wave_sum(int v) { return __builtin_amdgcn_readlane(wave_upto(v), 63); }
 
 // Q of a lane's row as the matrix instructions take it: INT8, in two terms of whole numbers relative to a power of two
-// of its own, most significant first (and, made where they are used, third terms above them); e4m3, the first and the last eight of sixteen channels as they are.
+// of its own, most significant first (third terms above them are kept apart); e4m3, the first and the last eight of
+// sixteen channels as they are.
 template <bool E4M3>
 struct Query {
     static constexpr float LARGEST = 127.0f * 256.0f;
@@ -257,8 +261,8 @@ struct Query {
             out[1][q] = __builtin_amdgcn_perm(cd, ab, 0x06040200u) ^ 0x80808080u;
         }
     }
-    // What sixteen channels have beyond the two terms, in 65536 units: at most 32, as no value is more than 512 times the
-    // row's mean and the two terms hold 8 times that or all.
+    // What sixteen channels have beyond the two terms, in 65536 units: at most 32, as no value is more than 512 times
+    // the row's mean and the two terms hold 8 times that or all.
     static __device__ __forceinline__ v4i beyond(const u32x4 &a, const u32x4 &b, float inverse)
     {
         v4i out;
@@ -1098,7 +1102,9 @@ Plan plan_of(const BlockAttentionArgs *a)
                            ((near / PAGE_ROWS < a->oriTableWidth ? near / PAGE_ROWS : a->oriTableWidth) + 1) / 2;
     // Units of 16 rows spread few rows over more work-groups and have the smallest states; units of 64 rows convert a key
     // for more of them, so that the matrix instructions bound them, but split contexts move four times the states.  With R
-    // tiles of 64 rows in a launch and `tiles` of 64 keys in a unit, the better one goes by R * R * tiles, and for units of
+    // tiles of 64 rows in a launch and `tiles` of 64 keys in a unit (by the block tables' width, as lengths are not known
+    // here: tables far wider than the contexts take larger units than these would, 8 requests of 64 heads over 4 K rows
+    // 25.7 us with a table of 4 K rows, 28.4 of 32 K and 39.0 of 128 K), the better one goes by R * R * tiles, and for units of
     // 64 rows by the tiles too (microseconds of 16, 32 and 64 rows a unit):
     //        64  1 request, 64 heads, 4 K      16.6, 18.5, 33.7     131 K  16 of 16 tokens, 8 K         82.3, 64.3, 63.7
     //       4 K  8, 64 heads, 4 K              25.5, 28.9, 38.2     131 K  1 of 128 tokens, 32 K         144,  101, 89.3

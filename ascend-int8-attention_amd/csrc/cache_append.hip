@@ -18,10 +18,11 @@
 // 26.5 us where this takes 18.8: 48 requests of 1-200 rows of four heads.)
 //
 // What bounds it.  1024 bytes read and 512 written for a row and head, beside
-// 185 vector instructions for the codes of a lane's eight values (e4m3 143); with
+// 185 vector instructions for a lane's eight values, all told (e4m3 214); with
 // few rows one chain of round trips (the requests' ends; the rows, their positions and
-// page; the angles and the old scale; the codes).  One row takes 4.1 us, 256
-// requests' 6.4, five prompts of 700-2600 rows 8.1, 65536 rows 31 (3.8 TB/s).  A
+// page; the angles and the old scale; the codes).  One row takes 4.2 us, 256
+// requests' 6.3 (7.0 where each one's scale grows and the page's codes are rounded
+// again), five prompts of 700-2600 rows 8.1, 65536 rows 31 (3.8 TB/s).  A
 // work-group takes a page: the rows that share a scale are in its registers from
 // the first read on, so they are read once and a launch needs no second pass.
 // Eight waves with four rows each: with two rows each 9.9 and 39 us for the last

@@ -74,16 +74,19 @@ class PreparedCacheAppend:
     absolute value and D = 127 or 448, where the page's row 0 is among them, and
     otherwise doubled as often as the new rows need, the codes before them
     rounded to the new scale.  Code = the value / scale to the nearest, ties to
-    even.  NaN is stored as 0 (INT8) or NaN (e4m3) and infinities as the largest
-    value; neither spoils the page's other rows.
+    even.  NaN is stored as 0 (INT8) or NaN (e4m3) and does not touch the page's
+    other rows.  Infinities count as the largest FP32 number, in the page's scale
+    too: its other rows, those before and behind, become zeros beside one (below
+    some 1e36, in e4m3 7e32), until the page is begun anew.
     inverse_scale FP32 [512] (INT8, one head): frozen channel scales, the codes
-    of PreparedCacheWrite.
+    of PreparedCacheWrite (NaN as -127).
 
     Rows on no page of the pool, past the block table or with a position outside
     the rotation are skipped, and what lies there counts as rows that the page has
-    (one whose new rows are all skipped stays as it is, its scale too); so are tokens past cu_q[batch] and requests with
-    seq_lens 0.  Bytes behind a request's last row are left as they are.  No two
-    requests append to one page in a call (PreparedPageFork sees to that).
+    (one whose new rows are all skipped stays as it is, its scale too); so are
+    tokens past cu_q[batch] and requests with seq_lens 0.  Bytes behind a request's
+    last row are left as they are.  No two requests append to one page in a call
+    (PreparedPageFork sees to that).
     run() launches on the current stream of the cache's device, allocates
     nothing, reads nothing back and can be captured.  Codes of a page whose rows
     were appended in several calls depend on how they were divided (by the
@@ -242,7 +245,9 @@ class PreparedBlockAttention:
 
     Rows on pages outside the pool, or past the block table, are masked; what
     masked rows hold (codes, scales, NaN or infinities) reaches no output.  A
-    token that sees no row gets 0 (lse = sink).  Tokens past cu_q[batch], and
+    token that sees no row gets 0 (lse = sink).  INT8 caches hold q to half of
+    min(largest |q|, 8 mean |q|) / 16256 of its row at worst, e4m3 caches as it is;
+    weights have FP16's 11 bits.  Tokens past cu_q[batch], and
     those of requests with seq_lens 0, are graph padding: zero.  cu_q rises from
     0; scales are not negative.
 

@@ -160,16 +160,17 @@ typedef struct PageCompactArgs {
  * Channels 2k and 2k + 1 of the rotated ones turn together where interleaved
  * is 1, else k and k + rotary / 2: a' = a cos - b sin, b' = a sin + b cos.
  * inverseScale (FP32 [512], one KV head, INT8): the codes of launch_cache_write,
- * of the rotated value as FP32.  Otherwise scale FP32 [pages][heads]
- * (scaleStride floats between pages) holds a scale for each page and KV head,
- * and codes are INT8 (codes 0, largest D = 127) or OCP e4m3 (1, D = 448):
+ * of the rotated value as FP32 (NaN becomes -127 there and here).  Otherwise
+ * scale FP32 [pages][heads] (scaleStride floats between pages) holds a scale for
+ * each page and KV head, and codes are INT8 (codes 0, largest D = 127) or OCP e4m3 (1, D = 448):
  *   a page whose row 0 is appended gets scale = max(m / D, 1e-8), m the largest
  *   absolute value of its new rows as FP32; one that has rows keeps its scale,
  *   doubled as often as it takes to reach m / D, and where it is doubled its
  *   codes become round(code / 2^k);
  *   code = round(value / scale), to the nearest, ties to even.
- * NaN values become 0 (INT8) or NaN of either sign (e4m3) and are none of m; infinities count
- * as the largest FP32 number.  A scale that is no positive number counts as
+ * NaN values become 0 (INT8) or NaN of either sign (e4m3) and are none of m;
+ * infinities count as the largest FP32 number, so the page's other rows become
+ * zeros beside one.  A scale that is no positive number counts as
  * that of a new page.  Rows on no page of the pool, past the block table,
  * below row 0 or with a position outside the table are skipped: what lies there
  * counts as rows that the page has, so a page of which every new row is skipped
